@@ -117,10 +117,12 @@ uint64_t snl_launch_count(void);
 
 /* Device error word of the current device: bit 0 = a bounded device-side wait on an
  * asynchronous copy gave up, bit 1 = a tensor-parallel peer did not answer within the
- * wait bound (the kernel returned instead of hanging). Returns the word (>= 0), clearing
- * it when clear != 0, or a negative code. The engine calls (forward_mm, forward_greedy,
- * mtp, generate) read it themselves: a set word makes them fail with SNL_E_TIMEOUT and
- * clears it. */
+ * wait bound (the kernel returned instead of hanging), bit 2 = a paged-cache call met an
+ * index outside of its range. Returns the word (>= 0), clearing it when clear != 0, or a
+ * negative code. The engine calls (forward_mm, forward_greedy, mtp, generate) read what
+ * their own kernels set themselves: they fail with SNL_E_TIMEOUT and clear it. The
+ * paged-cache calls return before their kernels have run and leave their bits (0 and 2)
+ * to the next snl_device_error(). */
 int snl_device_error(int clear);
 
 /* ModelConfig::validate (src/config.rs:194-240). */
@@ -263,6 +265,129 @@ typedef struct snl_sample_p {
 int snl_sample(const snl_sample_p* p, float* logits, uint32_t n, const uint32_t* hist_tok, const uint32_t* hist_cnt,
                uint32_t n_hist, const float* u, int64_t draft, uint32_t* out, void* scratch, void* stream);
 size_t snl_sample_scratch_bytes(void);
+/* ---- kernel level: paged key/value cache --------------------------------------------
+ *
+ * A cache in pages, for hosts that serve many sequences at once (no counterpart in the
+ * reference, whose engine keeps one contiguous cache). A sequence's tokens fill numbered
+ * slots; slot t lies in page table[b][t / page_size] at t % page_size. The four calls are
+ * the steps of serving from it: new rows enter (append), attend over their sequence
+ * (attend), what they looked at is added up per slot (weigh), and a sequence over its
+ * budget keeps its heaviest slots (evict).
+ *
+ * All arrays are device memory. Calls enqueue on `stream`, allocate nothing, wait for
+ * nothing and may be captured in a CUDA graph. Pointers and strides of q, k, v, gate, out
+ * and the pages are aligned to 16 bytes; the last dimension is contiguous. The shapes, types
+ * and host-side bounds are checked before anything is enqueued. What only the device can
+ * see is bounded there: a page number outside the cache, a length over max_len or the
+ * table's pages, a start array that leaves [0, n_rows], a position outside the rotary table. Such an
+ * entry is not read or written, its results are undefined, and bit 2 (value 4) of
+ * snl_device_error() is set. */
+
+/* Element types of q, k, v, gate and out. */
+enum { SNL_T_F32 = 0, SNL_T_F16 = 1, SNL_T_BF16 = 2 };
+
+/* Element (page, KV head, slot, dim) of k and v is at page * page_stride + head *
+ * head_stride + slot * slot_stride + dim (elements), so both [page][head][slot] and
+ * [page][slot][head] pages fit. page_size: a power of two of at least 8. head_dim: 128 or
+ * 256. weight: [n_pages][n_kv][page_size] accumulated attention weights, or NULL. */
+typedef struct snl_paged_cache {
+  void* k;
+  void* v;
+  float* weight;
+  uint64_t page_stride, head_stride, slot_stride;
+  uint32_t type; /* SNL_T_F16 or SNL_T_BF16 */
+  uint32_t n_pages, page_size, n_kv, head_dim, pad;
+} snl_paged_cache;
+
+/* The step's rows: rows start[b] .. start[b + 1] - 1 are the newest tokens of sequence b,
+ * which with them holds len[b] slots; row i of them is at slot len[b] - rows + i. table:
+ * [n_seqs][table_stride] page numbers. max_len: at least every len[b]. */
+typedef struct snl_paged_batch {
+  const int32_t* table;
+  const int32_t* start; /* [n_seqs + 1], start[0] = 0, start[n_seqs] = n_rows */
+  const int32_t* len;   /* [n_seqs] */
+  uint32_t n_seqs, n_rows, table_stride, max_len;
+} snl_paged_batch;
+
+/* The rotary table of snl_paged_append: table[pos][f] = (cos, sin) of pos *
+ * theta^(-2f / rot_dim), f < rot_dim / 2, angles in 64 bits. table: [n_pos][rot_dim / 2][2]. */
+int snl_rope_table(double theta, uint32_t rot_dim, uint32_t n_pos, float* table, void* stream);
+
+/* Which axis of a row's position (time, height, width) turns pair f. */
+enum {
+  SNL_ROPE_ONE = 0,        /* time only (text)                                            */
+  SNL_ROPE_SECTIONS = 1,   /* sections[0] pairs of time, then height, then width          */
+  SNL_ROPE_INTERLEAVED = 2 /* f % 3 == 1 and f < 3 sections[1]: height; f % 3 == 2 and
+                              f < 3 sections[2]: width; else time (as snl_attn_prep)      */
+};
+/* Which elements form pair f: (f, f + rot_dim / 2), or (2f, 2f + 1). */
+enum { SNL_ROPE_HALVES = 0, SNL_ROPE_ADJACENT = 1 };
+
+/* Strides in elements of row and head; q, k and v have in_type (f32, or the cache's). */
+typedef struct snl_paged_append_p {
+  uint32_t n_heads, in_type, rot_dim, axes, pairs, n_pos;
+  uint32_t sections[3];
+  float eps;
+  uint64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+} snl_paged_append_p;
+
+/* New rows enter the cache: q and k are normed (x / rms(x) * (1 + norm), where the norm is
+ * given), their first rot_dim elements turned by rope at pos, and rounded once to the
+ * cache's type; k and v go to the rows' slots, q to q_out [n_rows][n_heads][head_dim].
+ * pos: [n_rows][4] u32 (time, height, width, 0). q and q_out may both be NULL (n_heads 0);
+ * rot_dim 0 turns nothing. */
+int snl_paged_append(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_append_p* p, const void* q,
+                     const void* k, const void* v, const float* q_norm, const float* k_norm, const uint32_t* pos,
+                     const float* rope, void* q_out, void* stream);
+
+/* Row r of sequence b, at slot t, sees the keys of [max(first[r], t + 1 - window),
+ * min(len[b], max(t + 1, last[r]))): first gives documents and padding (a row whose first
+ * key is past its last sees nothing), last the end of a prefix or of an image block that
+ * is seen both ways. window 0, first NULL and last NULL leave that part out. A score is
+ * s = scale q.k, then cap * tanh(s / cap) when cap > 0, then s - slopes[h] * |t - key| when
+ * slopes ([n_heads]) is given. Distances count slots. */
+typedef struct snl_paged_attn_p {
+  const float* slopes;
+  const int32_t* first; /* [n_rows] */
+  const int32_t* last;  /* [n_rows] */
+  uint32_t n_heads, window;
+  float scale, cap;
+  uint32_t gate_type, out_type;
+  uint64_t q_row, q_head, gate_row, gate_head, out_row, out_head;
+} snl_paged_attn_p;
+
+/* out[r][h] = sum over the keys of softmax(s) v, times sigmoid(gate[r][h]) where gate is
+ * given; n_heads is a multiple of n_kv (at most 64 times), and query head h reads KV head
+ * h / (n_heads / n_kv). q has the cache's type, gate and out any. lse (or NULL):
+ * [n_rows][n_heads] log-sum-exp of the scores. A row that sees no key (or only scores of
+ * -inf) gives 0 and -inf. What a row does not see never reaches it, NaN and infinities
+ * included. Single tokens, chunks and mixtures of both; long caches are split over the GPU
+ * and joined in `work`, work_bytes of scratch (snl_paged_attend_workspace() of them, with
+ * the same structs, suffice) that concurrent calls may not share. */
+int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_attn_p* p, const void* q,
+                     const void* gate, void* out, float* lse, void* work, size_t work_bytes, void* stream);
+size_t snl_paged_attend_workspace(const snl_paged_cache* c, const snl_paged_batch* b, uint32_t n_heads);
+
+/* Accumulated attention weight: for each slot t of each sequence and each KV head,
+ * weight = decay * weight + sum over the step's rows and the head's group of exp(s - lse),
+ * over the rows that see t, with the lse of snl_paged_attend. The step's own slots start at
+ * 0; decay 0 does not read the old weights. gate and out of p are not used. */
+int snl_paged_weigh(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_attn_p* p, const void* q,
+                    const float* lse, float decay, void* stream);
+
+/* Thins sequences of more than `budget` slots to `budget`: per KV head, the first `sink`,
+ * the last `recent` and the heaviest others (equal weights: the lowest slot first; NaN as
+ * -inf) move, in order, with k, v and weight, to slots 0, 1, .. of the pages into
+ * [n_seqs][into_stride]; shorter sequences move whole. into == NULL: in place, in the
+ * batch's own pages. Otherwise the new pages and every page of the batch are distinct.
+ * new_len[b] = min(len[b], budget) (it may be the batch's own len in place). kept:
+ * [n_seqs][n_kv][budget], the slots that were kept, then -1. The batch's start is not used. */
+typedef struct snl_paged_evict_p {
+  uint32_t budget, sink, recent, into_stride;
+} snl_paged_evict_p;
+int snl_paged_evict(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_evict_p* p, int32_t* kept,
+                    const int32_t* into, int32_t* new_len, void* stream);
+
 /* ---- seeded synthetic tensors ------------------------------------------------------- */
 
 /* Fill device buffers with tensor `name` of the seeded synthetic model (the benchmark

@@ -114,6 +114,9 @@ constexpr int kRpStride = 12;
 
 // Device address of the library's device error word (bit 0: a bounded wait gave up).
 int device_error_word(int** out);
+// The paged-cache kernels' own word (bit 0: a bounded wait gave up; bit 2: an index that
+// only the device sees was out of range). Both words are read by snl_device_error().
+int paged_error_word(int** out);
 
 // Launches with programmatic stream serialization (unless SNL_NO_PDL is set): the
 // kernel may begin while the previous kernel on the stream finishes. Every kernel

@@ -23,22 +23,33 @@ namespace snl {
 // by snl_device_error().
 __device__ int g_dev_error;
 
-// Device address of g_dev_error on the current device, for kernels in other files
+// The same of the paged-cache kernels, which no engine call reads.
+__device__ int g_paged_error;
+
+// Device address of an error word on the current device, for kernels in other files
 // (looked up once per device).
-int device_error_word(int** out) {
-  static int* addr[64] = {nullptr};
+template <typename Sym>
+static int error_word(int** out, int* (&addr)[64], Sym& sym, const char* what) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (dev < 0 || dev >= 64) return fail(SNL_E_INVALID, "device ordinal out of range");
   if (!addr[dev]) {
     void* p = nullptr;
-    e = cudaGetSymbolAddress(&p, g_dev_error);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(g_dev_error)");
+    e = cudaGetSymbolAddress(&p, sym);
+    if (e != cudaSuccess) return cuda_fail(e, what);
     addr[dev] = static_cast<int*>(p);
   }
   *out = addr[dev];
   return SNL_OK;
+}
+int device_error_word(int** out) {
+  static int* addr[64] = {nullptr};
+  return error_word(out, addr, g_dev_error, "cudaGetSymbolAddress(g_dev_error)");
+}
+int paged_error_word(int** out) {
+  static int* addr[64] = {nullptr};
+  return error_word(out, addr, g_paged_error, "cudaGetSymbolAddress(g_paged_error)");
 }
 
 bool pdl_on() {
@@ -564,14 +575,14 @@ int launch_mat(int dtype, StepRef st, const snl_mat_p& p, const float* x, const 
 }  // namespace snl
 
 extern "C" int snl_device_error(int clear) {
-  int v = 0;
+  int v = 0, pv = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, snl::g_dev_error, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&pv, snl::g_paged_error, sizeof(int));
   if (e != cudaSuccess) return snl::cuda_fail(e, "snl_device_error");
-  if (clear && v) {
-    const int z = 0;
-    cudaMemcpyToSymbol(snl::g_dev_error, &z, sizeof(int));
-  }
-  return v;
+  const int z = 0;
+  if (clear && v) cudaMemcpyToSymbol(snl::g_dev_error, &z, sizeof(int));
+  if (clear && pv) cudaMemcpyToSymbol(snl::g_paged_error, &z, sizeof(int));
+  return v | pv;
 }
 
 extern "C" int snl_mat(int dtype, const snl_step_u* step, const snl_mat_p* p, const float* x, const void* wq,

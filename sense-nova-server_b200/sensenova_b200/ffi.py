@@ -28,6 +28,9 @@ SNL_FINISH_STOP, SNL_FINISH_LENGTH = 0, 1
 SNL_WORKER_SNAPSHOTS = 4
 SNL_VIS_HEAD_DIM = 72
 SNL_VIS_ACT_GELU_TANH, SNL_VIS_ACT_GELU_ERF = 1, 2
+SNL_T_F32, SNL_T_F16, SNL_T_BF16 = 0, 1, 2
+SNL_ROPE_ONE, SNL_ROPE_SECTIONS, SNL_ROPE_INTERLEAVED = 0, 1, 2
+SNL_ROPE_HALVES, SNL_ROPE_ADJACENT = 0, 1
 MAX_LAYERS = 256
 
 
@@ -97,6 +100,40 @@ class VisionConfigC(C.Structure):
     """snl_vision_config (VisionConfig, config.rs:40-70)."""
     _fields_ = [(n, C.c_uint32) for n in ("hidden", "intermediate", "intermediate_padded", "depth", "n_heads", "patch",
                                           "temporal_patch", "merge", "out_hidden", "pos_side")]
+
+
+class PagedCacheC(C.Structure):
+    """snl_paged_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("weight", C.c_void_p), ("page_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("slot_stride", C.c_uint64),
+                *((n, C.c_uint32) for n in ("type", "n_pages", "page_size", "n_kv", "head_dim", "pad"))]
+
+
+class PagedBatchC(C.Structure):
+    """snl_paged_batch."""
+    _fields_ = [("table", C.c_void_p), ("start", C.c_void_p), ("len", C.c_void_p),
+                *((n, C.c_uint32) for n in ("n_seqs", "n_rows", "table_stride", "max_len"))]
+
+
+class PagedAppendP(C.Structure):
+    """snl_paged_append_p."""
+    _fields_ = [*((n, C.c_uint32) for n in ("n_heads", "in_type", "rot_dim", "axes", "pairs", "n_pos")),
+                ("sections", C.c_uint32 * 3), ("eps", C.c_float),
+                *((n, C.c_uint64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row",
+                                            "out_head"))]
+
+
+class PagedAttnP(C.Structure):
+    """snl_paged_attn_p."""
+    _fields_ = [("slopes", C.c_void_p), ("first", C.c_void_p), ("last", C.c_void_p), ("n_heads", C.c_uint32),
+                ("window", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float), ("gate_type", C.c_uint32),
+                ("out_type", C.c_uint32),
+                *((n, C.c_uint64) for n in ("q_row", "q_head", "gate_row", "gate_head", "out_row", "out_head"))]
+
+
+class PagedEvictP(C.Structure):
+    """snl_paged_evict_p."""
+    _fields_ = [(n, C.c_uint32) for n in ("budget", "sink", "recent", "into_stride")]
 
 
 # Callback types of snl_worker_ops and snl_gen_request (include/snl_b200.h).
@@ -181,6 +218,12 @@ SIGNATURES = {
     "snl_conv_delta": (i32, [P(StepU), P(LinP), vp, vp, vp, vp, vp, vp, vp, vp]),
     "snl_argmax": (i32, [vp, u32, u32, vp, vp]),
     "snl_argmax_noalloc": (i32, [vp, u32, u32, vp, vp]),
+    "snl_rope_table": (i32, [C.c_double, u32, u32, vp, vp]),
+    "snl_paged_append": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedAppendP), *[vp] * 9]),
+    "snl_paged_attend": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedAttnP), *[vp] * 5, sz, vp]),
+    "snl_paged_attend_workspace": (sz, [P(PagedCacheC), P(PagedBatchC), u32]),
+    "snl_paged_weigh": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedAttnP), vp, vp, C.c_float, vp]),
+    "snl_paged_evict": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedEvictP), vp, vp, vp, vp]),
     "snl_synth_quant": (i32, [u64, C.c_char_p, i32, sz, sz, vp, vp, vp]),
     "snl_synth_f32": (i32, [u64, C.c_char_p, u32, sz, C.c_float, C.c_float, vp, vp]),
     "snl_engine_create": (i32, [P(ModelConfigC), sz, i32, u32, P(vp)]),

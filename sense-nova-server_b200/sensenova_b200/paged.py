@@ -1,0 +1,195 @@
+"""The paged key/value cache (snl_paged_* of include/snl_b200.h) for hosts that serve many
+sequences at once: new rows enter the pages, attend over their sequence, the attention
+weight of each slot is added up, and sequences over a budget keep their heaviest slots.
+
+Arguments are device tensors: anything with data_ptr(), shape, stride() and dtype, as
+torch.Tensor has. The caller owns every tensor; calls enqueue on `stream` (a CUDA stream
+handle; 0 is the default stream) and return, and the tensors have to live until that work
+is done. SnlError says what a call refuses; snl_device_error() what only the device saw.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Any
+
+from . import ffi
+from .ffi import PagedAppendP, PagedAttnP, PagedBatchC, PagedCacheC, PagedEvictP, SnlError
+
+ONE, SECTIONS, INTERLEAVED = 0, 1, 2  # which axis of a position turns which pair
+HALVES, ADJACENT = 0, 1  # which elements form a pair
+_TYPES = {"float32": ffi.SNL_T_F32, "float16": ffi.SNL_T_F16, "bfloat16": ffi.SNL_T_BF16}
+_type_of: dict[Any, int] = {}
+
+
+def _type(t) -> int:
+    """SNL_T_* of a tensor."""
+    code = _type_of.get(t.dtype)
+    if code is None:
+        name = str(t.dtype).rsplit(".", 1)[-1]
+        if name not in _TYPES:
+            raise SnlError(ffi.SNL_E_UNSUPPORTED, f"paged cache: tensors of {name}")
+        code = _type_of[t.dtype] = _TYPES[name]
+    return code
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise SnlError(ffi.SNL_E_INVALID, "paged cache: " + what)
+
+
+def _ints(t, what: str, *shape: int):
+    """A contiguous tensor of 32-bit integers of that shape; its address."""
+    _need(tuple(t.shape) == shape and str(t.dtype).endswith("int32") and t.is_contiguous(),
+          f"{what} must be contiguous 32-bit integers of shape {shape}")
+    return t.data_ptr()
+
+
+def _floats(t, what: str, *shape: int):
+    if t is None:
+        return None
+    _need(tuple(t.shape) == shape and _type(t) == ffi.SNL_T_F32 and t.is_contiguous(),
+          f"{what} must be contiguous float32 of shape {shape}")
+    return t.data_ptr()
+
+
+class PagedBatch:
+    """One step's rows: rows start[b] .. start[b + 1] - 1 are the newest tokens of sequence
+    b, whose slots lie in the pages table[b] and number lens[b] with them. table [seqs,
+    pages], start [seqs + 1] and lens [seqs] are int32 on the device and may change between
+    calls; n_rows and max_len (at least every length) are the host's."""
+
+    def __init__(self, table, start, lens, n_rows: int, max_len: int):
+        seqs, width = table.shape
+        self.tensors = (table, start, lens)
+        self.n_seqs, self.n_rows, self.max_len = seqs, n_rows, max_len
+        self.c = PagedBatchC(_ints(table, "table", seqs, width), _ints(start, "start", seqs + 1),
+                             _ints(lens, "lens", seqs), seqs, n_rows, width, max_len)
+        self.ref = C.byref(self.c)
+
+
+class PagedCache:
+    """Pages of keys and values [pages, kv heads, slots, head_dim] in f16 or bf16, as views of
+    either layout, and their accumulated attention weights [pages, kv heads, slots] in f32."""
+
+    def __init__(self, k, v, weight=None):
+        self.lib = ffi.load()
+        pages, n_kv, slots, d = k.shape
+        _need(tuple(v.shape) == tuple(k.shape) and v.stride() == k.stride() and v.dtype == k.dtype,
+              "k and v must have the same shape, strides and type")
+        _need(k.stride(3) == 1, "the last dimension must be contiguous")
+        self.type, self.n_kv, self.head_dim, self.page_size = _type(k), n_kv, d, slots
+        self.tensors = (k, v, weight)
+        self.c = PagedCacheC(k.data_ptr(), v.data_ptr(), _floats(weight, "weight", pages, n_kv, slots), k.stride(0),
+                             k.stride(1), k.stride(2), self.type, pages, slots, n_kv, d, 0)
+        self.ref = C.byref(self.c)
+
+    def _rows(self, t, what: str, batch: PagedBatch, heads: int) -> tuple[int, int, int]:
+        _need(tuple(t.shape) == (batch.n_rows, heads, self.head_dim) and t.stride(2) == 1,
+              f"{what} must be [{batch.n_rows}, {heads}, {self.head_dim}] with a contiguous last dimension")
+        return t.data_ptr(), t.stride(0), t.stride(1)
+
+    def append(self, batch: PagedBatch, q, k, v, q_out, pos=None, rope=None, *, axes: int = ONE, pairs: int = HALVES,
+               sections=(0, 0, 0), q_norm=None, k_norm=None, eps: float = 1e-6, stream: int = 0) -> None:
+        """New rows enter the cache (snl_paged_append). q [rows, heads, d] or None, k and v
+        [rows, kv heads, d] in f32 or the cache's type, any row and head strides; q_out like
+        q in the cache's type. pos [rows, 4] 32-bit integers (time, height, width, 0) and
+        rope [positions, rot / 2, 2] turn the first rot elements; None turns nothing."""
+        d = self.head_dim
+        p = PagedAppendP()
+        kp, p.k_row, p.k_head = self._rows(k, "k", batch, self.n_kv)
+        vp, p.v_row, p.v_head = self._rows(v, "v", batch, self.n_kv)
+        qp = op = None
+        p.in_type = _type(k)
+        _need(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k and v must have one type")
+        if q is not None:
+            p.n_heads = q.shape[1]
+            qp, p.q_row, p.q_head = self._rows(q, "q", batch, q.shape[1])
+            op, p.out_row, p.out_head = self._rows(q_out, "q_out", batch, q.shape[1])
+            _need(_type(q_out) == self.type, "q_out must have the cache's type")
+        tp = rp = None
+        if rope is not None:
+            n, half, two = rope.shape
+            _need(two == 2 and pos is not None, "rope must be [positions, rot / 2, 2] and pos be given")
+            p.rot_dim, p.n_pos = 2 * half, n
+            rp, tp = _floats(rope, "rope", n, half, 2), _ints(pos, "pos", batch.n_rows, 4)
+        p.axes, p.pairs, p.eps = axes, pairs, eps
+        p.sections[0], p.sections[1], p.sections[2] = sections
+        rc = self.lib.snl_paged_append(self.ref, batch.ref, C.byref(p), qp, kp, vp, _floats(q_norm, "q_norm", d),
+                                       _floats(k_norm, "k_norm", d), tp, rp, op, stream)
+        if rc:
+            ffi.check(rc)
+
+    def _attn(self, batch: PagedBatch, q, scale, cap, window, slopes, first, last) -> tuple[PagedAttnP, int]:
+        p = PagedAttnP()
+        heads = q.shape[1]
+        qp, p.q_row, p.q_head = self._rows(q, "q", batch, heads)
+        _need(_type(q) == self.type, "q must have the cache's type")
+        p.n_heads, p.window, p.cap = heads, window, cap
+        p.scale = self.head_dim ** -0.5 if scale is None else scale
+        if slopes is not None:
+            p.slopes = _floats(slopes, "slopes", heads)
+        if first is not None:
+            p.first = _ints(first, "first", batch.n_rows)
+        if last is not None:
+            p.last = _ints(last, "last", batch.n_rows)
+        return p, qp
+
+    def attend_workspace(self, batch: PagedBatch, heads: int) -> int:
+        """Bytes of scratch that attend needs for such a batch."""
+        return self.lib.snl_paged_attend_workspace(self.ref, batch.ref, heads)
+
+    def attend(self, batch: PagedBatch, q, out, work, *, lse=None, gate=None, scale: float | None = None,
+               cap: float = 0.0, window: int = 0, slopes=None, first=None, last=None, stream: int = 0) -> None:
+        """The rows attend over their sequences (snl_paged_attend): q [rows, heads, d] in the
+        cache's type, out and gate like it in any type, lse [rows, heads] f32, work a
+        contiguous tensor of scratch bytes. first, last [rows] int32 and slopes [heads] f32
+        are the masks and the distance bias; scale is 1 / sqrt(d) unless given."""
+        p, qp = self._attn(batch, q, scale, cap, window, slopes, first, last)
+        op, p.out_row, p.out_head = self._rows(out, "out", batch, p.n_heads)
+        p.out_type = _type(out)
+        gp = None
+        if gate is not None:
+            gp, p.gate_row, p.gate_head = self._rows(gate, "gate", batch, p.n_heads)
+            p.gate_type = _type(gate)
+        rc = self.lib.snl_paged_attend(self.ref, batch.ref, C.byref(p), qp, gp, op,
+                                       _floats(lse, "lse", batch.n_rows, p.n_heads), work.data_ptr(),
+                                       work.numel() * work.element_size(), stream)
+        if rc:
+            ffi.check(rc)
+
+    def weigh(self, batch: PagedBatch, q, lse, *, decay: float = 1.0, scale: float | None = None, cap: float = 0.0,
+              window: int = 0, slopes=None, first=None, last=None, stream: int = 0) -> None:
+        """weight = decay * weight + what the rows' attention (with attend's lse) gave each
+        slot, per KV head (snl_paged_weigh)."""
+        p, qp = self._attn(batch, q, scale, cap, window, slopes, first, last)
+        rc = self.lib.snl_paged_weigh(self.ref, batch.ref, C.byref(p), qp,
+                                      _floats(lse, "lse", batch.n_rows, p.n_heads), decay, stream)
+        if rc:
+            ffi.check(rc)
+
+    def evict(self, batch: PagedBatch, budget: int, kept, into=None, new_lens=None, *, sink: int = 0, recent: int = 0,
+              stream: int = 0) -> None:
+        """Sequences of more than `budget` slots keep `budget` per KV head (snl_paged_evict):
+        the first sink, the last recent and the heaviest others, moved in order to the pages
+        into [seqs, pages], or in place. kept [seqs, kv heads, budget] and new_lens [seqs]
+        receive the kept slots and the lengths; in place new_lens defaults to the batch's."""
+        seqs = batch.n_seqs
+        p = PagedEvictP(budget, sink, recent, 0)
+        ip = None
+        if into is not None:
+            p.into_stride = into.shape[1]
+            ip = _ints(into, "into", seqs, into.shape[1])
+            _need(new_lens is not None, "new_lens is needed with new pages")
+        lp = batch.c.len if new_lens is None else _ints(new_lens, "new_lens", seqs)
+        rc = self.lib.snl_paged_evict(self.ref, batch.ref, C.byref(p), _ints(kept, "kept", seqs, self.n_kv, budget), ip,
+                                      lp, stream)
+        if rc:
+            ffi.check(rc)
+
+
+def rope_table(out, theta: float, stream: int = 0) -> None:
+    """Fill out [positions, rot / 2, 2] with (cos, sin) of pos * theta^(-2f / rot)
+    (snl_rope_table)."""
+    n, half, two = out.shape
+    _need(two == 2, "rope must be [positions, rot / 2, 2]")
+    ffi.check(ffi.load().snl_rope_table(theta, 2 * half, n, _floats(out, "rope", n, half, 2), stream))

@@ -1,0 +1,545 @@
+"""The paged-cache operators on the GPU against their definitions in 64 bits."""
+import math
+
+import pytest
+
+from sensenova_b200 import ffi, paged
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+import paged_ref as ref  # noqa: E402
+from paged_ref import Problem  # noqa: E402
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _clean(torch_cuda, lib):
+    torch.cuda.synchronize()
+    lib.snl_device_error(1)
+    yield
+    torch.cuda.synchronize()
+    assert lib.snl_device_error(1) == 0
+
+
+def run_attend(p, q=None, gate=None, out_dtype=None, lse=True, stream=0, **masks):
+    q = p.q if q is None else q
+    cache, batch = p.cache(paged), p.batch(paged)
+    out = torch.full((p.n, p.heads, p.d), math.nan, dtype=out_dtype or p.dtype, device="cuda")
+    z = torch.full((p.n, p.heads), math.nan, device="cuda") if lse else None
+    work = torch.full((cache.attend_workspace(batch, p.heads),), 0xAB, dtype=torch.uint8, device="cuda")
+    cache.attend(batch, q, out, work, lse=z, gate=gate, stream=stream, **masks)
+    return out, z
+
+
+def check_attend(p, q=None, gate=None, out_dtype=None, **masks):
+    q = p.q if q is None else q
+    out, lse = run_attend(p, q, gate, out_dtype, **masks)
+    want, z, tol, ltol = ref.attend(p, q, gate, out_dtype=out_dtype, **masks)
+    assert torch.equal(torch.isneginf(lse), torch.isneginf(z))
+    assert ((lse.double() - z).abs().nan_to_num(0) <= ltol).all()
+    off = (out.double() - want).abs() - tol
+    assert (off <= 0).all(), float(off.max())
+    return out, lse
+
+
+SHAPES = [  # heads, kv, d, page, layout, type
+    (4, 1, 256, 16, "head", F16), (16, 4, 256, 64, "slot", F16), (32, 8, 128, 32, "head", BF16),
+    (6, 2, 256, 8, "slot", BF16), (20, 4, 128, 128, "head", F16), (8, 8, 256, 16, "slot", BF16),
+    (32, 1, 128, 16, "slot", F16), (64, 1, 256, 256, "head", F16),
+]
+
+
+@pytest.mark.parametrize("heads,kv,d,page,layout,dtype", SHAPES)
+@pytest.mark.parametrize("lens,rows", [
+    ([1], [1]), ([129], [1]), ([7, 300, 64, 1], [1, 1, 1, 1]), ([40], [40]), ([500, 63, 130], [37, 63, 2]),
+])
+def test_attend_shapes(heads, kv, d, page, layout, dtype, lens, rows):
+    check_attend(Problem(lens, rows, heads, kv, d, page, layout, dtype, seed=len(lens) + heads))
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 127, 128, 129, 255, 256, 257, 1000])
+@pytest.mark.parametrize("rows", [1, 31, 33])
+def test_attend_lengths(n, rows):
+    check_attend(Problem([n], [min(rows, n)], seed=n))
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attend_long(d, rows):
+    """Keys split over the GPU and joined; the sums over keys are longer, so is their share."""
+    p = Problem([5000, 9000, 130], [rows, rows, 1], 8, 2, d, 64, seed=d)
+    check_attend(p)
+
+
+MASKS = {
+    "cap": dict(cap=5.0),
+    "slopes": dict(slopes=True),
+    "window": dict(window=50),
+    "window 1": dict(window=1),
+    "docs": dict(docs=70),
+    "blocks": dict(block=48),
+    "prefix": dict(prefix=90),
+    "empty rows": dict(empty=True),
+    "all": dict(cap=20.0, slopes=True, window=100, docs=130, block=30, empty=True),
+    "scale": dict(scale=-0.11),
+}
+
+
+def masks_of(p, cap=0.0, slopes=False, window=0, docs=0, block=0, prefix=0, empty=False, scale=None):
+    t = p.slot()
+    first = last = None
+    if docs:
+        first = t // docs * docs
+    if empty:
+        first = torch.zeros_like(t) if first is None else first
+        first = torch.where(torch.arange(len(t)) % 5 == 2, 2**31 - 1, first)
+    if block:
+        last = (t // block + 1) * block
+    if prefix:
+        last = torch.full_like(t, prefix)
+    m = dict(cap=cap, window=window)
+    if slopes:
+        m["slopes"] = torch.tensor([2.0 ** (-8 * (h + 1) / p.heads) for h in range(p.heads)], device="cuda")
+    if first is not None:
+        m["first"] = first.to(torch.int32).cuda()
+    if last is not None:
+        m["last"] = last.to(torch.int32).cuda()
+    if scale is not None:
+        m["scale"] = scale
+    return m
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("d,rows", [(256, [37, 150, 1]), (128, [37, 150, 1]), (256, [1, 1, 1])])
+def test_attend_masks(mask, d, rows):
+    p = Problem([300, 150, 77], rows, 8, 2, d, 16, seed=d + rows[0])
+    check_attend(p, **masks_of(p, **MASKS[mask]))
+
+
+def test_attend_nothing_seen():
+    p = Problem([200, 40], [70, 1], seed=3)
+    out, lse = run_attend(p, first=torch.full((p.n,), 2**31 - 1, dtype=torch.int32, device="cuda"))
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_attend_empty_sequences():
+    """Sequences without rows, without slots, and a batch without rows."""
+    p = Problem([0, 40, 300, 0, 17], [0, 0, 33, 0, 1], 8, 2, seed=4)
+    check_attend(p)
+    p = Problem([0, 40], [0, 0], seed=4)
+    out, lse = run_attend(p)
+    assert out.shape[0] == 0
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_attend_hides_what_is_not_seen(rows):
+    """NaN and infinities in keys and values that a row does not see leave it as it is: before
+    the window, before the document, after its own slot (where later rows do see them)."""
+    p = Problem([400], [rows], 8, 2, seed=5)
+    pg, sl = p.where(0)
+    m = masks_of(p, window=90)
+    clean, _ = run_attend(p, **m)
+    low = 400 - rows - 89  # below every row's window
+    p.k[pg[:low - 1], :, sl[:low - 1]] = math.inf
+    p.v[pg[:low - 1], :, sl[:low - 1]] = math.nan
+    p.v[pg[low - 1], 0, sl[low - 1], 7] = -math.inf
+    assert torch.equal(run_attend(p, **m)[0], clean)
+    if rows > 1:
+        at = 360  # rows 0..59 are before it
+        for bad in (math.nan, math.inf):
+            p.v[pg[at], 1, sl[at], 9] = bad
+            out, _ = run_attend(p, **m)
+            assert torch.equal(out[:60], clean[:60])
+            same = torch.ones(8, 256, dtype=torch.bool)
+            same[4:, 9] = False
+            assert torch.equal(out[60:][:, same], clean[60:][:, same])
+            hit = out[60:, 4:, 9]
+            assert (hit.isnan() if math.isnan(bad) else hit == math.inf).all()
+        p.k[pg[at], 0, sl[at], 3] = math.nan
+        out, _ = run_attend(p, **m)
+        assert torch.equal(out[:60], clean[:60]) and out[60:, :4].isnan().all()
+
+
+def test_attend_nan_in_own_rows():
+    """A NaN query gives NaN in its own row and head only."""
+    p = Problem([300], [64], 8, 2, seed=6)
+    clean, z = run_attend(p)
+    q = p.q.clone()
+    q[10, 3, 5] = math.nan
+    out, lse = run_attend(p, q)
+    assert out[10, 3].isnan().all() and lse[10, 3].isnan()
+    keep = torch.ones(64, 8, dtype=torch.bool)
+    keep[10, 3] = False
+    assert torch.equal(out[keep], clean[keep]) and torch.equal(lse[keep], z[keep])
+
+
+@pytest.mark.parametrize("size", [1e-4, 60.0, 3e3])
+def test_attend_large_and_small_scores(size):
+    """Scores near zero, scores that leave one key, and scores of thousands."""
+    p = Problem([333], [45], 4, 1, seed=7, peak=1.0)
+    q = (p.q.float() * size).to(F16)
+    check_attend(p, q)
+
+
+@pytest.mark.parametrize("gate_dtype", [F16, F32])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attend_strides_gate_types(gate_dtype, rows):
+    """q, gate and out as parts of wider rows; f32 gate and out."""
+    p = Problem([200, 90], [rows, rows], 8, 2, seed=8)
+    wide = p.normal(p.n, 8, 2, 264).to(F16)
+    q = wide[:, :, 0, 8:]
+    gate = p.normal(p.n, 8, 512).to(gate_dtype)[:, :, 256:]
+    check_attend(p, q, gate)
+    cache, batch = p.cache(paged), p.batch(paged)
+    out = torch.full((8, p.n, 260), math.nan, device="cuda").transpose(0, 1)
+    work = torch.empty(cache.attend_workspace(batch, 8), dtype=torch.uint8, device="cuda")
+    cache.attend(batch, q, out[:, :, :256], work, gate=gate)
+    want, _, tol, _ = ref.attend(p, q, gate, out_dtype=F32)
+    assert ((out[:, :, :256].double() - want).abs() <= tol).all()
+    assert out[:, :, 256:].isnan().all()
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_attend_same_bits_every_time(rows):
+    p = Problem([3000, 700], [rows, rows], 8, 2, seed=9)
+    a, z = run_attend(p)
+    for _ in range(3):
+        b, y = run_attend(p)
+        assert torch.equal(a, b) and torch.equal(z, y)
+
+
+def test_attend_other_stream_and_graph():
+    p = Problem([1500, 64], [1, 1], 8, 2, seed=10)
+    a, _ = run_attend(p)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b, _ = run_attend(p, stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(a, b)
+    cache, batch = p.cache(paged), p.batch(paged)
+    out = torch.zeros_like(a)
+    work = torch.empty(cache.attend_workspace(batch, 8), dtype=torch.uint8, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        cache.attend(batch, p.q, out, work, stream=torch.cuda.current_stream().cuda_stream)
+    p.len_t[0] -= 5  # lengths are the device's: a replay sees the new ones
+    p.lens[0] -= 5
+    g.replay()
+    want, _, tol, _ = ref.attend(p, p.q)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_attend_far_pages():
+    """Pages past 2^32 elements of the pool."""
+    pages = 2**32 // (64 * 256) + 40
+    p = Problem([200], [20], 4, 1, 256, 64, seed=11)
+    k, v = (torch.empty(pages, 1, 64, 256, dtype=F16, device="cuda") for _ in range(2))
+    at = [pages - 1 - 3 * i for i in range(len(p.pages[0]))]
+    k[at], v[at] = p.k[p.pages[0]], p.v[p.pages[0]]
+    want, _ = run_attend(p)
+    p.k, p.v, p.pages = k, v, [at]
+    p.table = torch.tensor([at], dtype=torch.int32, device="cuda")
+    got, _ = run_attend(p)
+    assert torch.equal(got, want)
+
+
+def test_bad_indices_are_reported(lib):
+    """A page outside the cache and a length over max_len set bit 2, and leave other sequences alone."""
+    p = Problem([100, 100], [20, 20], 8, 2, seed=12)
+    want, _ = run_attend(p)
+    p.table[0, 2] = 10**6
+    got, _ = run_attend(p)
+    torch.cuda.synchronize()
+    assert lib.snl_device_error(1) == 4 and torch.equal(got[20:], want[20:])
+    p.table[0, 2] = p.pages[0][2]
+    p.len_t[0] = 500
+    got, _ = run_attend(p)
+    torch.cuda.synchronize()
+    assert lib.snl_device_error(1) == 4 and torch.equal(got[20:], want[20:])
+
+
+# ---- append --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,kv,d,page,layout,dtype", SHAPES)
+@pytest.mark.parametrize("axes,pairs,rot,normed,src", [
+    (paged.INTERLEAVED, paged.HALVES, 64, True, F32), (paged.SECTIONS, paged.ADJACENT, 64, False, None),
+    (paged.ONE, paged.HALVES, 128, True, None), (paged.SECTIONS, paged.HALVES, 10, True, F32), (paged.ONE, 0, 0, True, F32),
+])
+def test_append(heads, kv, d, page, layout, dtype, axes, pairs, rot, normed, src):
+    lens, rows = [37, 1, 200, 9], [5, 1, 131, 9]
+    p = Problem(lens, rows, heads, kv, d, page, layout, dtype, seed=rot + heads)
+    src = src or dtype
+    n = p.n
+    wide = p.normal(n, (2 * heads + 2 * kv) * d).to(src)  # per head [q | gate], then k, then v
+    q = wide[:, :2 * heads * d].view(n, heads, 2 * d)[:, :, :d]
+    k = wide[:, 2 * heads * d:(2 * heads + kv) * d].view(n, kv, d)
+    v = wide[:, (2 * heads + kv) * d:].view(n, kv, d)
+    qn, kn = (0.2 * p.normal(d), 0.2 * p.normal(d)) if normed else (None, None)
+    half = rot // 2
+    sections = (half - 2 * (half // 3), half // 3, half // 3)
+    pos = torch.randint(0, 5000, (n, 4), generator=p.gen, device="cuda", dtype=torch.int32)
+    rope = None
+    if rot:
+        rope = torch.empty(5000, half, 2, device="cuda")
+        paged.rope_table(rope, 1e7)
+    before = p.k.clone(), p.v.clone()
+    q_out = torch.empty(n, heads, d, dtype=dtype, device="cuda")
+    p.cache(paged).append(p.batch(paged), q, k, v, q_out, pos if rot else None, rope, axes=axes, pairs=pairs,
+                          sections=sections, q_norm=qn, k_norm=kn)
+    u = ref.UNIT[dtype]
+
+    def near(got, want, size):  # one rounding, and a few of 32 bits in the norm and the turn
+        return ((got.double() - want).abs() <= u * want.abs() + 16 * 2.0**-24 * size + ref.TINY[dtype]).all()
+
+    want = ref.turned(q, pos, rope, axes, pairs, sections, qn)
+    assert near(q_out, want, want.abs().amax(-1, keepdim=True))
+    want = ref.turned(k, pos, rope, axes, pairs, sections, kn)
+    fresh = torch.zeros(p.k.shape[0], page, dtype=torch.bool, device="cuda")
+    for i in range(len(lens)):
+        r0, r1 = p.seq_rows(i)
+        pg, sl = p.where(i)
+        pg, sl = pg[lens[i] - rows[i]:], sl[lens[i] - rows[i]:]
+        fresh[pg, sl] = True
+        assert near(p.k[pg, :, sl], want[r0:r1], want[r0:r1].abs().amax(-1, keepdim=True))
+        assert torch.equal(p.v[pg, :, sl], v[r0:r1].to(dtype))
+    for now, was in zip((p.k, p.v), before):  # nothing else is written
+        now, was = (x.transpose(1, 2)[~fresh].nan_to_num(77) for x in (now, was))
+        assert torch.equal(now, was)
+
+
+def test_append_without_q_and_other_stream():
+    p = Problem([20, 33], [4, 33], 4, 2, seed=1)
+    k, v = p.normal(p.n, 2, 256).to(F16), p.normal(p.n, 2, 256).to(F16)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    p.cache(paged).append(p.batch(paged), None, k, v, None, stream=s.cuda_stream)
+    s.synchronize()
+    pg, sl = p.where(1)
+    assert torch.equal(p.k[pg, :, sl], k[4:]) and torch.equal(p.v[pg, :, sl], v[4:])
+
+
+def test_rope_table_far_positions():
+    t = torch.empty(262144, 32, 2, device="cuda")
+    paged.rope_table(t, 1e7)
+    f = torch.arange(32, dtype=torch.float64, device="cuda")
+    a = torch.arange(262144, dtype=torch.float64, device="cuda")[:, None] * 1e7 ** (-2 * f / 64)
+    # one rounding to 32 bits, and 64-bit angles off by a few 2^-53 of up to 262144
+    assert ((t[..., 0].double() - a.cos()).abs() <= 2.0**-24).all()
+    assert ((t[..., 1].double() - a.sin()).abs() <= 2.0**-24).all()
+
+
+def test_append_reports_positions(lib):
+    p = Problem([5], [5], 4, 1, seed=2)
+    x = p.normal(5, 1, 256).to(F16)
+    pos = torch.tensor([[3, 0, 0, 0]] * 4 + [[40, 0, 0, 0]], dtype=torch.int32, device="cuda")
+    rope = torch.zeros(40, 16, 2, device="cuda")
+    p.cache(paged).append(p.batch(paged), None, x, x, None, pos, rope)
+    torch.cuda.synchronize()
+    assert lib.snl_device_error(1) == 4
+
+
+# ---- weigh ---------------------------------------------------------------------------------
+
+
+def check_weigh(p, decay=1.0, **masks):
+    _, lse, _, _ = ref.attend(p, p.q, **masks)
+    lse = lse.float()
+    want, tol = ref.weigh(p, p.q, lse, p.weight, decay, **masks)
+    p.cache(paged).weigh(p.batch(paged), p.q, lse, decay=decay, **masks)
+    got = p.weight.double()
+    assert torch.equal(got.isnan(), want.isnan())
+    off = ((got - want).abs() - tol).nan_to_num(0)
+    assert (off <= 0).all(), float(off.max())
+
+
+@pytest.mark.parametrize("heads,kv,d,page,layout,dtype", SHAPES)
+@pytest.mark.parametrize("lens,rows", [([1], [1]), ([7, 300, 64], [1, 1, 1]), ([500, 63, 130], [37, 63, 2])])
+def test_weigh_shapes(heads, kv, d, page, layout, dtype, lens, rows):
+    check_weigh(Problem(lens, rows, heads, kv, d, page, layout, dtype, seed=heads, weight=True))
+
+
+@pytest.mark.parametrize("n", [1, 2, 127, 128, 129, 257])
+@pytest.mark.parametrize("decay", [0.0, 0.5])
+def test_weigh_lengths(n, decay):
+    check_weigh(Problem([n, 40], [min(n, 33), 1], seed=n, weight=True), decay)
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("d,rows", [(256, [37, 150, 1]), (128, [1, 1, 1])])
+def test_weigh_masks(mask, d, rows):
+    p = Problem([300, 150, 77], rows, 8, 2, d, 16, seed=d, weight=True)
+    check_weigh(p, **masks_of(p, **MASKS[mask]))
+
+
+def test_weigh_hides_what_is_not_seen():
+    """Old weights of the step's own slots, NaN keys that no row sees, sequences without rows."""
+    p = Problem([300, 60, 0], [64, 0, 0], 8, 2, seed=13, weight=True)
+    pg, sl = p.where(0)
+    p.weight[pg[236:], :, sl[236:]] = math.nan
+    m = masks_of(p, window=50)
+    check_weigh(p, **m)
+    p.k[pg[:100], :, sl[:100]] = math.nan
+    before = p.weight.clone()
+    _, lse = run_attend(p, **m)
+    p.cache(paged).weigh(p.batch(paged), p.q, lse, **m)
+    assert torch.equal(p.weight[pg[:100], :, sl[:100]], before[pg[:100], :, sl[:100]])
+    assert not p.weight[pg, :, sl].isnan().any()
+
+
+def test_weigh_sums_to_the_rows():
+    """Every row hands out a weight of one per head."""
+    p = Problem([700], [90], 8, 2, seed=14, weight=True)
+    _, lse = run_attend(p)
+    p.cache(paged).weigh(p.batch(paged), p.q, lse, decay=0.0)
+    pg, sl = p.where(0)
+    total = p.weight[pg, :, sl].double().sum(0)
+    assert ((total - 90 * 4).abs() <= 90 * 4 * 2e-5).all()
+
+
+# ---- evict ---------------------------------------------------------------------------------
+
+
+def check_evict(p, budget, sink, recent, in_place, extra_pages=0):
+    kept = torch.full((len(p.lens), p.kv, budget), 99, dtype=torch.int32, device="cuda")
+    k, v, w = p.k.clone(), p.v.clone(), p.weight.clone()
+    cache, batch = p.cache(paged), p.batch(paged)
+    if in_place:
+        new_lens, to = p.len_t, p.pages
+        cache.evict(batch, budget, kept, sink=sink, recent=recent)
+    else:
+        n = -(-budget // p.page)
+        to = [p.free[i * n:(i + 1) * n] for i in range(len(p.lens))]
+        into = torch.tensor(to, dtype=torch.int32, device="cuda")
+        new_lens = torch.empty_like(p.len_t)
+        cache.evict(batch, budget, kept, into, new_lens, sink=sink, recent=recent)
+    assert new_lens.tolist() == [min(n, budget) for n in p.lens]
+    for i, n in enumerate(p.lens):
+        pg, sl = p.where(i)
+        at = torch.arange(min(n, budget))
+        ng, ns = torch.tensor(to[i], dtype=torch.long)[at // p.page].cuda(), (at % p.page).cuda()
+        old = w[pg, :, sl].cpu()
+        for h in range(p.kv):
+            want = ref.evict(old[:, h].tolist(), n, budget, sink, recent)
+            assert kept[i, h].tolist() == want + [-1] * (budget - len(want))
+            src = torch.tensor(want, dtype=torch.long, device="cuda")
+            for now, was in ((p.k, k), (p.v, v), (p.weight, w)):
+                a, b = now[ng, h, ns], was[pg[src], h, sl[src]]
+                assert torch.equal(a.nan_to_num(55), b.nan_to_num(55))
+    if not in_place:  # the old pages are as they were
+        mine = [x for s in p.pages for x in s]
+        assert torch.equal(p.k[mine].nan_to_num(55), k[mine].nan_to_num(55))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,budget,sink,recent", [
+    ([100, 30, 1, 0, 64], 64, 4, 16), ([1000, 1100], 512, 0, 0), ([300], 299, 4, 64), ([300], 1, 0, 0),
+    ([300], 300, 4, 4), ([300], 80, 16, 64), ([2500, 40], 1031, 1, 1), ([9], 8, 8, 0), ([9], 8, 0, 8),
+])
+@pytest.mark.parametrize("kv,d,page,layout", [(1, 256, 16, "head"), (3, 128, 32, "slot")])
+def test_evict(lens, budget, sink, recent, in_place, kv, d, page, layout):
+    p = Problem(lens, [min(n, 1) for n in lens], 4 * kv, kv, d, page, layout, seed=budget, weight=True,
+                spare=len(lens) * -(-budget // page))
+    check_evict(p, budget, sink, recent, in_place)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("values", ["ties", "zeros", "odd"])
+def test_evict_ties_and_odd_weights(values, in_place):
+    """Equal weights keep the lowest slots; -0 and 0 are equal; NaN counts as -inf."""
+    p = Problem([400, 777], [1, 1], 8, 2, seed=15, weight=True, spare=50)
+    if values == "ties":
+        p.weight = (p.weight * 6).round()
+    elif values == "zeros":
+        p.weight = torch.where(p.weight > 0.5, 0.0, -0.0)
+    else:
+        x = p.weight
+        pick = (x * 1000).nan_to_num(0).long() % 6
+        p.weight = torch.stack([x, x - 0.5, x * 1e-42, torch.full_like(x, math.inf), torch.full_like(x, -math.inf),
+                                torch.full_like(x, math.nan)])[pick, *torch.meshgrid(*[torch.arange(n, device="cuda") for n in x.shape], indexing="ij")]
+    check_evict(p, 350, 2, 30, in_place)
+
+
+# ---- together --------------------------------------------------------------------------------
+
+
+def test_serving_a_prompt_in_chunks_equals_one_chunk():
+    """append + attend in chunks and single tokens give what one chunk gives."""
+    p = Problem([150], [150], 8, 2, seed=16)
+    x = [p.normal(150, h, 256).to(F16) for h in (8, 2, 2)]
+    pos = torch.arange(150, dtype=torch.int32, device="cuda")[:, None].repeat(1, 4).contiguous()
+    rope = torch.empty(200, 32, 2, device="cuda")
+    paged.rope_table(rope, 1e4)
+    q_out = torch.empty(150, 8, 256, dtype=F16, device="cuda")
+    p.cache(paged).append(p.batch(paged), *x, q_out, pos, rope)
+    whole, _, tol, _ = ref.attend(p, q_out)
+    p.k.fill_(math.nan), p.v.fill_(math.nan)
+    got, at = [], 0
+    for n in (64, 1, 1, 70, 14):
+        p.lens, p.rows, p.n = [at + n], [n], n
+        p.len_t.fill_(at + n)
+        p.start = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        s = slice(at, at + n)
+        out = torch.empty(n, 8, 256, dtype=F16, device="cuda")
+        p.cache(paged).append(p.batch(paged), *(y[s] for y in x), out, pos[s].contiguous(), rope)
+        assert torch.equal(out, q_out[s])
+        got.append(run_attend(p, out)[0])
+        at += n
+    assert ((torch.cat(got).double() - whole).abs() <= tol).all()
+
+
+def test_evicted_cache_attends_like_its_kept_slots():
+    """attend -> weigh -> evict -> attend of the next token sees the kept slots of each head."""
+    p = Problem([600], [100], 8, 2, seed=17, weight=True, spare=20)
+    _, lse = run_attend(p)
+    cache, batch = p.cache(paged), p.batch(paged)
+    cache.weigh(batch, p.q, lse, decay=0.0)
+    kept = torch.empty(1, 2, 256, dtype=torch.int32, device="cuda")
+    k, v = (p.keys(0, x) for x in (p.k, p.v))
+    cache.evict(batch, 256, kept, sink=4, recent=32)
+    assert int(p.len_t[0]) == 256
+    p.lens, p.rows, p.n = [256], [1], 1
+    p.start = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    p.q = p.q[-1:]
+    out, lse = check_attend(p)
+    for h in range(2):
+        i = kept[0, h].long()
+        s = p.q[0, 4 * h:4 * h + 4].double() @ k[i, h].T / 16
+        want = torch.softmax(s, -1) @ v[i, h]
+        assert ((out[0, 4 * h:4 * h + 4].double() - want).abs() <= 4e-3).all()  # 8 roundings of 2^-11 of values up to 1
+
+
+def test_matches_the_contiguous_cache(lib):
+    """append and attend over pages against snl_attn_prep and snl_attend over the engine's cache."""
+    import ctypes as C
+
+    from sensenova_b200.ffi import AttnP, StepU
+
+    n, heads, kv = 96, 16, 4
+    p = Problem([n], [n], heads, kv, seed=18)
+    proj = p.normal(n, (2 * heads + 2 * kv) * 256)
+    norms = 0.1 * p.normal(512)
+    pos = torch.randint(0, 3000, (n, 4), generator=p.gen, device="cuda", dtype=torch.int32)
+    ap = AttnP(heads, kv, 64, proj.shape[1], 1e7, 1e-6, 1 / 16.0, (33 << 16) | 30)
+    st = StepU(n, 0, 1, 0)
+    ptr = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    qbuf = torch.empty(n, heads * 256, device="cuda")
+    kc, vc = (torch.empty(n * kv * 256, dtype=F16, device="cuda") for _ in range(2))
+    want = torch.empty(n, heads * 256, device="cuda")
+    ffi.check(lib.snl_attn_prep(C.byref(st), C.byref(ap), ptr(proj), ptr(qbuf), ptr(kc), ptr(vc), ptr(norms), ptr(pos), None))
+    ffi.check(lib.snl_attend(C.byref(st), C.byref(ap), ptr(proj), ptr(qbuf), ptr(kc), ptr(vc), ptr(want), None, None))
+    rope = torch.empty(3000, 32, 2, device="cuda")
+    paged.rope_table(rope, 1e7)
+    per = proj[:, :2 * heads * 256].view(n, heads, 512)
+    q_out = torch.empty(n, heads, 256, dtype=F16, device="cuda")
+    p.cache(paged).append(p.batch(paged), per[:, :, :256], proj[:, 2 * heads * 256:(2 * heads + kv) * 256].view(n, kv, 256),
+                          proj[:, (2 * heads + kv) * 256:].view(n, kv, 256), q_out, pos, rope, axes=paged.INTERLEAVED,
+                          sections=(11, 11, 10), q_norm=norms[:256].contiguous(), k_norm=norms[256:].contiguous())
+    pg, sl = p.where(0)
+    # the engine's 32-bit angles at positions up to 3000 are off by up to 2e-4
+    assert (p.k[pg, :, sl].float() - kc.view(n, kv, 256).float()).abs().max() < 5e-3
+    assert torch.equal(p.v[pg, :, sl], vc.view(n, kv, 256))
+    out, _ = run_attend(p, q_out, per[:, :, 256:], out_dtype=F32)
+    assert (out.view(n, -1) - want).abs().max() < 4e-3 * want.abs().max()
