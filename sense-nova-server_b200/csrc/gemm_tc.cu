@@ -36,8 +36,22 @@
 #include "common.cuh"
 #include "ptx.cuh"
 #include "tc.cuh"
+#include "tensor_map.cuh"
 
 namespace snl {
+
+PFN_cuTensorMapEncodeTiled tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return (PFN_cuTensorMapEncodeTiled) nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
+  }();
+  return fn;
+}
+
 namespace {
 
 constexpr uint32_t kTcM = 128;
@@ -490,18 +504,6 @@ __global__ void tc_xpack_kernel(const float* __restrict__ x, uint32_t x_stride, 
   *reinterpret_cast<uint2*>(planes + total + o) = *reinterpret_cast<const uint2*>(lo);
 }
 
-PFN_cuTensorMapEncodeTiled encode_fn() {
-  static PFN_cuTensorMapEncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return (PFN_cuTensorMapEncodeTiled) nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
-  }();
-  return fn;
-}
-
 // Per-device scratch for the x planes of one GEMM, grown on demand.
 __half* planes_scratch(size_t halves) {
   static std::mutex mu;
@@ -543,7 +545,7 @@ int launch_gemm_tc(int dtype, const snl_mat_p& p, uint32_t m, const float* x, co
                    cudaStream_t s, const __half* wplanes) {
   if (dtype != SNL_Q8_0 && dtype != SNL_Q4_0) return fail(SNL_E_INVALID, "gemm_tc: dtype");
   if (p.k % 32 || p.k == 0 || m == 0) return fail(SNL_E_INVALID, "gemm_tc: k must be a positive multiple of 32");
-  PFN_cuTensorMapEncodeTiled enc = encode_fn();
+  PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
   if (!enc) return fail(SNL_E_CUDA, "gemm_tc: cuTensorMapEncodeTiled is unavailable");
   int* err = nullptr;
   if (int rc = device_error_word(&err)) return rc;

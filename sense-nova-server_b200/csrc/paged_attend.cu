@@ -4,9 +4,13 @@
 #include <string>
 
 #include "paged.cuh"
+#include "tc.cuh"
+#include "tensor_map.cuh"
 
 namespace snl {
 namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
   PagedView c;
@@ -18,66 +22,572 @@ struct AttendArgs {
   float* lse;
   const float* lse_in;
   float decay;
+  uint32_t group, toks;              // query heads per KV head; tokens of one tile (128 / group)
+  uint32_t slots, n_split, split_len;  // tile slots; parts of the keys and keys of one part
+  float* part;                       // [row][head][part][D], then [row][head][part][max, sum]
+  float2* part_ml;
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh x = 1 - 2 / (1 + e^2x): off by less than 2^-22, which tanh.approx (2^-11) is not.
+__device__ __forceinline__ float tanh_(float x) { return fmaf(-2.f, rcp(1.f + ex2(2.f * kLog2e * x)), 1.f); }
+
+// A bounded wait of about 0.15 s: the longest that one of these is due is some microseconds.
+__device__ __forceinline__ bool wait_mbar(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 28); }
+__device__ __forceinline__ void bar_sync(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t id, uint32_t n) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ---- tensor-core pieces ----------------------------------------------------------------
+
+// Keys of one tile and the tensor-memory columns of a CTA (512 in all): the output, the
+// queries (A operand of the scores, 16-bit pairs), and two score tiles that the
+// probabilities overwrite.
+template <int D>
+struct Geo {
+  static constexpr uint32_t KT = D == 256 ? 64 : 128;
+  static constexpr uint32_t kTile = KT * D * 2;  // bytes of a K or V tile (32 KB)
+  static constexpr uint32_t kGroup = D * 16;     // bytes of 8 keys
+  static constexpr uint32_t kStages = 6;
+  static constexpr uint32_t kSmem = kStages * kTile + 1024;
+  static constexpr uint32_t kO = 0, kQ = D, kS = D == 256 ? 384 : 256;
+};
+
+template <typename T>
+constexpr uint32_t idesc16(uint32_t n, bool b_mn) {  // D f32, A and B f16 or bf16, M = 128
+  const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// A tile in shared memory is [8-key group][64-element chunk][8 keys][128 bytes], 128-byte
+// swizzled. As K (K-major) the groups are the 8-row groups, sbo apart; as V (MN-major) the
+// chunks are lbo and the groups sbo apart.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// A from tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int c1, int c3, int c4, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(c1), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// 32 columns of this thread's lane, not waited for.
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+// Waits for this thread's loads; the empty statements keep uses of the registers behind it.
+template <int N>
+__device__ __forceinline__ void tm_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Where a tile of rows lies: sequence, first row, tokens, slot of the first token.
+struct TileInfo {
+  uint32_t b, row0, toks;
+  int32_t t0, len;
+};
+
+// Slot s belongs to the last sequence b with start[b] / toks + b <= s: a sequence has at
+// least as many slots as tiles, found without a sum over the batch. One warp.
+__device__ __forceinline__ TileInfo find_tile(const AttendArgs& a, uint32_t s, uint32_t lane) {
+  uint32_t lo = 0, hi = a.c.n_seqs;
+  while (hi - lo > 1) {
+    const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const bool le = at < hi && (at == lo || (uint32_t)__ldg(a.c.start + at) / a.toks + at <= s);
+    const uint32_t n = __popc(__ballot_sync(0xffffffffu, le));
+    const uint32_t below = lo + (max(n, 1u) - 1) * step;
+    hi = min(hi, below + step);
+    lo = below;
+  }
+  TileInfo w{lo, 0, 0, 0, 0};
+  const int2 rr = paged_rows(a.c, lo);
+  const uint32_t base = (uint32_t)rr.x / a.toks + lo;
+  if (s < base) return w;
+  const uint32_t off = (s - base) * a.toks;
+  if (off >= (uint32_t)(rr.y - rr.x)) return w;
+  w.row0 = rr.x + off;
+  w.toks = min(a.toks, (uint32_t)(rr.y - rr.x) - off);
+  w.len = paged_len(a.c, lo);
+  w.t0 = w.len - (rr.y - rr.x) + (int32_t)off;
+  return w;
+}
+
+constexpr uint32_t kSoftWarps = 8;
+constexpr uint32_t kAttendThreads = (kSoftWarps + 2) * 32;
+constexpr float kRefSlack = 8.f;  // log2 that scores may exceed the reference before O is rescaled
+
+// CTA = (tile of 128 (token, head) rows of one KV head's group, part of the keys). Warp 8
+// loads K and V tiles by TMA, 8 keys of one page at a time; warp 9 issues S = Q K^T and
+// O += P V (tcgen05, accumulators in tensor memory); two warpgroups turn the score tiles
+// into probabilities in turn, thread = row. The maximum that the exponentials refer to is
+// handed from tile to tile and moves only when a score exceeds it by kRefSlack.
+template <typename T, int D, bool GENERAL>
+__global__ void __launch_bounds__(kAttendThreads, 1)
+    attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap) {
+  using G = Geo<D>;
+  constexpr uint32_t KT = G::KT, NS = G::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[NS], empty[NS], s_full[2], p_ready[2], pv_done[2], drained;
+  __shared__ uint32_t tmem_sh;
+  __shared__ TileInfo info_sh;
+  __shared__ int32_t lohi[4][kSoftWarps / 2];  // per warp: least and largest lo, least and largest hi
+  __shared__ float ref_sh[128], l_sh[2][128], lref_sh[2][128];
+  __shared__ volatile int fail_sh;
+  __shared__ int odd_v;
+  pdl_trigger();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t kh = blockIdx.x % a.c.n_kv, unit = blockIdx.x / a.c.n_kv;
+  const uint32_t split = unit % a.n_split, slot = a.slots - 1 - unit / a.n_split;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+
+  if (tid == 0) {
+    for (uint32_t s = 0; s < NS; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; s++) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_ready[s], kSoftWarps / 2);
+      mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(&drained, 1);
+    fail_sh = 0;
+    odd_v = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(&tmem_sh, 512);
+  pdl_wait();
+  if (warp == 8) {
+    const TileInfo w = find_tile(a, slot, lane);
+    if (lane == 0) info_sh = w;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_sh;
+  const TileInfo w = info_sh;
+
+  // Row of this thread (both warpgroups hold all 128): token and head, its keys.
+  const uint32_t row = tid & 127, tok = row / a.group, head = kh * a.group + row % a.group;
+  const bool valid = warp < kSoftWarps && tok < w.toks;
+  int2 keys = make_int2(0, 0);
+  if (valid) keys = paged_keys(a.m, w.row0 + tok, w.t0 + (int32_t)tok, w.len);
+  if (warp < kSoftWarps / 2) {
+    const bool some = keys.x < keys.y;
+    const int32_t lo0 = __reduce_min_sync(0xffffffffu, some ? keys.x : INT32_MAX);
+    const int32_t hi1 = __reduce_max_sync(0xffffffffu, some ? keys.y : 0);
+    // a valid row without keys makes every tile a masked one
+    const int32_t lo1 = __reduce_max_sync(0xffffffffu, !valid ? 0 : some ? keys.x : INT32_MAX);
+    const int32_t hi0 = __reduce_min_sync(0xffffffffu, !valid ? INT32_MAX : keys.y);
+    if (lane == 0) {
+      lohi[0][warp] = lo0;
+      lohi[1][warp] = lo1;
+      lohi[2][warp] = hi0;
+      lohi[3][warp] = hi1;
+    }
+  }
+  const float sl = fmaxf(fabsf(a.m.scale) * kLog2e, 1e-30f);  // not 0: -inf of a masked score has to stay
+  if (warp < kSoftWarps) {
+    // Queries into tensor memory, lane = row, the sign of the scale folded in.
+    const uint32_t wg = warp >> 2, flip = a.m.scale < 0.f ? 0x80008000u : 0u;
+    const uint16_t* src = a.q + (uint64_t)(w.row0 + tok) * a.p.q_row + (uint64_t)head * a.p.q_head;
+    const uint32_t lanes = ((warp & 3) * 32) << 16;
+#pragma unroll
+    for (uint32_t c = 0; c < D / 4; c += 32) {
+      uint32_t r[32];
+#pragma unroll
+      for (uint32_t i = 0; i < 32; i += 4) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (valid) x = __ldg(reinterpret_cast<const uint4*>(src + 2 * (wg * (D / 4) + c + i)));
+        r[i] = x.x ^ flip, r[i + 1] = x.y ^ flip, r[i + 2] = x.z ^ flip, r[i + 3] = x.w ^ flip;
+      }
+      __syncwarp();
+      tm_st32(tmem + lanes + G::kQ + wg * (D / 4) + c, r);
+    }
+    tm_wait_st();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int32_t lo0 = lohi[0][0], lo1 = lohi[1][0], hi0 = lohi[2][0], hi1 = lohi[3][0];
+#pragma unroll
+  for (uint32_t i = 1; i < kSoftWarps / 2; i++) {
+    lo0 = min(lo0, lohi[0][i]);
+    lo1 = max(lo1, lohi[1][i]);
+    hi0 = min(hi0, lohi[2][i]);
+    hi1 = max(hi1, lohi[3][i]);
+  }
+  // Tiles [j0, j0 + nt): what the rows see, cut to this part.
+  const int32_t c0 = (int32_t)(split * a.split_len);
+  const int32_t beg = max(lo0 == INT32_MAX ? 0 : lo0, c0), end = min(hi1, c0 + (int32_t)a.split_len);
+  const uint32_t j0 = beg < end ? (uint32_t)beg / KT : 0, nt = beg < end ? ((uint32_t)end + KT - 1) / KT - j0 : 0;
+  // The i-th load: K tiles run one ahead of V tiles, as the MMAs do.
+  auto k_load = [&](uint32_t i) { return i == 0 ? 0u : 2 * i - 1; };
+  auto v_load = [&](uint32_t i) { return i + 1 == nt ? 2 * nt - 1 : 2 * i + 2; };
+
+  if (warp == 8) {
+    // Lane g < KT / 8 loads the tile's g-th 8 keys; keys past the length and pages outside
+    // the cache come from a page coordinate past the end, which reads zeros.
+    auto page_of = [&](uint32_t i) -> int32_t {
+      const uint32_t key = (j0 + i) * KT + 8 * lane;
+      int32_t p = -1;
+      if (i < nt && lane < KT / 8 && (int32_t)key < w.len) p = paged_page(a.c, w.b, key);
+      return p < 0 ? (int32_t)a.c.n_pages : p;
+    };
+    int32_t now = page_of(0), next = page_of(1), prev = now;
+    uint32_t n = 0;
+    auto load = [&](const CUtensorMap* map, uint32_t i, int32_t page) -> bool {
+      const uint32_t st = n % NS;
+      bool ok = n < NS || wait_mbar(&empty[st], (n / NS - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok && !fail_sh);
+      if (!ok) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], G::kTile);
+      __syncwarp();
+      if (lane < KT / 8)
+        tma_load_5d(smem_u32(smem + st * G::kTile + lane * G::kGroup), map,
+                    (int)(((j0 + i) * KT + 8 * lane) & ((1u << a.c.shift) - 1)), (int)kh, page, &full[st]);
+      n++;
+      return true;
+    };
+    bool ok = true;
+    for (uint32_t i = 0; ok && i <= nt; i++) {
+      if (i < nt) ok = load(&kmap, i, now);
+      if (ok && i > 0) ok = load(&vmap, i - 1, prev);
+      prev = now;
+      now = next;
+      next = page_of(i + 2);
+    }
+    if (!ok && lane == 0) fail_sh = 1;
+    // every load lands before the CTA ends, whatever became of its readers
+    for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) (void)wait_mbar(&full[i % NS], (i / NS) & 1);
+  } else if (warp == 9) {
+    if (lane == 0) {
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && !fail_sh && wait_mbar(bar, parity); };
+      auto scores = [&](uint32_t i) {
+        const uint32_t n = k_load(i), st = n % NS;
+        wait(&full[st], (n / NS) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t base = smem_u32(smem + st * G::kTile);
+#pragma unroll
+        for (uint32_t kk = 0; kk < D / 16; kk++)
+          mma_ts(tmem + G::kS + (i & 1) * KT, tmem + G::kQ + kk * 8,
+                 tile_desc(base + (kk / 4) * 1024 + (kk % 4) * 32, 16, G::kGroup), idesc16<T>(KT, false), kk != 0);
+        tc_commit(&empty[st]);
+        tc_commit(&s_full[i & 1]);
+      };
+      if (nt) scores(0);
+      for (uint32_t i = 0; ok && i < nt; i++) {
+        if (i + 1 < nt) scores(i + 1);
+        const uint32_t n = v_load(i), st = n % NS;
+        wait(&full[st], (n / NS) & 1);
+        wait(&p_ready[i & 1], (i >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t base = smem_u32(smem + st * G::kTile);
+#pragma unroll
+        for (uint32_t kk = 0; kk < KT / 16; kk++)
+          mma_ts(tmem + G::kO, tmem + G::kS + (i & 1) * KT + kk * 8, tile_desc(base + kk * 2 * G::kGroup, 1024, G::kGroup),
+                 idesc16<T>(D, true), (i | kk) != 0);
+        tc_commit(&empty[st]);
+        tc_commit(&pv_done[i & 1]);
+      }
+      if (!ok) {
+        fail_sh = 1;
+        report_timeout(a.c.err);
+      }
+      tc_commit(&drained);  // and every MMA before the tensor memory is given back
+      (void)wait_mbar(&drained, 0);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t wg = warp >> 2;
+    const uint32_t lanes = ((warp & 3) * 32) << 16;
+    const bool live = __any_sync(0xffffffffu, valid);
+    const float slope = GENERAL && a.m.slopes && valid ? __ldg(a.m.slopes + head) * kLog2e : 0.f;
+    const float cap = a.m.cap, pre = GENERAL && cap > 0.f ? a.m.scale / cap : 0.f;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = __all_sync(0xffffffffu, ok && !fail_sh && wait_mbar(bar, parity));
+    };
+    auto masked_tile = [&](int32_t k0) { return k0 < lo1 || k0 + (int32_t)KT > hi0; };
+    float l = 0.f, ref = -INFINITY;
+    for (uint32_t i = wg; i < nt; i += 2) {
+      const int32_t k0 = (int32_t)((j0 + i) * KT);
+      const bool masked = masked_tile(k0);
+      float s[KT];
+      uint32_t* r = reinterpret_cast<uint32_t*>(s);
+      wait(&s_full[wg], (i >> 1) & 1);
+      tc_fence_after();
+      float mx = -INFINITY;
+      if (live) {
+#pragma unroll
+        for (uint32_t c = 0; c < KT; c += 32) tm_ld32(tmem + lanes + G::kS + wg * KT + c, r + c);
+        tm_wait_ld<KT>(r);
+        if constexpr (GENERAL) {
+          const float gap = (float)(w.t0 + (int32_t)tok - k0);
+#pragma unroll
+          for (uint32_t c = 0; c < KT; c++) {
+            // the sign of the scale is in the queries already
+            float x = cap > 0.f ? cap * kLog2e * tanh_(s[c] * fabsf(pre)) : s[c] * sl;
+            s[c] = fmaf(-slope, fabsf(gap - (float)c), x);
+          }
+        }
+        if (masked) {
+          const int32_t x0 = keys.x - k0, n = keys.y - keys.x;
+#pragma unroll
+          for (uint32_t c = 0; c < KT; c++)
+            if ((uint32_t)((int32_t)c - x0) >= (uint32_t)n) s[c] = -INFINITY;
+        }
+        float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (uint32_t c = 4; c < KT; c++) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if constexpr (!GENERAL) mx *= sl;
+      }
+      // The reference passes from tile to tile between the warpgroups.
+      float before = -INFINITY;
+      if (i > 0) {
+        bar_sync(1 + ((i - 1) & 1), 256);
+        before = ref_sh[row];
+      }
+      const float now = mx > before + kRefSlack ? mx : before;
+      if (i + 1 < nt) {
+        ref_sh[row] = now;
+        bar_arrive(1 + (i & 1), 256);
+      }
+      if (i > 0 && __any_sync(0xffffffffu, now != before)) {
+        wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1);
+        tc_fence_after();
+        const float f = now != before ? ex2(before - now) : 1.f;
+#pragma unroll 1
+        for (uint32_t c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tm_ld32(tmem + lanes + G::kO + c, o);
+          tm_wait_ld<32>(o);
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tm_st32(tmem + lanes + G::kO + c, o);
+        }
+        tm_wait_st();
+      }
+      if (now != ref) l *= ex2(ref - now);
+      ref = now;
+      const float zero = now == -INFINITY ? 0.f : now;
+      if (live) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t c = 0; c < KT; c += 2) {
+          const float p0 = ex2(GENERAL ? s[c] - zero : fmaf(s[c], sl, -zero));
+          const float p1 = ex2(GENERAL ? s[c + 1] - zero : fmaf(s[c + 1], sl, -zero));
+          sum[c & 2] += p0;
+          sum[(c & 2) + 1] += p1;
+          r[c / 2] = pack2(p0, p1, T());
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (uint32_t c = 0; c < KT / 2; c += 32) tm_st32(tmem + lanes + G::kS + wg * KT + c, r + c);
+        tm_wait_st();
+      }
+      if (masked) {
+        // A row's probability for a key that it does not see is 0, but 0 * NaN is not: values that
+        // are not finite leave the tile, and reach the rows that see them at the end.
+        const uint32_t n = v_load(i);
+        wait(&full[n % NS], (n / NS) & 1);
+        if (ok) {
+          constexpr uint32_t inf2 = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+          uint4* tile = reinterpret_cast<uint4*>(smem + (n % NS) * G::kTile);
+          bool odd = false;
+#pragma unroll 4
+          for (uint32_t e = tid & 127; e < G::kTile / 16; e += 128) {
+            uint4 x = tile[e];
+            const uint32_t b0 = __vcmpeq2(x.x & inf2, inf2), b1 = __vcmpeq2(x.y & inf2, inf2),
+                           b2 = __vcmpeq2(x.z & inf2, inf2), b3 = __vcmpeq2(x.w & inf2, inf2);
+            if (b0 | b1 | b2 | b3) {
+              odd = true;
+              tile[e] = make_uint4(x.x & ~b0, x.y & ~b1, x.z & ~b2, x.w & ~b3);
+            }
+          }
+          if (odd) odd_v = 1;
+          fence_proxy_async_smem();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[wg]);
+      if (i + 1 == nt) ref_sh[row] = now;
+    }
+    // Sums of both warpgroups, referred to the last reference.
+    l_sh[wg][row] = l;
+    lref_sh[wg][row] = ref;
+    if (nt) wait(&pv_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1);
+    bar_sync(3, 256);
+    tc_fence_after();
+    const float fin = nt ? ref_sh[row] : -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+      const float rg = lref_sh[g][row];
+      if (rg != -INFINITY) l += rg == fin ? l_sh[g][row] : l_sh[g][row] * ex2(rg - fin);
+      else if (l_sh[g][row] != 0.f) l = NAN;  // only scores of NaN
+    }
+    const bool parts = a.n_split > 1;
+    const uint64_t rh = (uint64_t)(w.row0 + tok) * a.p.n_heads + head;
+    if (valid && wg == 0) {
+      if (parts) a.part_ml[rh * a.n_split + split] = make_float2(fin, l);
+      else if (a.lse) a.lse[rh] = l == 0.f ? -INFINITY : ((fin == -INFINITY ? 0.f : fin) + log2f(l)) * (1.f / kLog2e);
+    }
+    const float inv = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+    for (uint32_t c = wg * (D / 2); live && c < (wg + 1) * (D / 2); c += 32) {
+      uint32_t r[32];
+      float* o = reinterpret_cast<float*>(r);
+      __syncwarp();
+      if (nt) {
+        tm_ld32(tmem + lanes + G::kO + c, r);
+        tm_wait_ld<32>(r);
+      }
+      if (!valid || (parts && nt == 0)) continue;
+      if (odd_v) {
+        for (uint32_t j = j0; j < j0 + nt; j++) {
+          if (!masked_tile((int32_t)(j * KT))) continue;
+          const int32_t k1 = min(min((int32_t)((j + 1) * KT), keys.y), end);
+          for (int32_t key = max((int32_t)(j * KT), keys.x); key < k1; key++) {
+            const int32_t page = paged_page(a.c, w.b, key);
+            if (page < 0) continue;
+            const T* v = reinterpret_cast<const T*>(a.c.v + paged_at(a.c, page, kh, key)) + c;
+            for (int e = 0; e < 32; e++) {
+              const float x = (float)v[e];
+              if (!(fabsf(x) < INFINITY))
+#pragma unroll
+                for (int f = 0; f < 32; f++)
+                  if (f == e) o[f] += x;
+            }
+          }
+        }
+      }
+      if (l == 0.f)
+#pragma unroll
+        for (int e = 0; e < 32; e++) o[e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 32; e++) o[e] *= inv;
+      if (parts) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) store_from_float<4>(a.part, (rh * a.n_split + split) * D + c + e, SNL_T_F32, o + e);
+        continue;
+      }
+      if (a.gate) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          float g[8];
+          load_as_float<8>(a.gate, (uint64_t)(w.row0 + tok) * a.p.gate_row + (uint64_t)head * a.p.gate_head + c + e,
+                           a.p.gate_type, g);
+#pragma unroll
+          for (int f = 0; f < 8; f++) o[e + f] *= sigmoidf_(g[f]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+        store_from_float<8>(a.out, (uint64_t)(w.row0 + tok) * a.p.out_row + (uint64_t)head * a.p.out_head + c + e,
+                            a.p.out_type, o + e);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of a row: one warp per (row, head), over the parts that its keys touch.
+constexpr uint32_t kWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int E = D / 32;
+  pdl_trigger();
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t item = (uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const uint32_t r = (uint32_t)(item / a.p.n_heads), h = (uint32_t)(item % a.p.n_heads);
+  pdl_wait();
+  if (r >= a.c.n_rows) return;
+  const uint32_t b = paged_seq(a.c, r, lane);
+  const int2 rr = paged_rows(a.c, b);
+  const int32_t len = paged_len(a.c, b), t = len - (rr.y - (int32_t)r);
+  const int2 keys = (int32_t)r < rr.x || (int32_t)r >= rr.y ? make_int2(0, 0) : paged_keys(a.m, r, t, len);
+  const uint32_t p0 = (uint32_t)keys.x / a.split_len, p1 = keys.x < keys.y ? (uint32_t)(keys.y - 1) / a.split_len + 1 : p0;
+  const float2* ml = a.part_ml + item * a.n_split;
+  float top = -INFINITY, l = 0.f, o[E];
+  for (uint32_t s = p0; s < p1; s++) top = fmaxf(top, ml[s].x);
+  const float zero = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] = 0.f;
+  for (uint32_t s = p0; s < p1; s++) {
+    const float2 x = ml[s];
+    if (x.y == 0.f) continue;
+    const float f = x.x == -INFINITY ? 1.f : ex2(x.x - zero);
+    float v[E];
+    load_as_float<E>(a.part, (item * a.n_split + s) * D + lane * E, SNL_T_F32, v);
+    l = fmaf(x.y, f, l);
+#pragma unroll
+    for (int i = 0; i < E; i++) o[i] = fmaf(v[i], f, o[i]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float g[E];
+  if (a.gate) load_as_float<E>(a.gate, r * a.p.gate_row + h * a.p.gate_head + lane * E, a.p.gate_type, g);
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] *= a.gate ? inv * sigmoidf_(g[i]) : inv;
+  store_from_float<E>(a.out, r * a.p.out_row + h * a.p.out_head + lane * E, a.p.out_type, o);
+  if (a.lse && lane == 0) a.lse[item] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
+}
 
 // Score in units of log2 from the raw product: cap, then the distance bias.
 __device__ __forceinline__ float paged_score(const PagedMask& m, float qk, float slope, int32_t t, int32_t key) {
   float s = qk * m.scale;
   if (m.cap > 0.f) s = m.cap * tanhf(s / m.cap);
   return (s - slope * fabsf((float)(t - key))) * kLog2e;
-}
-
-constexpr uint32_t kWarps = 8;
-
-// One warp per (row, head), one key at a time.
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) attend_simple_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int E = D / 32;
-  pdl_trigger();
-  pdl_wait();
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t item = (uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const uint32_t r = (uint32_t)(item / a.p.n_heads), h = (uint32_t)(item % a.p.n_heads);
-  if (r >= a.c.n_rows) return;
-  const uint32_t type = std::is_same<T, __half>::value ? SNL_T_F16 : SNL_T_BF16;
-  const uint32_t kh = h / (a.p.n_heads / a.c.n_kv);
-  const uint32_t b = paged_seq(a.c, r, lane);
-  const int2 rr = paged_rows(a.c, b);
-  const int32_t len = paged_len(a.c, b), t = len - (rr.y - (int32_t)r);
-  const int2 keys = (int32_t)r < rr.x || (int32_t)r >= rr.y ? make_int2(0, 0) : paged_keys(a.m, r, t, len);
-  const float slope = a.m.slopes ? __ldg(a.m.slopes + h) : 0.f;
-  float q[E], o[E];
-  load_as_float<E>(a.q, r * a.p.q_row + h * a.p.q_head + lane * E, type, q);
-#pragma unroll
-  for (int i = 0; i < E; i++) o[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int32_t key = keys.x; key < keys.y; key++) {
-    const int32_t page = paged_page(a.c, b, key);
-    if (page < 0) continue;
-    float x[E], s = 0.f;
-    load_as_float<E>(a.c.k, paged_at(a.c, page, kh, key) + lane * E, type, x);
-#pragma unroll
-    for (int i = 0; i < E; i++) s = fmaf(q[i], x[i], s);
-    s = paged_score(a.m, warp_sum(s), slope, t, key);
-    const float top = fmaxf(m, s);
-    if (m == -INFINITY && s == -INFINITY) continue;
-    const float old = exp2f(m - top), p = exp2f(s - top);
-    m = top;
-    l = fmaf(l, old, p);
-    load_as_float<E>(a.c.v, paged_at(a.c, page, kh, key) + lane * E, type, x);
-#pragma unroll
-    for (int i = 0; i < E; i++) o[i] = fmaf(o[i], old, p * x[i]);
-  }
-  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-  float g[E];
-  if (a.gate) load_as_float<E>(a.gate, r * a.p.gate_row + h * a.p.gate_head + lane * E, a.p.gate_type, g);
-#pragma unroll
-  for (int i = 0; i < E; i++) o[i] *= a.gate ? inv * sigmoidf_(g[i]) : inv;
-  store_from_float<E>(a.out, r * a.p.out_row + h * a.p.out_head + lane * E, a.p.out_type, o);
-  if (a.lse && lane == 0)
-    a.lse[(uint64_t)r * a.p.n_heads + h] = l > 0.f || l != l ? (m + log2f(l)) / kLog2e : -INFINITY;
 }
 
 // One warp per (slot, KV head, sequence), one row and head at a time.
@@ -134,8 +644,80 @@ using namespace snl;
       SNL_PDL_LAUNCH(what, (kern<__nv_bfloat16, 128>), grid, block, smem, s, __VA_ARGS__);                     \
   } while (0)
 
+namespace {
+
+struct AttendPlan {
+  uint32_t toks, slots, n_split, split_len;
+};
+
+// How many parts the keys are cut into: the fewest microseconds of a model of waves of CTAs
+// (one per SM), each with a start and an end, and the traffic and launch of the join.
+// Per key a CTA takes about 11 ns at head_dim 256 when the tensor cores bound it.
+AttendPlan plan_attend(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t n_heads) {
+  AttendPlan pl{};
+  const uint32_t group = n_heads / c.n_kv;
+  pl.toks = 128 / group;
+  pl.slots = b.n_rows / pl.toks + b.n_seqs;
+  const uint64_t max_len = std::min<uint64_t>(b.max_len, (uint64_t)b.table_stride * c.page_size);
+  const uint64_t units = (uint64_t)std::min<uint64_t>(pl.slots, b.n_rows) * c.n_kv;
+  const double per_key = c.head_dim == 256 ? 0.015 : 0.008, sms = sm_count();
+  double best = 1e30;
+  pl.n_split = 1;
+  for (uint32_t n = 1; n <= 64; n++) {
+    const uint64_t len = ((max_len + n - 1) / n + 127) / 128 * 128;
+    if (n > 1 && len < 128) break;
+    const double waves = std::max(1.0, (double)((units * n + (uint64_t)sms - 1) / (uint64_t)sms));
+    double t = waves * (len * per_key + 3.0);
+    if (n > 1) t += 3.0 + (double)b.n_rows * n_heads * n * c.head_dim * 8 / 4e6;
+    if (t < best) {
+      best = t;
+      pl.n_split = n;
+    }
+  }
+  pl.split_len = (uint32_t)(((max_len + pl.n_split - 1) / pl.n_split + 127) / 128 * 128);
+  if (pl.split_len == 0) pl.split_len = 128;
+  pl.n_split = std::max<uint32_t>(1, (uint32_t)((max_len + pl.split_len - 1) / pl.split_len));
+  return pl;
+}
+
+// The pages as (64 elements, slot, chunk of 64, head, page): a box is 8 slots of a head.
+int page_map(CUtensorMap* map, const snl_paged_cache& c, void* base) {
+  PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
+  if (!enc) return fail(SNL_E_CUDA, "paged cache: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[5] = {64, c.page_size, c.head_dim / 64, c.n_kv, c.n_pages};
+  const cuuint64_t str[4] = {c.slot_stride * 2, 128, c.n_kv > 1 ? c.head_stride * 2 : 128,
+                             c.n_pages > 1 ? c.page_stride * 2 : 128};
+  const cuuint32_t box[5] = {64, 8, c.head_dim / 64, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, c.type == SNL_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+                         base, dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SNL_OK : fail(SNL_E_INVALID, "paged cache: the pages' strides do not fit a tensor map");
+}
+
+size_t part_bytes(const AttendPlan& pl, const snl_paged_cache& c, const snl_paged_batch& b, uint32_t n_heads) {
+  return pl.n_split == 1 ? 16 : (size_t)b.n_rows * n_heads * pl.n_split * (c.head_dim + 2) * sizeof(float);
+}
+
+template <typename T, int D, bool GENERAL>
+int go_attend(const AttendArgs& a, const CUtensorMap& km, const CUtensorMap& vm, uint32_t grid, cudaStream_t s) {
+  static bool attr[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr[dev]) {
+    SNL_CUDA_TRY(cudaFuncSetAttribute(attend_kernel<T, D, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)Geo<D>::kSmem));
+    if (dev >= 0 && dev < 64) attr[dev] = true;
+  }
+  SNL_PDL_LAUNCH("attend_kernel", (attend_kernel<T, D, GENERAL>), dim3(grid), dim3(kAttendThreads),
+                 (size_t)Geo<D>::kSmem, s, a, km, vm);
+  return SNL_OK;
+}
+
+}  // namespace
+
 extern "C" size_t snl_paged_attend_workspace(const snl_paged_cache* c, const snl_paged_batch* b, uint32_t n_heads) {
-  return c && b && n_heads ? 16 : 0;
+  if (!c || !b || c->n_kv == 0 || n_heads == 0 || n_heads % c->n_kv || n_heads / c->n_kv > 64) return 0;
+  return part_bytes(plan_attend(*c, *b, n_heads), *c, *b, n_heads);
 }
 
 extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_attn_p* p,
@@ -151,19 +733,40 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
       !paged_strides(p->out_type, p->out_row, p->out_head) ||
       (gate && !paged_strides(p->gate_type, p->gate_row, p->gate_head)))
     return fail(SNL_E_INVALID, w + ": rows must be aligned to 16 bytes");
-  if (work_bytes < snl_paged_attend_workspace(c, b, p->n_heads)) return fail(SNL_E_INVALID, w + ": work is too small");
+  const AttendPlan pl = plan_attend(*c, *b, p->n_heads);
+  if (work_bytes < part_bytes(pl, *c, *b, p->n_heads)) return fail(SNL_E_INVALID, w + ": work is too small");
   if (!work) return fail(SNL_E_INVALID, w + ": null argument");
   if (b->n_rows == 0 || b->n_seqs == 0) return SNL_OK;
+  SNL_TRY(paged_error_word(&a.c.err));
+  const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv;
+  if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
+  CUtensorMap km, vm;
+  SNL_TRY(page_map(&km, *c, c->k));
+  SNL_TRY(page_map(&vm, *c, c->v));
   a.p = *p;
   a.q = static_cast<const uint16_t*>(q);
   a.gate = gate;
   a.out = out;
   a.lse = lse;
-  SNL_TRY(paged_error_word(&a.c.err));
+  a.group = p->n_heads / c->n_kv;
+  a.toks = pl.toks;
+  a.slots = pl.slots;
+  a.n_split = pl.n_split;
+  a.split_len = pl.split_len;
+  a.part = static_cast<float*>(work);
+  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)b->n_rows * p->n_heads * pl.n_split * c->head_dim);
+  const cudaStream_t s = (cudaStream_t)stream;
+  const bool half = c->type == SNL_T_F16, wide = c->head_dim == 256, gen = p->cap > 0.f || p->slopes;
+  const uint32_t g = (uint32_t)grid;
+  if (half && wide) SNL_TRY(gen ? (go_attend<__half, 256, true>(a, km, vm, g, s)) : (go_attend<__half, 256, false>(a, km, vm, g, s)));
+  else if (half) SNL_TRY(gen ? (go_attend<__half, 128, true>(a, km, vm, g, s)) : (go_attend<__half, 128, false>(a, km, vm, g, s)));
+  else if (wide) SNL_TRY(gen ? (go_attend<__nv_bfloat16, 256, true>(a, km, vm, g, s)) : (go_attend<__nv_bfloat16, 256, false>(a, km, vm, g, s)));
+  else SNL_TRY(gen ? (go_attend<__nv_bfloat16, 128, true>(a, km, vm, g, s)) : (go_attend<__nv_bfloat16, 128, false>(a, km, vm, g, s)));
+  if (pl.n_split == 1) return SNL_OK;
   const uint64_t items = (uint64_t)b->n_rows * p->n_heads;
-  if (items > (1ull << 33)) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
-  SNL_BY_TYPE(attend_simple_kernel, "attend_simple_kernel", dim3((unsigned)((items + kWarps - 1) / kWarps)),
-              dim3(kWarps * 32), (size_t)0, (cudaStream_t)stream, a);
+  const dim3 jg((unsigned)((items + kWarps - 1) / kWarps));
+  if (wide) SNL_PDL_LAUNCH("join_kernel", join_kernel<256>, jg, dim3(kWarps * 32), (size_t)0, s, a);
+  else SNL_PDL_LAUNCH("join_kernel", join_kernel<128>, jg, dim3(kWarps * 32), (size_t)0, s, a);
   return SNL_OK;
 }
 
