@@ -220,9 +220,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     const bool some = keys.x < keys.y;
     const int32_t lo0 = __reduce_min_sync(0xffffffffu, some ? keys.x : INT32_MAX);
     const int32_t hi1 = __reduce_max_sync(0xffffffffu, some ? keys.y : 0);
-    // a valid row without keys makes every tile a masked one
-    const int32_t lo1 = __reduce_max_sync(0xffffffffu, !valid ? 0 : some ? keys.x : INT32_MAX);
-    const int32_t hi0 = __reduce_min_sync(0xffffffffu, !valid ? INT32_MAX : keys.y);
+    const int32_t lo1 = __reduce_max_sync(0xffffffffu, some ? keys.x : 0);
+    const int32_t hi0 = __reduce_min_sync(0xffffffffu, some ? keys.y : INT32_MAX);
     if (lane == 0) {
       lohi[0][warp] = lo0;
       lohi[1][warp] = lo1;
@@ -355,7 +354,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = __all_sync(0xffffffffu, ok && !fail_sh && wait_mbar(bar, parity));
     };
+    // Tiles with a key that some row, some row of this warp (one without keys counts) does not see.
     auto masked_tile = [&](int32_t k0) { return k0 < lo1 || k0 + (int32_t)KT > hi0; };
+    const bool some = keys.x < keys.y;
+    const int32_t wlo = __reduce_max_sync(0xffffffffu, some ? keys.x : valid ? INT32_MAX : 0);
+    const int32_t whi = __reduce_min_sync(0xffffffffu, some ? keys.y : valid ? 0 : INT32_MAX);
     float l = 0.f, ref = -INFINITY;
     for (uint32_t i = wg; i < nt; i += 2) {
       const int32_t k0 = (int32_t)((j0 + i) * KT);
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
             s[c] = fmaf(-slope, fabsf(gap - (float)c), x);
           }
         }
-        if (masked) {
+        if (k0 < wlo || k0 + (int32_t)KT > whi) {
           const int32_t x0 = keys.x - k0, n = keys.y - keys.x;
 #pragma unroll
           for (uint32_t c = 0; c < KT; c++)
@@ -449,7 +452,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
             const uint32_t b0 = __vcmpeq2(x.x & inf2, inf2), b1 = __vcmpeq2(x.y & inf2, inf2),
                            b2 = __vcmpeq2(x.z & inf2, inf2), b3 = __vcmpeq2(x.w & inf2, inf2);
             if (b0 | b1 | b2 | b3) {
-              odd = true;
+              const int32_t key = k0 + (int32_t)(e * 16 / G::kGroup * 8 + e * 16 % 1024 / 128);
+              odd = odd || (key >= lo0 && key < hi1);
               tile[e] = make_uint4(x.x & ~b0, x.y & ~b1, x.z & ~b2, x.w & ~b3);
             }
           }
