@@ -41,56 +41,127 @@ __device__ __forceinline__ float rcp(float x) {
 // tanh x = 1 - 2 / (1 + e^2x): off by less than 2^-22, which tanh.approx (2^-11) is not.
 __device__ __forceinline__ float tanh_(float x) { return fmaf(-2.f, rcp(1.f + ex2(2.f * kLog2e * x)), 1.f); }
 
-// A bounded wait of about 0.15 s: the longest that one of these is due is some microseconds.
-__device__ __forceinline__ bool wait_mbar(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 28); }
 __device__ __forceinline__ void bar_sync(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(uint32_t id, uint32_t n) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+// One lane of the warp, known to the compiler as one: what it alone issues (MMAs) then takes
+// its operands from uniform registers. A region entered by lane == 0 took 67 cycles an MMA.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
 }
 
 // ---- tensor-core pieces ----------------------------------------------------------------
+//
+// Two CTAs of a cluster work as one (cta_group::2): each holds 128 rows of queries, half of
+// every K tile (64 of its 128 keys) and half of every V tile (half of head_dim), so each
+// byte of the cache is fetched and held once for 256 rows. One CTA's leader thread issues the
+// MMAs of both.
 
-// Keys of one tile and the tensor-memory columns of a CTA (512 in all): the output, the
-// queries (A operand of the scores, 16-bit pairs), and two score tiles that the
-// probabilities overwrite.
+// Shared and tensor memory of one CTA. A K or V tile's half is [8-key group][64-element
+// chunk][8 keys][128 bytes], 128-byte swizzled; queries are [chunk][128 rows][128 bytes].
+// Tensor memory: the output from column 0, two score tiles (which the probabilities
+// overwrite) from 256.
 template <int D>
 struct Geo {
-  static constexpr uint32_t KT = D == 256 ? 64 : 128;
-  static constexpr uint32_t kTile = KT * D * 2;  // bytes of a K or V tile (32 KB)
-  static constexpr uint32_t kGroup = D * 16;     // bytes of 8 keys
-  static constexpr uint32_t kStages = 6;
-  static constexpr uint32_t kSmem = kStages * kTile + 1024;
-  static constexpr uint32_t kO = 0, kQ = D, kS = D == 256 ? 384 : 256;
+  static constexpr uint32_t KT = 128;            // keys of a tile
+  static constexpr uint32_t kQ = 128 * D * 2;    // bytes of the queries
+  static constexpr uint32_t kTile = 64 * D * 2;  // bytes of half a K tile, of half a V tile
+  static constexpr uint32_t kGroupK = D * 16, kGroupV = D * 8;  // bytes of 8 keys
+  static constexpr uint32_t kStages = D == 256 ? 5 : 10;
+  static constexpr uint32_t kSmem = kQ + kStages * kTile + 1024;
+  static constexpr uint32_t kS = 256;
 };
 
 template <typename T>
-constexpr uint32_t idesc16(uint32_t n, bool b_mn) {  // D f32, A and B f16 or bf16, M = 128
+constexpr uint32_t idesc16(uint32_t n, bool b_mn) {  // D f32, A and B f16 or bf16, M = 256
   const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
-// A tile in shared memory is [8-key group][64-element chunk][8 keys][128 bytes], 128-byte
-// swizzled. As K (K-major) the groups are the 8-row groups, sbo apart; as V (MN-major) the
-// chunks are lbo and the groups sbo apart.
+// 128-byte swizzled operand. K-major: sbo between 8-row groups. MN-major: lbo between
+// chunks of 64 along MN, sbo between groups of 8 along K.
 __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// A from tensor memory.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// A from tensor memory.
+__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int c1, int c3, int c4, uint64_t* bar) {
+// Arrives on both CTAs' barriers once the MMAs issued so far have completed.
+__device__ __forceinline__ void commit2(uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(map), "r"(0), "r"(c1), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc2(uint32_t* dst) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t base) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address of the same shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// With release, what this thread wrote to memory is seen by who waits (about 1000 cycles at
+// cluster scope); tensor memory is ordered by its own fences and needs none.
+__device__ __forceinline__ void arrive_cluster(uint32_t bar, bool release) {
+  if (release) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded waits of about 0.15 s: the longest that one of these is due is some microseconds.
+// The second sees what the other CTA released.
+__device__ __forceinline__ bool wait_mbar(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 28); }
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity) {
+  if (try_wait_cluster(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!try_wait_cluster(bar, parity))
+    if (clock64() - t0 > (1ll << 28)) return false;
+  return true;
+}
+// Into this CTA, counted on a barrier that may be the other CTA's.
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int slot, int chunk, int head, int page,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(slot), "r"(chunk), "r"(head), "r"(page), "r"(bar)
       : "memory");
 }
 
@@ -130,13 +201,14 @@ struct TileInfo {
   int32_t t0, len;
 };
 
-// Slot s belongs to the last sequence b with start[b] / toks + b <= s: a sequence has at
+// Slot s belongs to the last sequence b with start[b] / (2 toks) + b <= s: a sequence has at
 // least as many slots as tiles, found without a sum over the batch. One warp.
 __device__ __forceinline__ TileInfo find_tile(const AttendArgs& a, uint32_t s, uint32_t lane) {
+  const uint32_t per = 2 * a.toks;
   uint32_t lo = 0, hi = a.c.n_seqs;
   while (hi - lo > 1) {
     const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const bool le = at < hi && (at == lo || (uint32_t)__ldg(a.c.start + at) / a.toks + at <= s);
+    const bool le = at < hi && (at == lo || (uint32_t)__ldg(a.c.start + at) / per + at <= s);
     const uint32_t n = __popc(__ballot_sync(0xffffffffu, le));
     const uint32_t below = lo + (max(n, 1u) - 1) * step;
     hi = min(hi, below + step);
@@ -144,12 +216,12 @@ __device__ __forceinline__ TileInfo find_tile(const AttendArgs& a, uint32_t s, u
   }
   TileInfo w{lo, 0, 0, 0, 0};
   const int2 rr = paged_rows(a.c, lo);
-  const uint32_t base = (uint32_t)rr.x / a.toks + lo;
+  const uint32_t base = (uint32_t)rr.x / per + lo;
   if (s < base) return w;
-  const uint32_t off = (s - base) * a.toks;
+  const uint32_t off = (s - base) * per;
   if (off >= (uint32_t)(rr.y - rr.x)) return w;
   w.row0 = rr.x + off;
-  w.toks = min(a.toks, (uint32_t)(rr.y - rr.x) - off);
+  w.toks = min(per, (uint32_t)(rr.y - rr.x) - off);
   w.len = paged_len(a.c, lo);
   w.t0 = w.len - (rr.y - rr.x) + (int32_t)off;
   return w;
@@ -159,30 +231,32 @@ constexpr uint32_t kSoftWarps = 8;
 constexpr uint32_t kAttendThreads = (kSoftWarps + 2) * 32;
 constexpr float kRefSlack = 8.f;  // log2 that scores may exceed the reference before O is rescaled
 
-// CTA = (tile of 128 (token, head) rows of one KV head's group, part of the keys). Warp 8
-// loads K and V tiles by TMA, 8 keys of one page at a time; warp 9 issues S = Q K^T and
-// O += P V (tcgen05, accumulators in tensor memory); two warpgroups turn the score tiles
-// into probabilities in turn, thread = row. The maximum that the exponentials refer to is
-// handed from tile to tile and moves only when a score exceeds it by kRefSlack.
+// A cluster = (two tiles of 128 (token, head) rows of one KV head's group, part of the
+// keys). Warp 8 of each CTA loads its halves of the K and V tiles by TMA, 8 keys of one page
+// at a time; warp 9 of the first issues S = Q K^T and O += P V; two warpgroups of each CTA
+// turn the score tiles into probabilities in turn, thread = row. The maximum that the
+// exponentials refer to is handed from tile to tile and moves only when a score exceeds it
+// by kRefSlack.
 template <typename T, int D, bool GENERAL>
-__global__ void __launch_bounds__(kAttendThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using G = Geo<D>;
   constexpr uint32_t KT = G::KT, NS = G::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[NS], empty[NS], s_full[2], p_ready[2], pv_done[2], drained;
+  __shared__ uint64_t full[NS], empty[NS], s_full[2], p_ready[2], pv_done[2], v_landed[2], drained;
   __shared__ uint32_t tmem_sh;
   __shared__ TileInfo info_sh;
   __shared__ int32_t lohi[4][kSoftWarps / 2];  // per warp: least and largest lo, least and largest hi
-  __shared__ float ref_sh[128], l_sh[2][128], lref_sh[2][128];
+  __shared__ float ref_sh[128];
   __shared__ volatile int fail_sh;
   __shared__ int odd_v;
   pdl_trigger();
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t kh = blockIdx.x % a.c.n_kv, unit = blockIdx.x / a.c.n_kv;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
+  const uint32_t kh = (blockIdx.x / 2) % a.c.n_kv, unit = (blockIdx.x / 2) / a.c.n_kv;
   const uint32_t split = unit % a.n_split, slot = a.slots - 1 - unit / a.n_split;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* smem_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* smem = smem_q + G::kQ;
 
   if (tid == 0) {
     for (uint32_t s = 0; s < NS; s++) {
@@ -191,15 +265,16 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], kSoftWarps / 2);
+      mbar_init(&p_ready[s], kSoftWarps);  // half of the warps of both CTAs
       mbar_init(&pv_done[s], 1);
+      mbar_init(&v_landed[s], 1);
     }
     mbar_init(&drained, 1);
     fail_sh = 0;
     odd_v = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(&tmem_sh, 512);
+  if (warp == 9) tmem_alloc2(&tmem_sh);
   pdl_wait();
   if (warp == 8) {
     const TileInfo w = find_tile(a, slot, lane);
@@ -209,49 +284,48 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_sh;
-  const TileInfo w = info_sh;
+  const TileInfo w = info_sh;  // of the cluster: up to 2 a.toks tokens
 
   // Row of this thread (both warpgroups hold all 128): token and head, its keys.
-  const uint32_t row = tid & 127, tok = row / a.group, head = kh * a.group + row % a.group;
-  const bool valid = warp < kSoftWarps && tok < w.toks;
+  const uint32_t row = tid & 127, tok0 = row / a.group, head = kh * a.group + row % a.group;
+  const uint32_t tok = tok0 + rank * a.toks;
+  const bool mine = warp < kSoftWarps && tok0 < a.toks, valid = mine && tok < w.toks;
   int2 keys = make_int2(0, 0);
   if (valid) keys = paged_keys(a.m, w.row0 + tok, w.t0 + (int32_t)tok, w.len);
   if (warp < kSoftWarps / 2) {
-    const bool some = keys.x < keys.y;
-    const int32_t lo0 = __reduce_min_sync(0xffffffffu, some ? keys.x : INT32_MAX);
-    const int32_t hi1 = __reduce_max_sync(0xffffffffu, some ? keys.y : 0);
-    const int32_t lo1 = __reduce_max_sync(0xffffffffu, some ? keys.x : 0);
-    const int32_t hi0 = __reduce_min_sync(0xffffffffu, some ? keys.y : INT32_MAX);
+    // The same row of the other CTA too: both walk the same tiles.
+    const uint32_t tok1 = tok0 + (rank ^ 1) * a.toks;
+    int2 k1 = make_int2(0, 0);
+    if (mine && tok1 < w.toks) k1 = paged_keys(a.m, w.row0 + tok1, w.t0 + (int32_t)tok1, w.len);
+    const bool s0 = keys.x < keys.y, s1 = k1.x < k1.y;
+    const int32_t lo0 = min(s0 ? keys.x : INT32_MAX, s1 ? k1.x : INT32_MAX), lo1 = max(s0 ? keys.x : 0, s1 ? k1.x : 0);
+    const int32_t hi0 = min(s0 ? keys.y : INT32_MAX, s1 ? k1.y : INT32_MAX), hi1 = max(s0 ? keys.y : 0, s1 ? k1.y : 0);
+    const int32_t r0 = __reduce_min_sync(0xffffffffu, lo0), r1 = __reduce_max_sync(0xffffffffu, lo1);
+    const int32_t r2 = __reduce_min_sync(0xffffffffu, hi0), r3 = __reduce_max_sync(0xffffffffu, hi1);
     if (lane == 0) {
-      lohi[0][warp] = lo0;
-      lohi[1][warp] = lo1;
-      lohi[2][warp] = hi0;
-      lohi[3][warp] = hi1;
+      lohi[0][warp] = r0;
+      lohi[1][warp] = r1;
+      lohi[2][warp] = r2;
+      lohi[3][warp] = r3;
     }
   }
   const float sl = fmaxf(fabsf(a.m.scale) * kLog2e, 1e-30f);  // not 0: -inf of a masked score has to stay
   if (warp < kSoftWarps) {
-    // Queries into tensor memory, lane = row, the sign of the scale folded in.
-    const uint32_t wg = warp >> 2, flip = a.m.scale < 0.f ? 0x80008000u : 0u;
-    const uint16_t* src = a.q + (uint64_t)(w.row0 + tok) * a.p.q_row + (uint64_t)head * a.p.q_head;
-    const uint32_t lanes = ((warp & 3) * 32) << 16;
-#pragma unroll
-    for (uint32_t c = 0; c < D / 4; c += 32) {
-      uint32_t r[32];
-#pragma unroll
-      for (uint32_t i = 0; i < 32; i += 4) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (valid) x = __ldg(reinterpret_cast<const uint4*>(src + 2 * (wg * (D / 4) + c + i)));
-        r[i] = x.x ^ flip, r[i + 1] = x.y ^ flip, r[i + 2] = x.z ^ flip, r[i + 3] = x.w ^ flip;
-      }
-      __syncwarp();
-      tm_st32(tmem + lanes + G::kQ + wg * (D / 4) + c, r);
+    // Queries into shared memory, the sign of the scale folded in.
+    const uint32_t flip = a.m.scale < 0.f ? 0x80008000u : 0u;
+    for (uint32_t e = tid; e < G::kQ / 16; e += kSoftWarps * 32) {
+      const uint32_t r = e / (D / 8), u = e % (D / 8), t = r / a.group + rank * a.toks;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r / a.group < a.toks && t < w.toks)
+        x = __ldg(reinterpret_cast<const uint4*>(a.q + (uint64_t)(w.row0 + t) * a.p.q_row +
+                                                 (uint64_t)(kh * a.group + r % a.group) * a.p.q_head + 8 * u));
+      x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+      *reinterpret_cast<uint4*>(smem_q + (u / 8) * 16384 + r * 128 + ((u % 8 ^ r % 8) << 4)) = x;
     }
-    tm_wait_st();
+    fence_proxy_async_smem();
   }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
+  cluster_sync();  // barriers and queries of both CTAs are there
   int32_t lo0 = lohi[0][0], lo1 = lohi[1][0], hi0 = lohi[2][0], hi1 = lohi[3][0];
 #pragma unroll
   for (uint32_t i = 1; i < kSoftWarps / 2; i++) {
@@ -267,10 +341,15 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
   // The i-th load: K tiles run one ahead of V tiles, as the MMAs do.
   auto k_load = [&](uint32_t i) { return i == 0 ? 0u : 2 * i - 1; };
   auto v_load = [&](uint32_t i) { return i + 1 == nt ? 2 * nt - 1 : 2 * i + 2; };
+  // Tiles with a key that some row of the cluster does not see.
+  auto masked_tile = [&](uint32_t j) { return (int32_t)(j * KT) < lo1 || (int32_t)(j * KT + KT) > hi0; };
 
+  // Results of the softmax warps, used after the loop.
+  float l = 0.f, ref = -INFINITY;
   if (warp == 8) {
-    // Lane g < KT / 8 loads the tile's g-th 8 keys; keys past the length and pages outside
-    // the cache come from a page coordinate past the end, which reads zeros.
+    // Lane g < 16 loads 8 keys of the V tile, and of the K tile where they are of this CTA's
+    // half; keys past the length and pages outside the cache come from a page coordinate past
+    // the end, which reads zeros.
     auto page_of = [&](uint32_t i) -> int32_t {
       const uint32_t key = (j0 + i) * KT + 8 * lane;
       int32_t p = -1;
@@ -279,34 +358,41 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     };
     int32_t now = page_of(0), next = page_of(1), prev = now;
     uint32_t n = 0;
-    auto load = [&](const CUtensorMap* map, uint32_t i, int32_t page) -> bool {
+    auto load = [&](bool is_k, uint32_t i, int32_t page) -> bool {
       const uint32_t st = n % NS;
       bool ok = n < NS || wait_mbar(&empty[st], (n / NS - 1) & 1);
       ok = __all_sync(0xffffffffu, ok && !fail_sh);
       if (!ok) return false;
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], G::kTile);
+      if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&full[st], 2 * G::kTile);
       __syncwarp();
-      if (lane < KT / 8)
-        tma_load_5d(smem_u32(smem + st * G::kTile + lane * G::kGroup), map,
-                    (int)(((j0 + i) * KT + 8 * lane) & ((1u << a.c.shift) - 1)), (int)kh, page, &full[st]);
+      const uint32_t bar = in_cta(&full[st], 0), dst = smem_u32(smem + st * G::kTile);
+      const int slot0 = (int)(((j0 + i) * KT + 8 * lane) & ((1u << a.c.shift) - 1));
+      if (is_k && lane / 8 == rank)
+        tma_load_5d(dst + (lane % 8) * G::kGroupK, &kmap, slot0, 0, (int)kh, page, bar);
+      if (!is_k && lane < KT / 8)
+        tma_load_5d(dst + lane * G::kGroupV, &vmap, slot0, (int)(rank * (D / 128)), (int)kh, page, bar);
       n++;
       return true;
     };
     bool ok = true;
     for (uint32_t i = 0; ok && i <= nt; i++) {
-      if (i < nt) ok = load(&kmap, i, now);
-      if (ok && i > 0) ok = load(&vmap, i - 1, prev);
+      if (i < nt) ok = load(true, i, now);
+      if (ok && i > 0) ok = load(false, i - 1, prev);
       prev = now;
       now = next;
       next = page_of(i + 2);
     }
     if (!ok && lane == 0) fail_sh = 1;
-    // every load lands before the CTA ends, whatever became of its readers
-    for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) (void)wait_mbar(&full[i % NS], (i / NS) & 1);
+    // every load of both CTAs lands before they part, whatever became of its readers
+    if (rank == 0)
+      for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) (void)wait_mbar(&full[i % NS], (i / NS) & 1);
   } else if (warp == 9) {
-    if (lane == 0) {
+    if (rank == 0 && elect_one()) {
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && !fail_sh && wait_mbar(bar, parity); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!mbar_try_wait(bar, parity)) ok = ok && !fail_sh && wait_mbar(bar, parity);
+      };
+      const uint32_t qbase = smem_u32(smem_q);
       auto scores = [&](uint32_t i) {
         const uint32_t n = k_load(i), st = n % NS;
         wait(&full[st], (n / NS) & 1);
@@ -315,54 +401,60 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
         const uint32_t base = smem_u32(smem + st * G::kTile);
 #pragma unroll
         for (uint32_t kk = 0; kk < D / 16; kk++)
-          mma_ts(tmem + G::kS + (i & 1) * KT, tmem + G::kQ + kk * 8,
-                 tile_desc(base + (kk / 4) * 1024 + (kk % 4) * 32, 16, G::kGroup), idesc16<T>(KT, false), kk != 0);
-        tc_commit(&empty[st]);
-        tc_commit(&s_full[i & 1]);
+          mma2_ss(tmem + G::kS + (i & 1) * KT, tile_desc(qbase + (kk / 4) * 16384 + (kk % 4) * 32, 16, 1024),
+                  tile_desc(base + (kk / 4) * 1024 + (kk % 4) * 32, 16, G::kGroupK), idesc16<T>(KT, false), kk != 0);
+        commit2(&empty[st]);
+        commit2(&s_full[i & 1]);
       };
       if (nt) scores(0);
       for (uint32_t i = 0; ok && i < nt; i++) {
         if (i + 1 < nt) scores(i + 1);
         const uint32_t n = v_load(i), st = n % NS;
         wait(&full[st], (n / NS) & 1);
-        wait(&p_ready[i & 1], (i >> 1) & 1);
+        if (ok && masked_tile(j0 + i)) {  // the warpgroups look through it first
+          arrive_cluster(in_cta(&v_landed[i & 1], 0), true);
+          arrive_cluster(in_cta(&v_landed[i & 1], 1), true);
+          ok = wait_cluster(&p_ready[i & 1], (i >> 1) & 1);
+        } else {
+          wait(&p_ready[i & 1], (i >> 1) & 1);
+        }
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = smem_u32(smem + st * G::kTile);
 #pragma unroll
         for (uint32_t kk = 0; kk < KT / 16; kk++)
-          mma_ts(tmem + G::kO, tmem + G::kS + (i & 1) * KT + kk * 8, tile_desc(base + kk * 2 * G::kGroup, 1024, G::kGroup),
-                 idesc16<T>(D, true), (i | kk) != 0);
-        tc_commit(&empty[st]);
-        tc_commit(&pv_done[i & 1]);
+          mma2_ts(tmem, tmem + G::kS + (i & 1) * KT + kk * 8, tile_desc(base + kk * 2 * G::kGroupV, 1024, G::kGroupV),
+                  idesc16<T>(D, true), (i | kk) != 0);
+        commit2(&empty[st]);
+        commit2(&pv_done[i & 1]);
       }
       if (!ok) {
         fail_sh = 1;
         report_timeout(a.c.err);
       }
-      tc_commit(&drained);  // and every MMA before the tensor memory is given back
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&drained))
+                   : "memory");  // and every MMA before the tensor memory is given back
       (void)wait_mbar(&drained, 0);
     }
     __syncwarp();
   } else {
-    const uint32_t wg = warp >> 2;
-    const uint32_t lanes = ((warp & 3) * 32) << 16;
+    const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16, tm_s = tmem + lanes + G::kS + wg * KT;
     const bool live = __any_sync(0xffffffffu, valid);
     const float slope = GENERAL && a.m.slopes && valid ? __ldg(a.m.slopes + head) * kLog2e : 0.f;
-    const float cap = a.m.cap, pre = GENERAL && cap > 0.f ? a.m.scale / cap : 0.f;
+    const float cap = a.m.cap, pre = GENERAL && cap > 0.f ? fabsf(a.m.scale / cap) : 0.f;
+    const uint32_t ready = in_cta(&p_ready[wg], 0);
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = __all_sync(0xffffffffu, ok && !fail_sh && wait_mbar(bar, parity));
+      ok = __all_sync(0xffffffffu, ok && (mbar_try_wait(bar, parity) || (!fail_sh && wait_mbar(bar, parity))));
+      if (!ok) fail_sh = 1;
     };
-    // Tiles with a key that some row, some row of this warp (one without keys counts) does not see.
-    auto masked_tile = [&](int32_t k0) { return k0 < lo1 || k0 + (int32_t)KT > hi0; };
+    // Tiles with a key that some row of this warp (one without keys counts) does not see.
     const bool some = keys.x < keys.y;
     const int32_t wlo = __reduce_max_sync(0xffffffffu, some ? keys.x : valid ? INT32_MAX : 0);
     const int32_t whi = __reduce_min_sync(0xffffffffu, some ? keys.y : valid ? 0 : INT32_MAX);
-    float l = 0.f, ref = -INFINITY;
+    uint32_t landed = 0;
     for (uint32_t i = wg; i < nt; i += 2) {
       const int32_t k0 = (int32_t)((j0 + i) * KT);
-      const bool masked = masked_tile(k0);
       float s[KT];
       uint32_t* r = reinterpret_cast<uint32_t*>(s);
       wait(&s_full[wg], (i >> 1) & 1);
@@ -370,14 +462,13 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
       float mx = -INFINITY;
       if (live) {
 #pragma unroll
-        for (uint32_t c = 0; c < KT; c += 32) tm_ld32(tmem + lanes + G::kS + wg * KT + c, r + c);
+        for (uint32_t c = 0; c < KT; c += 32) tm_ld32(tm_s + c, r + c);
         tm_wait_ld<KT>(r);
         if constexpr (GENERAL) {
           const float gap = (float)(w.t0 + (int32_t)tok - k0);
 #pragma unroll
           for (uint32_t c = 0; c < KT; c++) {
-            // the sign of the scale is in the queries already
-            float x = cap > 0.f ? cap * kLog2e * tanh_(s[c] * fabsf(pre)) : s[c] * sl;
+            const float x = cap > 0.f ? cap * kLog2e * tanh_(s[c] * pre) : s[c] * sl;
             s[c] = fmaf(-slope, fabsf(gap - (float)c), x);
           }
         }
@@ -400,10 +491,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
         before = ref_sh[row];
       }
       const float now = mx > before + kRefSlack ? mx : before;
-      if (i + 1 < nt) {
-        ref_sh[row] = now;
-        bar_arrive(1 + (i & 1), 256);
-      }
+      ref_sh[row] = now;
+      if (i + 1 < nt) bar_arrive(1 + (i & 1), 256);
       if (i > 0 && __any_sync(0xffffffffu, now != before)) {
         wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1);
         tc_fence_after();
@@ -411,11 +500,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
 #pragma unroll 1
         for (uint32_t c = 0; c < D; c += 32) {
           uint32_t o[32];
-          tm_ld32(tmem + lanes + G::kO + c, o);
+          tm_ld32(tmem + lanes + c, o);
           tm_wait_ld<32>(o);
 #pragma unroll
           for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tm_st32(tmem + lanes + G::kO + c, o);
+          tm_st32(tmem + lanes + c, o);
         }
         tm_wait_st();
       }
@@ -434,15 +523,17 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-        for (uint32_t c = 0; c < KT / 2; c += 32) tm_st32(tmem + lanes + G::kS + wg * KT + c, r + c);
+        for (uint32_t c = 0; c < KT / 2; c += 32) tm_st32(tm_s + c, r + c);
         tm_wait_st();
       }
+      const bool masked = masked_tile(j0 + i);
       if (masked) {
         // A row's probability for a key that it does not see is 0, but 0 * NaN is not: values that
         // are not finite leave the tile, and reach the rows that see them at the end.
-        const uint32_t n = v_load(i);
-        wait(&full[n % NS], (n / NS) & 1);
+        ok = __all_sync(0xffffffffu, ok && wait_cluster(&v_landed[wg], landed & 1));
+        landed++;
         if (ok) {
+          const uint32_t n = v_load(i);
           constexpr uint32_t inf2 = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
           uint4* tile = reinterpret_cast<uint4*>(smem + (n % NS) * G::kTile);
           bool odd = false;
@@ -452,33 +543,41 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
             const uint32_t b0 = __vcmpeq2(x.x & inf2, inf2), b1 = __vcmpeq2(x.y & inf2, inf2),
                            b2 = __vcmpeq2(x.z & inf2, inf2), b3 = __vcmpeq2(x.w & inf2, inf2);
             if (b0 | b1 | b2 | b3) {
-              const int32_t key = k0 + (int32_t)(e * 16 / G::kGroup * 8 + e * 16 % 1024 / 128);
+              const int32_t key = k0 + (int32_t)(e * 16 / G::kGroupV * 8 + e * 16 % 1024 / 128);
               odd = odd || (key >= lo0 && key < hi1);
               tile[e] = make_uint4(x.x & ~b0, x.y & ~b1, x.z & ~b2, x.w & ~b3);
             }
           }
-          if (odd) odd_v = 1;
+          if (odd) {
+            odd_v = 1;
+            asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(in_cta(&odd_v, rank ^ 1)) : "memory");
+          }
           fence_proxy_async_smem();
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[wg]);
-      if (i + 1 == nt) ref_sh[row] = now;
+      if (lane == 0) arrive_cluster(ready, masked);
     }
-    // Sums of both warpgroups, referred to the last reference.
-    l_sh[wg][row] = l;
-    lref_sh[wg][row] = ref;
     if (nt) wait(&pv_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1);
+  }
+  __syncwarp();
+  cluster_sync();  // nothing of one CTA is used by the other after this
+  if (warp < kSoftWarps) {
+    const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16;
+    const bool live = __any_sync(0xffffffffu, valid);
+    // Sums of both warpgroups, referred to the last reference; the tiles' memory is free now.
+    float2* lsum = reinterpret_cast<float2*>(smem);
+    lsum[wg * 128 + row] = make_float2(l, ref);
     bar_sync(3, 256);
     tc_fence_after();
     const float fin = nt ? ref_sh[row] : -INFINITY;
     l = 0.f;
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-      const float rg = lref_sh[g][row];
-      if (rg != -INFINITY) l += rg == fin ? l_sh[g][row] : l_sh[g][row] * ex2(rg - fin);
-      else if (l_sh[g][row] != 0.f) l = NAN;  // only scores of NaN
+      const float2 x = lsum[g * 128 + row];
+      if (x.y != -INFINITY) l += x.y == fin ? x.x : x.x * ex2(x.y - fin);
+      else if (x.x != 0.f) l = NAN;  // only scores of NaN
     }
     const bool parts = a.n_split > 1;
     const uint64_t rh = (uint64_t)(w.row0 + tok) * a.p.n_heads + head;
@@ -493,13 +592,13 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
       float* o = reinterpret_cast<float*>(r);
       __syncwarp();
       if (nt) {
-        tm_ld32(tmem + lanes + G::kO + c, r);
+        tm_ld32(tmem + lanes + c, r);
         tm_wait_ld<32>(r);
       }
       if (!valid || (parts && nt == 0)) continue;
       if (odd_v) {
         for (uint32_t j = j0; j < j0 + nt; j++) {
-          if (!masked_tile((int32_t)(j * KT))) continue;
+          if (!masked_tile(j)) continue;
           const int32_t k1 = min(min((int32_t)((j + 1) * KT), keys.y), end);
           for (int32_t key = max((int32_t)(j * KT), keys.x); key < k1; key++) {
             const int32_t page = paged_page(a.c, w.b, key);
@@ -543,7 +642,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 9) tmem_dealloc2(tmem);
 }
 
 // Joins the parts of a row: one warp per (row, head), over the parts that its keys touch.
@@ -661,10 +760,10 @@ AttendPlan plan_attend(const snl_paged_cache& c, const snl_paged_batch& b, uint3
   AttendPlan pl{};
   const uint32_t group = n_heads / c.n_kv;
   pl.toks = 128 / group;
-  pl.slots = b.n_rows / pl.toks + b.n_seqs;
+  pl.slots = b.n_rows / (2 * pl.toks) + b.n_seqs;
   const uint64_t max_len = std::min<uint64_t>(b.max_len, (uint64_t)b.table_stride * c.page_size);
   const uint64_t units = (uint64_t)std::min<uint64_t>(pl.slots, b.n_rows) * c.n_kv;
-  const double per_key = c.head_dim == 256 ? 0.015 : 0.008, sms = sm_count();
+  const double per_key = c.head_dim == 256 ? 0.011 : 0.006, sms = std::max(1, sm_count() / 2);
   double best = 1e30;
   pl.n_split = 1;
   for (uint32_t n = 1; n <= 64; n++) {
@@ -684,14 +783,15 @@ AttendPlan plan_attend(const snl_paged_cache& c, const snl_paged_batch& b, uint3
   return pl;
 }
 
-// The pages as (64 elements, slot, chunk of 64, head, page): a box is 8 slots of a head.
-int page_map(CUtensorMap* map, const snl_paged_cache& c, void* base) {
+// The pages as (64 elements, slot, chunk of 64, head, page): a box is 8 slots of a head, or of half
+// of one.
+int page_map(CUtensorMap* map, const snl_paged_cache& c, void* base, uint32_t chunks) {
   PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
   if (!enc) return fail(SNL_E_CUDA, "paged cache: cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[5] = {64, c.page_size, c.head_dim / 64, c.n_kv, c.n_pages};
   const cuuint64_t str[4] = {c.slot_stride * 2, 128, c.n_kv > 1 ? c.head_stride * 2 : 128,
                              c.n_pages > 1 ? c.page_stride * 2 : 128};
-  const cuuint32_t box[5] = {64, 8, c.head_dim / 64, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+  const cuuint32_t box[5] = {64, 8, chunks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(map, c.type == SNL_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                          base, dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -742,11 +842,11 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
   if (!work) return fail(SNL_E_INVALID, w + ": null argument");
   if (b->n_rows == 0 || b->n_seqs == 0) return SNL_OK;
   SNL_TRY(paged_error_word(&a.c.err));
-  const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv;
+  const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv * 2;
   if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
   CUtensorMap km, vm;
-  SNL_TRY(page_map(&km, *c, c->k));
-  SNL_TRY(page_map(&vm, *c, c->v));
+  SNL_TRY(page_map(&km, *c, c->k, c->head_dim / 64));
+  SNL_TRY(page_map(&vm, *c, c->v, c->head_dim / 128));
   a.p = *p;
   a.q = static_cast<const uint16_t*>(q);
   a.gate = gate;
