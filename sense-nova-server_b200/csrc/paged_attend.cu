@@ -41,10 +41,23 @@ __device__ __forceinline__ float rcp(float x) {
 // tanh x = 1 - 2 / (1 + e^2x): off by less than 2^-22, which tanh.approx (2^-11) is not.
 __device__ __forceinline__ float tanh_(float x) { return fmaf(-2.f, rcp(1.f + ex2(2.f * kLog2e * x)), 1.f); }
 
-__device__ __forceinline__ void bar_sync(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-__device__ __forceinline__ void bar_arrive(uint32_t id, uint32_t n) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ void bar_sync(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 // One lane of the warp, known to the compiler as one: what it alone issues (MMAs) then takes
 // its operands from uniform registers. A region entered by lane == 0 took 67 cycles an MMA.
 __device__ __forceinline__ bool elect_one() {
@@ -71,7 +84,7 @@ struct Geo {
   static constexpr uint32_t kTile = 64 * D * 2;  // bytes of half a K tile, of half a V tile
   static constexpr uint32_t kGroupK = D * 16, kGroupV = D * 8;  // bytes of 8 keys
   static constexpr uint32_t kStages = D == 256 ? 5 : 10;
-  static constexpr uint32_t kSmem = kQ + kStages * kTile + 1024;
+  static constexpr uint32_t kSmem = kQ + kStages * kTile;
   static constexpr uint32_t kS = 256;
 };
 
@@ -234,29 +247,31 @@ constexpr float kRefSlack = 8.f;  // log2 that scores may exceed the reference b
 // A cluster = (two tiles of 128 (token, head) rows of one KV head's group, part of the
 // keys). Warp 8 of each CTA loads its halves of the K and V tiles by TMA, 8 keys of one page
 // at a time; warp 9 of the first issues S = Q K^T and O += P V; two warpgroups of each CTA
-// turn the score tiles into probabilities in turn, thread = row. The maximum that the
-// exponentials refer to is handed from tile to tile and moves only when a score exceeds it
-// by kRefSlack.
+// turn half of a score tile's columns into probabilities each, thread = row. The maximum
+// that the exponentials refer to moves only when a score exceeds it by kRefSlack.
 template <typename T, int D, bool GENERAL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using G = Geo<D>;
   constexpr uint32_t KT = G::KT, NS = G::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[NS], empty[NS], s_full[2], p_ready[2], pv_done[2], v_landed[2], drained;
+  extern __shared__ __align__(1024) uint8_t smem_q[];
+  __shared__ uint64_t full[NS], empty[NS], s_full[2], p_ready[2], pv_done[2], v_landed, drained;
   __shared__ uint32_t tmem_sh;
   __shared__ TileInfo info_sh;
   __shared__ int32_t lohi[4][kSoftWarps / 2];  // per warp: least and largest lo, least and largest hi
-  __shared__ float ref_sh[128];
+  __shared__ float max_sh[2][2][128];
   __shared__ volatile int fail_sh;
   __shared__ int odd_v;
   pdl_trigger();
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
   const uint32_t kh = (blockIdx.x / 2) % a.c.n_kv, unit = (blockIdx.x / 2) / a.c.n_kv;
   const uint32_t split = unit % a.n_split, slot = a.slots - 1 - unit / a.n_split;
-  uint8_t* smem_q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* smem = smem_q + G::kQ;
+  if (smem_u32(smem_q) & 1023) {  // the swizzle needs it; the same for every CTA
+    report_timeout(a.c.err);
+    return;
+  }
 
   if (tid == 0) {
     for (uint32_t s = 0; s < NS; s++) {
@@ -265,10 +280,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], kSoftWarps);  // half of the warps of both CTAs
+      mbar_init(&p_ready[s], 2 * kSoftWarps);  // the warps of both CTAs
       mbar_init(&pv_done[s], 1);
-      mbar_init(&v_landed[s], 1);
     }
+    mbar_init(&v_landed, 1);
     mbar_init(&drained, 1);
     fail_sh = 0;
     odd_v = 0;
@@ -412,8 +427,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
         const uint32_t n = v_load(i), st = n % NS;
         wait(&full[st], (n / NS) & 1);
         if (ok && masked_tile(j0 + i)) {  // the warpgroups look through it first
-          arrive_cluster(in_cta(&v_landed[i & 1], 0), true);
-          arrive_cluster(in_cta(&v_landed[i & 1], 1), true);
+          arrive_cluster(in_cta(&v_landed, 0), true);
+          arrive_cluster(in_cta(&v_landed, 1), true);
           ok = wait_cluster(&p_ready[i & 1], (i >> 1) & 1);
         } else {
           wait(&p_ready[i & 1], (i >> 1) & 1);
@@ -438,11 +453,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     }
     __syncwarp();
   } else {
-    const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16, tm_s = tmem + lanes + G::kS + wg * KT;
+    // Half of a tile's columns each: warps w and w + 4 hold the same 32 rows.
+    const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16;
     const bool live = __any_sync(0xffffffffu, valid);
     const float slope = GENERAL && a.m.slopes && valid ? __ldg(a.m.slopes + head) * kLog2e : 0.f;
     const float cap = a.m.cap, pre = GENERAL && cap > 0.f ? fabsf(a.m.scale / cap) : 0.f;
-    const uint32_t ready = in_cta(&p_ready[wg], 0);
+    const uint32_t ready[2] = {in_cta(&p_ready[0], 0), in_cta(&p_ready[1], 0)};
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = __all_sync(0xffffffffu, ok && (mbar_try_wait(bar, parity) || (!fail_sh && wait_mbar(bar, parity))));
@@ -452,85 +468,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     const bool some = keys.x < keys.y;
     const int32_t wlo = __reduce_max_sync(0xffffffffu, some ? keys.x : valid ? INT32_MAX : 0);
     const int32_t whi = __reduce_min_sync(0xffffffffu, some ? keys.y : valid ? 0 : INT32_MAX);
+    constexpr uint32_t NC = KT / 2;  // columns of this warp
     uint32_t landed = 0;
-    for (uint32_t i = wg; i < nt; i += 2) {
-      const int32_t k0 = (int32_t)((j0 + i) * KT);
-      float s[KT];
+    for (uint32_t i = 0; i < nt; i++) {
+      const int32_t k0 = (int32_t)((j0 + i) * KT + wg * NC);
+      const uint32_t tm_s = tmem + lanes + G::kS + (i & 1) * KT;
+      float s[NC];
       uint32_t* r = reinterpret_cast<uint32_t*>(s);
-      wait(&s_full[wg], (i >> 1) & 1);
+      wait(&s_full[i & 1], (i >> 1) & 1);
       tc_fence_after();
-      float mx = -INFINITY;
       if (live) {
 #pragma unroll
-        for (uint32_t c = 0; c < KT; c += 32) tm_ld32(tm_s + c, r + c);
-        tm_wait_ld<KT>(r);
+        for (uint32_t c = 0; c < NC; c += 32) tm_ld32(tm_s + wg * NC + c, r + c);
+        tm_wait_ld<NC>(r);
         if constexpr (GENERAL) {
           const float gap = (float)(w.t0 + (int32_t)tok - k0);
 #pragma unroll
-          for (uint32_t c = 0; c < KT; c++) {
+          for (uint32_t c = 0; c < NC; c++) {
             const float x = cap > 0.f ? cap * kLog2e * tanh_(s[c] * pre) : s[c] * sl;
             s[c] = fmaf(-slope, fabsf(gap - (float)c), x);
           }
         }
-        if (k0 < wlo || k0 + (int32_t)KT > whi) {
+        if (k0 < wlo || k0 + (int32_t)NC > whi) {
           const int32_t x0 = keys.x - k0, n = keys.y - keys.x;
 #pragma unroll
-          for (uint32_t c = 0; c < KT; c++)
+          for (uint32_t c = 0; c < NC; c++)
             if ((uint32_t)((int32_t)c - x0) >= (uint32_t)n) s[c] = -INFINITY;
         }
         float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (uint32_t c = 4; c < KT; c++) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
-        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        for (uint32_t c = 4; c < NC; c++) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if constexpr (!GENERAL) mx *= sl;
-      }
-      // The reference passes from tile to tile between the warpgroups.
-      float before = -INFINITY;
-      if (i > 0) {
-        bar_sync(1 + ((i - 1) & 1), 256);
-        before = ref_sh[row];
-      }
-      const float now = mx > before + kRefSlack ? mx : before;
-      ref_sh[row] = now;
-      if (i + 1 < nt) bar_arrive(1 + (i & 1), 256);
-      if (i > 0 && __any_sync(0xffffffffu, now != before)) {
-        wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1);
-        tc_fence_after();
-        const float f = now != before ? ex2(before - now) : 1.f;
+        // The tile's maximum from both halves; after this barrier both have read their scores, which
+        // the probabilities overwrite.
+        max_sh[i & 1][wg][row] = mx;
+        bar_sync(1 + (warp & 3), 64);
+        mx = fmaxf(mx, max_sh[i & 1][wg ^ 1][row]);
+        const float now = mx > ref + kRefSlack ? mx : ref;
+        if (i > 0 && __any_sync(0xffffffffu, now != ref)) {
+          wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1);
+          tc_fence_after();
+          const float f = now != ref ? ex2(ref - now) : 1.f;
 #pragma unroll 1
-        for (uint32_t c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tm_ld32(tmem + lanes + c, o);
-          tm_wait_ld<32>(o);
+          for (uint32_t c = wg * (D / 2); c < (wg + 1) * (D / 2); c += 32) {
+            uint32_t o[32];
+            tm_ld32(tmem + lanes + c, o);
+            tm_wait_ld<32>(o);
 #pragma unroll
-          for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tm_st32(tmem + lanes + c, o);
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tm_st32(tmem + lanes + c, o);
+          }
+          l *= f;
         }
-        tm_wait_st();
-      }
-      if (now != ref) l *= ex2(ref - now);
-      ref = now;
-      const float zero = now == -INFINITY ? 0.f : now;
-      if (live) {
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        ref = now;
+        const float zero = now == -INFINITY ? 0.f : now;
+        float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-        for (uint32_t c = 0; c < KT; c += 2) {
-          const float p0 = ex2(GENERAL ? s[c] - zero : fmaf(s[c], sl, -zero));
-          const float p1 = ex2(GENERAL ? s[c + 1] - zero : fmaf(s[c + 1], sl, -zero));
-          sum[c & 2] += p0;
-          sum[(c & 2) + 1] += p1;
-          r[c / 2] = pack2(p0, p1, T());
+        for (uint32_t c = 0; c < NC; c += 2) {
+          float2 p = make_float2(s[c], s[c + 1]);
+          p = GENERAL ? make_float2(p.x - zero, p.y - zero) : fma2(p, make_float2(sl, sl), make_float2(-zero, -zero));
+          p = make_float2(ex2(p.x), ex2(p.y));
+          sum[(c / 2) & 1] = add2(sum[(c / 2) & 1], p);
+          r[c / 2] = pack2(p.x, p.y, T());
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-        for (uint32_t c = 0; c < KT / 2; c += 32) tm_st32(tm_s + c, r + c);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
+        tm_st32(tm_s + wg * (NC / 2), r);
         tm_wait_st();
       }
       const bool masked = masked_tile(j0 + i);
       if (masked) {
         // A row's probability for a key that it does not see is 0, but 0 * NaN is not: values that
         // are not finite leave the tile, and reach the rows that see them at the end.
-        ok = __all_sync(0xffffffffu, ok && wait_cluster(&v_landed[wg], landed & 1));
+        ok = __all_sync(0xffffffffu, ok && wait_cluster(&v_landed, landed & 1));
         landed++;
         if (ok) {
           const uint32_t n = v_load(i);
@@ -538,12 +549,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
           uint4* tile = reinterpret_cast<uint4*>(smem + (n % NS) * G::kTile);
           bool odd = false;
 #pragma unroll 4
-          for (uint32_t e = tid & 127; e < G::kTile / 16; e += 128) {
+          for (uint32_t e = tid; e < G::kTile / 16; e += 256) {
             uint4 x = tile[e];
             const uint32_t b0 = __vcmpeq2(x.x & inf2, inf2), b1 = __vcmpeq2(x.y & inf2, inf2),
                            b2 = __vcmpeq2(x.z & inf2, inf2), b3 = __vcmpeq2(x.w & inf2, inf2);
             if (b0 | b1 | b2 | b3) {
-              const int32_t key = k0 + (int32_t)(e * 16 / G::kGroupV * 8 + e * 16 % 1024 / 128);
+              const int32_t key = (int32_t)((j0 + i) * KT + e * 16 / G::kGroupV * 8 + e * 16 % 1024 / 128);
               odd = odd || (key >= lo0 && key < hi1);
               tile[e] = make_uint4(x.x & ~b0, x.y & ~b1, x.z & ~b2, x.w & ~b3);
             }
@@ -557,7 +568,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_cluster(ready, masked);
+      if (lane == 0) arrive_cluster(ready[i & 1], masked);
     }
     if (nt) wait(&pv_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1);
   }
@@ -566,19 +577,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
   if (warp < kSoftWarps) {
     const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16;
     const bool live = __any_sync(0xffffffffu, valid);
-    // Sums of both warpgroups, referred to the last reference; the tiles' memory is free now.
-    float2* lsum = reinterpret_cast<float2*>(smem);
-    lsum[wg * 128 + row] = make_float2(l, ref);
-    bar_sync(3, 256);
+    // Sums of both halves; the maxima's memory is free after the barrier above.
+    max_sh[0][wg][row] = l;
+    bar_sync(1 + (warp & 3), 64);
     tc_fence_after();
-    const float fin = nt ? ref_sh[row] : -INFINITY;
-    l = 0.f;
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-      const float2 x = lsum[g * 128 + row];
-      if (x.y != -INFINITY) l += x.y == fin ? x.x : x.x * ex2(x.y - fin);
-      else if (x.x != 0.f) l = NAN;  // only scores of NaN
-    }
+    l += max_sh[0][wg ^ 1][row];
+    const float fin = ref;
     const bool parts = a.n_split > 1;
     const uint64_t rh = (uint64_t)(w.row0 + tok) * a.p.n_heads + head;
     if (valid && wg == 0) {
