@@ -26,6 +26,7 @@ struct AttendArgs {
   uint32_t slots, n_split, split_len;  // tile slots; parts of the keys and keys of one part
   float* part;                       // [row][head][part][D], then [row][head][part][max, sum]
   float2* part_ml;
+  uint32_t vrun;                     // keys of a page that one box of V loads
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -74,7 +75,7 @@ __device__ __forceinline__ bool elect_one() {
 // MMAs of both.
 
 // Shared and tensor memory of one CTA. A K or V tile's half is [8-key group][64-element
-// chunk][8 keys][128 bytes], 128-byte swizzled; queries are [chunk][128 rows][128 bytes].
+// chunk][8 keys][128 bytes], 128-byte swizzled (V: 16 keys where the pages hold them); queries are [chunk][128 rows][128 bytes].
 // Tensor memory: the output from column 0, two score tiles (which the probabilities
 // overwrite) from 256.
 template <int D>
@@ -83,8 +84,8 @@ struct Geo {
   static constexpr uint32_t kQ = 128 * D * 2;    // bytes of the queries
   static constexpr uint32_t kTile = 64 * D * 2;  // bytes of half a K tile, of half a V tile
   static constexpr uint32_t kGroupK = D * 16, kGroupV = D * 8;  // bytes of 8 keys
-  static constexpr uint32_t kStages = D == 256 ? 5 : 10;
-  static constexpr uint32_t kSmem = kQ + kStages * kTile;
+  static constexpr uint32_t kStagesK = D == 256 ? 2 : 4, kStagesV = D == 256 ? 3 : 6;
+  static constexpr uint32_t kSmem = kQ + (kStagesK + kStagesV) * kTile;
   static constexpr uint32_t kS = 256;
 };
 
@@ -241,12 +242,13 @@ __device__ __forceinline__ TileInfo find_tile(const AttendArgs& a, uint32_t s, u
 }
 
 constexpr uint32_t kSoftWarps = 8;
-constexpr uint32_t kAttendThreads = (kSoftWarps + 2) * 32;
+constexpr uint32_t kAttendThreads = (kSoftWarps + 3) * 32;
 constexpr float kRefSlack = 8.f;  // log2 that scores may exceed the reference before O is rescaled
 
 // A cluster = (two tiles of 128 (token, head) rows of one KV head's group, part of the
-// keys). Warp 8 of each CTA loads its halves of the K and V tiles by TMA, 8 keys of one page
-// at a time; warp 9 of the first issues S = Q K^T and O += P V; two warpgroups of each CTA
+// keys). Warps 8 and 10 of each CTA load its halves of the K and V tiles by TMA, 8 or 16 keys
+// of one page at a time (one box takes about 70 cycles to issue: a single warp for both
+// held the MMAs up); warp 9 of the first issues S = Q K^T and O += P V; two warpgroups of each CTA
 // turn half of a score tile's columns into probabilities each, thread = row. The maximum
 // that the exponentials refer to moves only when a score exceeds it by kRefSlack.
 template <typename T, int D, bool GENERAL>
@@ -254,9 +256,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using G = Geo<D>;
-  constexpr uint32_t KT = G::KT, NS = G::kStages;
+  constexpr uint32_t KT = G::KT, NK = G::kStagesK, NV = G::kStagesV;
   extern __shared__ __align__(1024) uint8_t smem_q[];
-  __shared__ uint64_t full[NS], empty[NS], s_full[2], p_ready[2], pv_done[2], v_landed, drained;
+  __shared__ uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_ready[2], pv_done[2], v_landed, drained;
   __shared__ uint32_t tmem_sh;
   __shared__ TileInfo info_sh;
   __shared__ int32_t lohi[4][kSoftWarps / 2];  // per warp: least and largest lo, least and largest hi
@@ -267,16 +269,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
   const uint32_t kh = (blockIdx.x / 2) % a.c.n_kv, unit = (blockIdx.x / 2) / a.c.n_kv;
   const uint32_t split = unit % a.n_split, slot = a.slots - 1 - unit / a.n_split;
-  uint8_t* smem = smem_q + G::kQ;
+  uint8_t *smem_k = smem_q + G::kQ, *smem_v = smem_k + NK * G::kTile;
   if (smem_u32(smem_q) & 1023) {  // the swizzle needs it; the same for every CTA
     report_timeout(a.c.err);
     return;
   }
 
   if (tid == 0) {
-    for (uint32_t s = 0; s < NS; s++) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+    for (uint32_t s = 0; s < NK; s++) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (uint32_t s = 0; s < NV; s++) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&s_full[s], 1);
@@ -349,53 +355,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     hi0 = min(hi0, lohi[2][i]);
     hi1 = max(hi1, lohi[3][i]);
   }
-  // Tiles [j0, j0 + nt): what the rows see, cut to this part.
+  // Tiles [j0, j0 + nt): what the rows see, cut to this part, from the last one down. The
+  // largest scores are mostly near the row itself, above all under a distance bias, whose
+  // scores would outgrow the reference at every tile of the other order.
   const int32_t c0 = (int32_t)(split * a.split_len);
   const int32_t beg = max(lo0 == INT32_MAX ? 0 : lo0, c0), end = min(hi1, c0 + (int32_t)a.split_len);
-  const uint32_t j0 = beg < end ? (uint32_t)beg / KT : 0, nt = beg < end ? ((uint32_t)end + KT - 1) / KT - j0 : 0;
-  // The i-th load: K tiles run one ahead of V tiles, as the MMAs do.
-  auto k_load = [&](uint32_t i) { return i == 0 ? 0u : 2 * i - 1; };
-  auto v_load = [&](uint32_t i) { return i + 1 == nt ? 2 * nt - 1 : 2 * i + 2; };
+  const uint32_t j0 = beg < end ? (uint32_t)beg / KT : 0, nt = beg < end ? ((uint32_t)end + KT - 1) / KT - j0 : 0, jl = j0 + nt - 1;
   // Tiles with a key that some row of the cluster does not see.
   auto masked_tile = [&](uint32_t j) { return (int32_t)(j * KT) < lo1 || (int32_t)(j * KT + KT) > hi0; };
 
   // Results of the softmax warps, used after the loop.
   float l = 0.f, ref = -INFINITY;
-  if (warp == 8) {
-    // Lane g < 16 loads 8 keys of the V tile, and of the K tile where they are of this CTA's
-    // half; keys past the length and pages outside the cache come from a page coordinate past
-    // the end, which reads zeros.
+  const uint32_t vrun = a.vrun;  // keys of a V box: 8 or 16
+  if (warp == 8 || warp == 10) {
+    // Lane g loads the g-th run of keys of the tile (K: of this CTA's half). Keys past the
+    // length and pages outside the cache come from a page coordinate past the end, which reads
+    // zeros.
+    const bool is_k = warp == 8;
+    const uint32_t run = is_k ? 8 : vrun, lanes = is_k ? 8 : KT / vrun, key0 = (is_k ? rank * (KT / 2) : 0) + lane * run;
+    const uint32_t NS = is_k ? NK : NV;
+    uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
     auto page_of = [&](uint32_t i) -> int32_t {
-      const uint32_t key = (j0 + i) * KT + 8 * lane;
+      const uint32_t key = (jl - i) * KT + key0;
       int32_t p = -1;
-      if (i < nt && lane < KT / 8 && (int32_t)key < w.len) p = paged_page(a.c, w.b, key);
+      if (i < nt && lane < lanes && (int32_t)key < w.len) p = paged_page(a.c, w.b, key);
       return p < 0 ? (int32_t)a.c.n_pages : p;
     };
-    int32_t now = page_of(0), next = page_of(1), prev = now;
-    uint32_t n = 0;
-    auto load = [&](bool is_k, uint32_t i, int32_t page) -> bool {
-      const uint32_t st = n % NS;
-      bool ok = n < NS || wait_mbar(&empty[st], (n / NS - 1) & 1);
-      ok = __all_sync(0xffffffffu, ok && !fail_sh);
-      if (!ok) return false;
+    int32_t now = page_of(0), next = page_of(1);
+    uint32_t st = 0, par = 0, n = 0;
+    bool ok = true;
+    for (; n < nt; n++) {
+      const int32_t later = page_of(n + 2);
+      if (n >= NS) ok = __all_sync(0xffffffffu, mbar_try_wait(&empty[st], par ^ 1) || (!fail_sh && wait_mbar(&empty[st], par ^ 1)));
+      if (!ok) break;
       if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&full[st], 2 * G::kTile);
       __syncwarp();
-      const uint32_t bar = in_cta(&full[st], 0), dst = smem_u32(smem + st * G::kTile);
-      const int slot0 = (int)(((j0 + i) * KT + 8 * lane) & ((1u << a.c.shift) - 1));
-      if (is_k && lane / 8 == rank)
-        tma_load_5d(dst + (lane % 8) * G::kGroupK, &kmap, slot0, 0, (int)kh, page, bar);
-      if (!is_k && lane < KT / 8)
-        tma_load_5d(dst + lane * G::kGroupV, &vmap, slot0, (int)(rank * (D / 128)), (int)kh, page, bar);
-      n++;
-      return true;
-    };
-    bool ok = true;
-    for (uint32_t i = 0; ok && i <= nt; i++) {
-      if (i < nt) ok = load(true, i, now);
-      if (ok && i > 0) ok = load(false, i - 1, prev);
-      prev = now;
+      if (lane < lanes)
+        tma_load_5d(smem_u32((is_k ? smem_k : smem_v) + st * G::kTile) + lane * run * (is_k ? D * 2 : D), is_k ? &kmap : &vmap,
+                    (int)(((jl - n) * KT + key0) & ((1u << a.c.shift) - 1)), is_k ? 0 : (int)(rank * (D / 128)), (int)kh, now,
+                    in_cta(&full[st], 0));
       now = next;
-      next = page_of(i + 2);
+      next = later;
+      if (++st == NS) st = 0, par ^= 1;
     }
     if (!ok && lane == 0) fail_sh = 1;
     // every load of both CTAs lands before they part, whatever became of its readers
@@ -407,26 +408,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (!mbar_try_wait(bar, parity)) ok = ok && !fail_sh && wait_mbar(bar, parity);
       };
-      const uint32_t qbase = smem_u32(smem_q);
+      const uint32_t qbase = smem_u32(smem_q), v_sbo = vrun == 8 ? G::kGroupV : 1024;
       auto scores = [&](uint32_t i) {
-        const uint32_t n = k_load(i), st = n % NS;
-        wait(&full[st], (n / NS) & 1);
+        const uint32_t st = i % NK;
+        wait(&k_full[st], (i / NK) & 1);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t base = smem_u32(smem + st * G::kTile);
+        const uint32_t base = smem_u32(smem_k + st * G::kTile);
 #pragma unroll
         for (uint32_t kk = 0; kk < D / 16; kk++)
           mma2_ss(tmem + G::kS + (i & 1) * KT, tile_desc(qbase + (kk / 4) * 16384 + (kk % 4) * 32, 16, 1024),
                   tile_desc(base + (kk / 4) * 1024 + (kk % 4) * 32, 16, G::kGroupK), idesc16<T>(KT, false), kk != 0);
-        commit2(&empty[st]);
+        commit2(&k_empty[st]);
         commit2(&s_full[i & 1]);
       };
       if (nt) scores(0);
       for (uint32_t i = 0; ok && i < nt; i++) {
         if (i + 1 < nt) scores(i + 1);
-        const uint32_t n = v_load(i), st = n % NS;
-        wait(&full[st], (n / NS) & 1);
-        if (ok && masked_tile(j0 + i)) {  // the warpgroups look through it first
+        const uint32_t st = i % NV;
+        wait(&v_full[st], (i / NV) & 1);
+        if (ok && masked_tile(jl - i)) {  // the warpgroups look through it first
           arrive_cluster(in_cta(&v_landed, 0), true);
           arrive_cluster(in_cta(&v_landed, 1), true);
           ok = wait_cluster(&p_ready[i & 1], (i >> 1) & 1);
@@ -435,12 +436,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
         }
         if (!ok) break;
         tc_fence_after();
-        const uint32_t base = smem_u32(smem + st * G::kTile);
+        const uint32_t base = smem_u32(smem_v + st * G::kTile);
 #pragma unroll
         for (uint32_t kk = 0; kk < KT / 16; kk++)
-          mma2_ts(tmem, tmem + G::kS + (i & 1) * KT + kk * 8, tile_desc(base + kk * 2 * G::kGroupV, 1024, G::kGroupV),
+          mma2_ts(tmem, tmem + G::kS + (i & 1) * KT + kk * 8, tile_desc(base + kk * 2 * G::kGroupV, vrun * 128, v_sbo),
                   idesc16<T>(D, true), (i | kk) != 0);
-        commit2(&empty[st]);
+        commit2(&v_empty[st]);
         commit2(&pv_done[i & 1]);
       }
       if (!ok) {
@@ -471,7 +472,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     constexpr uint32_t NC = KT / 2;  // columns of this warp
     uint32_t landed = 0;
     for (uint32_t i = 0; i < nt; i++) {
-      const int32_t k0 = (int32_t)((j0 + i) * KT + wg * NC);
+      const int32_t k0 = (int32_t)((jl - i) * KT + wg * NC);
       const uint32_t tm_s = tmem + lanes + G::kS + (i & 1) * KT;
       float s[NC];
       uint32_t* r = reinterpret_cast<uint32_t*>(s);
@@ -537,16 +538,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
         tm_st32(tm_s + wg * (NC / 2), r);
         tm_wait_st();
       }
-      const bool masked = masked_tile(j0 + i);
+      const bool masked = masked_tile(jl - i);
       if (masked) {
         // A row's probability for a key that it does not see is 0, but 0 * NaN is not: values that
         // are not finite leave the tile, and reach the rows that see them at the end.
         ok = __all_sync(0xffffffffu, ok && wait_cluster(&v_landed, landed & 1));
         landed++;
         if (ok) {
-          const uint32_t n = v_load(i);
           constexpr uint32_t inf2 = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-          uint4* tile = reinterpret_cast<uint4*>(smem + (n % NS) * G::kTile);
+          uint4* tile = reinterpret_cast<uint4*>(smem_v + (i % NV) * G::kTile);
           bool odd = false;
 #pragma unroll 4
           for (uint32_t e = tid; e < G::kTile / 16; e += 256) {
@@ -554,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
             const uint32_t b0 = __vcmpeq2(x.x & inf2, inf2), b1 = __vcmpeq2(x.y & inf2, inf2),
                            b2 = __vcmpeq2(x.z & inf2, inf2), b3 = __vcmpeq2(x.w & inf2, inf2);
             if (b0 | b1 | b2 | b3) {
-              const int32_t key = (int32_t)((j0 + i) * KT + e * 16 / G::kGroupV * 8 + e * 16 % 1024 / 128);
+              const int32_t key = (int32_t)((jl - i) * KT + e * 16 / (vrun * D) * vrun + e * 16 % (vrun * 128) / 128);
               odd = odd || (key >= lo0 && key < hi1);
               tile[e] = make_uint4(x.x & ~b0, x.y & ~b1, x.z & ~b2, x.w & ~b3);
             }
@@ -787,15 +787,15 @@ AttendPlan plan_attend(const snl_paged_cache& c, const snl_paged_batch& b, uint3
   return pl;
 }
 
-// The pages as (64 elements, slot, chunk of 64, head, page): a box is 8 slots of a head, or of half
-// of one.
-int page_map(CUtensorMap* map, const snl_paged_cache& c, void* base, uint32_t chunks) {
+// The pages as (64 elements, slot, chunk of 64, head, page): a box is some slots of a head, or of
+// half of one.
+int page_map(CUtensorMap* map, const snl_paged_cache& c, void* base, uint32_t slots, uint32_t chunks) {
   PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
   if (!enc) return fail(SNL_E_CUDA, "paged cache: cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[5] = {64, c.page_size, c.head_dim / 64, c.n_kv, c.n_pages};
   const cuuint64_t str[4] = {c.slot_stride * 2, 128, c.n_kv > 1 ? c.head_stride * 2 : 128,
                              c.n_pages > 1 ? c.page_stride * 2 : 128};
-  const cuuint32_t box[5] = {64, 8, chunks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+  const cuuint32_t box[5] = {64, slots, chunks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(map, c.type == SNL_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                          base, dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -848,9 +848,10 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
   SNL_TRY(paged_error_word(&a.c.err));
   const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv * 2;
   if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
+  a.vrun = c->page_size >= 16 ? 16 : 8;
   CUtensorMap km, vm;
-  SNL_TRY(page_map(&km, *c, c->k, c->head_dim / 64));
-  SNL_TRY(page_map(&vm, *c, c->v, c->head_dim / 128));
+  SNL_TRY(page_map(&km, *c, c->k, 8, c->head_dim / 64));
+  SNL_TRY(page_map(&vm, *c, c->v, a.vrun, c->head_dim / 128));
   a.p = *p;
   a.q = static_cast<const uint16_t*>(q);
   a.gate = gate;
