@@ -45,7 +45,7 @@ constexpr uint32_t kAppendWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int E = D / 32;
-  __shared__ float rows[kAppendWarps][D];
+  __shared__ __align__(16) float rows[kAppendWarps][D];
   pdl_trigger();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t heads = a.p.n_heads + 2 * a.c.n_kv;

@@ -1,16 +1,11 @@
-// Attention over the paged cache (snl_paged_attend) and the accumulated attention weights
-// of its slots (snl_paged_weigh).
+// Attention over the paged cache (snl_paged_attend).
 #include <algorithm>
 #include <string>
 
-#include "paged.cuh"
-#include "tc.cuh"
-#include "tensor_map.cuh"
+#include "paged_tc.cuh"
 
 namespace snl {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
   PagedView c;
@@ -20,8 +15,6 @@ struct AttendArgs {
   const void* gate;
   void* out;
   float* lse;
-  const float* lse_in;
-  float decay;
   uint32_t group, toks;              // query heads per KV head; tokens of one tile (128 / group)
   uint32_t slots, n_split, split_len;  // tile slots; parts of the keys and keys of one part
   float* part;                       // [row][head][part][D], then [row][head][part][max, sum]
@@ -29,46 +22,6 @@ struct AttendArgs {
   uint32_t vrun;                     // keys of a page that one box of V loads
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// tanh x = 1 - 2 / (1 + e^2x): off by less than 2^-22, which tanh.approx (2^-11) is not.
-__device__ __forceinline__ float tanh_(float x) { return fmaf(-2.f, rcp(1.f + ex2(2.f * kLog2e * x)), 1.f); }
-
-// Two 32-bit operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ void bar_sync(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-// One lane of the warp, known to the compiler as one: what it alone issues (MMAs) then takes
-// its operands from uniform registers. A region entered by lane == 0 took 67 cycles an MMA.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-  return p != 0;
-}
-
-// ---- tensor-core pieces ----------------------------------------------------------------
-//
 // Two CTAs of a cluster work as one (cta_group::2): each holds 128 rows of queries, half of
 // every K tile (64 of its 128 keys) and half of every V tile (half of head_dim), so each
 // byte of the cache is fetched and held once for 256 rows. One CTA's leader thread issues the
@@ -88,126 +41,6 @@ struct Geo {
   static constexpr uint32_t kSmem = kQ + (kStagesK + kStagesV) * kTile;
   static constexpr uint32_t kS = 256;
 };
-
-template <typename T>
-constexpr uint32_t idesc16(uint32_t n, bool b_mn) {  // D f32, A and B f16 or bf16, M = 256
-  const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((256u >> 4) << 24);
-}
-// 128-byte swizzled operand. K-major: sbo between 8-row groups. MN-major: lbo between
-// chunks of 64 along MN, sbo between groups of 8 along K.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-// A from tensor memory.
-__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-// Arrives on both CTAs' barriers once the MMAs issued so far have completed.
-__device__ __forceinline__ void commit2(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_alloc2(uint32_t* dst) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc2(uint32_t base) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// Address of the same shared variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-// With release, what this thread wrote to memory is seen by who waits (about 1000 cycles at
-// cluster scope); tensor memory is ordered by its own fences and needs none.
-__device__ __forceinline__ void arrive_cluster(uint32_t bar, bool release) {
-  if (release) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-  else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded waits of about 0.15 s: the longest that one of these is due is some microseconds.
-// The second sees what the other CTA released.
-__device__ __forceinline__ bool wait_mbar(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 28); }
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity) {
-  if (try_wait_cluster(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!try_wait_cluster(bar, parity))
-    if (clock64() - t0 > (1ll << 28)) return false;
-  return true;
-}
-// Into this CTA, counted on a barrier that may be the other CTA's.
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int slot, int chunk, int head, int page,
-                                            uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(map), "r"(0), "r"(slot), "r"(chunk), "r"(head), "r"(page), "r"(bar)
-      : "memory");
-}
-
-// 32 columns of this thread's lane, not waited for.
-__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-      : "memory");
-}
-// Waits for this thread's loads; the empty statements keep uses of the registers behind it.
-template <int N>
-__device__ __forceinline__ void tm_wait_ld(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));
-}
-__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Where a tile of rows lies: sequence, first row, tokens, slot of the first token.
 struct TileInfo {
@@ -690,66 +523,10 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant
   if (a.lse && lane == 0) a.lse[item] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
 }
 
-// Score in units of log2 from the raw product: cap, then the distance bias.
-__device__ __forceinline__ float paged_score(const PagedMask& m, float qk, float slope, int32_t t, int32_t key) {
-  float s = qk * m.scale;
-  if (m.cap > 0.f) s = m.cap * tanhf(s / m.cap);
-  return (s - slope * fabsf((float)(t - key))) * kLog2e;
-}
-
-// One warp per (slot, KV head, sequence), one row and head at a time.
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) weigh_simple_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int E = D / 32;
-  pdl_trigger();
-  pdl_wait();
-  const uint32_t type = std::is_same<T, __half>::value ? SNL_T_F16 : SNL_T_BF16;
-  const uint32_t lane = threadIdx.x & 31, kh = blockIdx.y, b = blockIdx.z;
-  const int32_t key = (int32_t)(blockIdx.x * kWarps + (threadIdx.x >> 5)), len = paged_len(a.c, b);
-  if (key >= len) return;
-  const int32_t page = paged_page(a.c, b, key);
-  if (page < 0) return;
-  const int2 rr = paged_rows(a.c, b);
-  const uint32_t group = a.p.n_heads / a.c.n_kv;
-  float x[E], sum = 0.f;
-  load_as_float<E>(a.c.k, paged_at(a.c, page, kh, key) + lane * E, type, x);
-  for (int32_t r = rr.x; r < rr.y; r++) {
-    const int32_t t = len - (rr.y - r);
-    const int2 keys = paged_keys(a.m, r, t, len);
-    if (key < keys.x || key >= keys.y) continue;
-    for (uint32_t g = 0; g < group; g++) {
-      const uint32_t h = kh * group + g;
-      float q[E], s = 0.f;
-      load_as_float<E>(a.q, r * a.p.q_row + h * a.p.q_head + lane * E, type, q);
-#pragma unroll
-      for (int i = 0; i < E; i++) s = fmaf(q[i], x[i], s);
-      s = paged_score(a.m, warp_sum(s), a.m.slopes ? __ldg(a.m.slopes + h) : 0.f, t, key);
-      sum += exp2f(s - a.lse_in[(uint64_t)r * a.p.n_heads + h] * kLog2e);
-    }
-  }
-  if (lane == 0) {
-    float* w = a.c.weight + paged_weight_at(a.c, page, kh, key);
-    const bool old = a.decay != 0.f && key < len - (rr.y - rr.x);
-    *w = old ? fmaf(*w, a.decay, sum) : sum;
-  }
-}
-
 }  // namespace
 }  // namespace snl
 
 using namespace snl;
-
-#define SNL_BY_TYPE(kern, what, grid, block, smem, s, ...)                                                     \
-  do {                                                                                                         \
-    if (c->type == SNL_T_F16 && c->head_dim == 256)                                                            \
-      SNL_PDL_LAUNCH(what, (kern<__half, 256>), grid, block, smem, s, __VA_ARGS__);                            \
-    else if (c->type == SNL_T_F16)                                                                             \
-      SNL_PDL_LAUNCH(what, (kern<__half, 128>), grid, block, smem, s, __VA_ARGS__);                            \
-    else if (c->head_dim == 256)                                                                               \
-      SNL_PDL_LAUNCH(what, (kern<__nv_bfloat16, 256>), grid, block, smem, s, __VA_ARGS__);                     \
-    else                                                                                                       \
-      SNL_PDL_LAUNCH(what, (kern<__nv_bfloat16, 128>), grid, block, smem, s, __VA_ARGS__);                     \
-  } while (0)
 
 namespace {
 
@@ -785,21 +562,6 @@ AttendPlan plan_attend(const snl_paged_cache& c, const snl_paged_batch& b, uint3
   if (pl.split_len == 0) pl.split_len = 128;
   pl.n_split = std::max<uint32_t>(1, (uint32_t)((max_len + pl.split_len - 1) / pl.split_len));
   return pl;
-}
-
-// The pages as (64 elements, slot, chunk of 64, head, page): a box is some slots of a head, or of
-// half of one.
-int page_map(CUtensorMap* map, const snl_paged_cache& c, void* base, uint32_t slots, uint32_t chunks) {
-  PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
-  if (!enc) return fail(SNL_E_CUDA, "paged cache: cuTensorMapEncodeTiled is unavailable");
-  const cuuint64_t dims[5] = {64, c.page_size, c.head_dim / 64, c.n_kv, c.n_pages};
-  const cuuint64_t str[4] = {c.slot_stride * 2, 128, c.n_kv > 1 ? c.head_stride * 2 : 128,
-                             c.n_pages > 1 ? c.page_stride * 2 : 128};
-  const cuuint32_t box[5] = {64, slots, chunks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(map, c.type == SNL_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-                         base, dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? SNL_OK : fail(SNL_E_INVALID, "paged cache: the pages' strides do not fit a tensor map");
 }
 
 size_t part_bytes(const AttendPlan& pl, const snl_paged_cache& c, const snl_paged_batch& b, uint32_t n_heads) {
@@ -876,27 +638,5 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
   const dim3 jg((unsigned)((items + kWarps - 1) / kWarps));
   if (wide) SNL_PDL_LAUNCH("join_kernel", join_kernel<256>, jg, dim3(kWarps * 32), (size_t)0, s, a);
   else SNL_PDL_LAUNCH("join_kernel", join_kernel<128>, jg, dim3(kWarps * 32), (size_t)0, s, a);
-  return SNL_OK;
-}
-
-extern "C" int snl_paged_weigh(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_attn_p* p,
-                               const void* q, const float* lse, float decay, void* stream) {
-  const std::string w = "snl_paged_weigh";
-  AttendArgs a{};
-  SNL_TRY(paged_check("snl_paged_weigh", c, b, &a.c));
-  if (b->n_rows && (!q || !lse)) return fail(SNL_E_INVALID, w + ": null argument");
-  SNL_TRY(paged_check_attn("snl_paged_weigh", *c, *b, p, &a.m));
-  if (!c->weight) return fail(SNL_E_INVALID, w + ": the cache has no weights");
-  if (!(decay >= 0.f) || decay > 3e38f) return fail(SNL_E_INVALID, w + ": decay must be finite and not negative");
-  if (!paged_aligned(q)) return fail(SNL_E_INVALID, w + ": q rows must be aligned to 16 bytes");
-  if (b->n_seqs == 0 || a.c.max_len == 0) return SNL_OK;
-  a.p = *p;
-  a.q = static_cast<const uint16_t*>(q);
-  a.lse_in = lse;
-  SNL_TRY(paged_error_word(&a.c.err));
-  a.decay = decay;
-  SNL_BY_TYPE(weigh_simple_kernel, "weigh_simple_kernel",
-              dim3((unsigned)((a.c.max_len + kWarps - 1) / kWarps), c->n_kv, b->n_seqs), dim3(kWarps * 32), (size_t)0,
-              (cudaStream_t)stream, a);
   return SNL_OK;
 }
