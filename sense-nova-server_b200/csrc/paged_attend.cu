@@ -236,24 +236,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     if (rank == 0)
       for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) (void)wait_mbar(&full[i % NS], (i / NS) & 1);
   } else if (warp == 9) {
-    if (rank == 0 && elect_one()) {
+    if (rank == 0) {
+      const uint32_t lead = elect_one();
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!mbar_try_wait(bar, parity)) ok = ok && !fail_sh && wait_mbar(bar, parity);
+        ok = __all_sync(0xffffffffu, ok && (mbar_try_wait(bar, parity) || (!fail_sh && wait_mbar(bar, parity))));
       };
-      const uint32_t qbase = smem_u32(smem_q), v_sbo = vrun == 8 ? G::kGroupV : 1024;
+      const uint32_t q_lo = desc_lo(smem_u32(smem_q), 16), v_hi = desc_hi(vrun == 8 ? G::kGroupV : 1024);
       auto scores = [&](uint32_t i) {
         const uint32_t st = i % NK;
         wait(&k_full[st], (i / NK) & 1);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t base = smem_u32(smem_k + st * G::kTile);
+        const uint32_t k_lo = desc_lo(smem_u32(smem_k) + st * G::kTile, 16), d = tmem + G::kS + (i & 1) * KT;
 #pragma unroll
         for (uint32_t kk = 0; kk < D / 16; kk++)
-          mma2_ss(tmem + G::kS + (i & 1) * KT, tile_desc(qbase + (kk / 4) * 16384 + (kk % 4) * 32, 16, 1024),
-                  tile_desc(base + (kk / 4) * 1024 + (kk % 4) * 32, 16, G::kGroupK), idesc16<T>(KT, false), kk != 0);
-        commit2(&k_empty[st]);
-        commit2(&s_full[i & 1]);
+          mma2_ss(lead, d, q_lo + (kk / 4) * 1024 + (kk % 4) * 2, desc_hi(1024), k_lo + (kk / 4) * 64 + (kk % 4) * 2,
+                  desc_hi(G::kGroupK), idesc16<T>(KT, false), kk != 0);
+        commit2(lead, &k_empty[st]);
+        commit2(lead, &s_full[i & 1]);
       };
       if (nt) scores(0);
       for (uint32_t i = 0; ok && i < nt; i++) {
@@ -261,31 +262,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
         const uint32_t st = i % NV;
         wait(&v_full[st], (i / NV) & 1);
         if (ok && masked_tile(jl - i)) {  // the warpgroups look through it first
-          arrive_cluster(in_cta(&v_landed, 0), true);
-          arrive_cluster(in_cta(&v_landed, 1), true);
-          ok = wait_cluster(&p_ready[i & 1], (i >> 1) & 1);
+          if (lane < 2) arrive_cluster(in_cta(&v_landed, lane), true);
+          ok = __all_sync(0xffffffffu, wait_cluster(&p_ready[i & 1], (i >> 1) & 1));
         } else {
           wait(&p_ready[i & 1], (i >> 1) & 1);
         }
         if (!ok) break;
         tc_fence_after();
-        const uint32_t base = smem_u32(smem_v + st * G::kTile);
+        const uint32_t v_lo = desc_lo(smem_u32(smem_v) + st * G::kTile, vrun * 128), p = tmem + G::kS + (i & 1) * KT;
 #pragma unroll
         for (uint32_t kk = 0; kk < KT / 16; kk++)
-          mma2_ts(tmem, tmem + G::kS + (i & 1) * KT + kk * 8, tile_desc(base + kk * 2 * G::kGroupV, vrun * 128, v_sbo),
-                  idesc16<T>(D, true), (i | kk) != 0);
-        commit2(&v_empty[st]);
-        commit2(&pv_done[i & 1]);
+          mma2_ts(lead, tmem, p + kk * 8, v_lo + kk * 2 * (G::kGroupV / 16), v_hi, idesc16<T>(D, true), (i | kk) != 0);
+        commit2(lead, &v_empty[st]);
+        commit2(lead, &pv_done[i & 1]);
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         fail_sh = 1;
         report_timeout(a.c.err);
       }
-      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&drained))
-                   : "memory");  // and every MMA before the tensor memory is given back
+      commit_own(lead, &drained);  // and every MMA before the tensor memory is given back
       (void)wait_mbar(&drained, 0);
     }
-    __syncwarp();
   } else {
     // Half of a tile's columns each: warps w and w + 4 hold the same 32 rows.
     const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16;

@@ -41,12 +41,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 __device__ __forceinline__ void bar_sync(uint32_t id, uint32_t n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-// One lane of the warp, known to the compiler as one: what it alone issues (MMAs) can take
-// its operands from uniform registers.
-__device__ __forceinline__ bool elect_one() {
+// 1 in one lane of the warp.
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t p;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-  return p != 0;
+  return p;
 }
 
 template <typename T>
@@ -54,32 +53,44 @@ constexpr uint32_t idesc16(uint32_t n, bool b_mn) {  // D f32, A and B f16 or bf
   const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
   return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
-// 128-byte swizzled operand. K-major: sbo between 8-row groups. MN-major: lbo between
-// chunks of 64 along MN, sbo between groups of 8 along K.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Descriptor of a 128-byte swizzled operand, as halves. K-major: sbo between 8-row groups.
+// MN-major: lbo between chunks of 64 along MN, sbo between groups of 8 along K. The low half
+// of an address further on is the low half plus the distance / 16 (shared memory ends below
+// 2^18), one addition where the whole descriptor anew took 80 cycles an MMA.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return saddr >> 4 | (lbo >> 4) << 16; }
+__device__ __forceinline__ uint32_t desc_hi(uint32_t sbo) { return sbo >> 4 | 1u << 14 | 2u << 29; }
+// The whole warp runs the code around an MMA and `lead` (one lane) issues it.
+__device__ __forceinline__ void mma2_ss(uint32_t lead, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 q, %7, 0;\n mov.b64 a, {%1, %2};\n"
+      " mov.b64 b, {%3, %4};\n @q tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
 // A from tensor memory.
-__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma2_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                        uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n mov.b64 b, {%2, %3};\n"
+      " @q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-// Arrives on both CTAs' barriers once the MMAs issued so far have completed.
-__device__ __forceinline__ void commit2(uint64_t* bar) {
+// Arrives on both CTAs' barriers, or this one's, once the MMAs issued so far have completed.
+__device__ __forceinline__ void commit2(uint32_t lead, uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit_own(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ void tmem_alloc2(uint32_t* dst) {
@@ -162,6 +173,19 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tm_st(uint32_t taddr, const uint32_t* r) {
+  static_assert(N == 16 || N == 32, "columns");
+  if constexpr (N == 16) tm_st16(taddr, r);
+  else tm_st32(taddr, r);
 }
 // Waits for this thread's loads; the empty statements keep uses of the registers behind it.
 template <int N>

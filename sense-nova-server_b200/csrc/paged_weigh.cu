@@ -125,16 +125,17 @@ __global__ void __launch_bounds__(kWeighWarps * 32, 2) weigh_rows_kernel(const _
 // ---- many rows: S^T = K Q^T on the tensor cores ---------------------------------------------
 
 // Shared memory of one CTA: its 128 keys [8-key group][64-element chunk][8 keys][128 bytes],
-// and stages of half a query tile [chunk][64 rows][128 bytes]. Tensor memory: four tiles of
-// 128 keys x 128 (token, head) rows.
+// and stages of half a query tile [chunk][64 rows][128 bytes]. Tensor memory: three tiles of
+// 128 keys x 128 (token, head) rows, and from column 384 the keys, the products' A operand
+// (from shared memory it and the queries would take the whole of its bandwidth).
 template <int D>
 struct WeighGeo {
   static constexpr uint32_t kK = 128 * D * 2, kGroup = D * 16;
   static constexpr uint32_t kQ = 64 * D * 2;
-  static constexpr uint32_t kStages = 4, kMeta = 4;
+  static constexpr uint32_t kStages = 4, kMeta = 4, kBufs = 3, kTK = 384;
   static constexpr uint32_t kSmem = kK + kStages * kQ;
 };
-constexpr uint32_t kWeighThreads = (8 + 3) * 32;
+constexpr uint32_t kSumWarps = 16, kWeighThreads = (kSumWarps + 3) * 32;  // 16: the exponentials bound the sums
 
 // What the sums need of a query tile's 128 rows (read 16 bytes at a time).
 struct alignas(16) WeighMeta {
@@ -146,20 +147,20 @@ struct alignas(16) WeighMeta {
 
 // A cluster = (256 keys of a sequence and KV head), a CTA 128 of them, thread = key: the
 // scores of a query tile come with a key's row in one lane of tensor memory, so its sum over
-// the rows needs no exchange. Warp 10 lists the query tiles that see the keys, with what each
-// row needs; warp 8 loads their queries by TMA, warp 9 of the first CTA issues the products.
+// the rows needs no exchange. The last warp lists the query tiles that see the keys, with what
+// each row needs; one loads their queries by TMA, one of the first CTA issues the products.
 template <typename T, int D, bool GENERAL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
     weigh_tile_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap qmap) {
   using G = WeighGeo<D>;
-  constexpr uint32_t NS = G::kStages, NM = G::kMeta;
+  constexpr uint32_t NS = G::kStages, NM = G::kMeta, NB = G::kBufs;
   extern __shared__ __align__(1024) uint8_t smem_k[];
   uint8_t* smem_q = smem_k + G::kK;
   __shared__ WeighMeta meta[NM];
-  __shared__ uint64_t k_full, q_full[NS], q_empty[NS], m_full[NM], m_empty[NM], s_full[4], s_empty[4], drained;
+  __shared__ uint64_t k_full, q_full[NS], q_empty[NS], m_full[NM], m_empty[NM], s_full[G::kBufs], s_empty[G::kBufs], k_there, drained;
   __shared__ uint32_t tmem_sh;
-  __shared__ float half_sh[128];
+  __shared__ float part_sh[3][128];
   __shared__ volatile int fail_sh;
   pdl_trigger();
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
@@ -176,17 +177,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
     }
     for (uint32_t s = 0; s < NM; s++) {
       mbar_init(&m_full[s], 1);
-      mbar_init(&m_empty[s], 10);  // warps 0 to 9
+      mbar_init(&m_empty[s], kSumWarps + 2);
     }
-    for (uint32_t s = 0; s < 4; s++) {
+    for (uint32_t s = 0; s < NB; s++) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_empty[s], 16);  // the warps of both CTAs
+      mbar_init(&s_empty[s], 2 * kSumWarps);  // of both CTAs
     }
+    mbar_init(&k_there, 2 * kSumWarps);
     mbar_init(&drained, 1);
     fail_sh = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc2(&tmem_sh);
+  if (warp == kSumWarps + 1) tmem_alloc2(&tmem_sh);
   pdl_wait();
   const int32_t len = paged_len(a.c, b), k0 = (int32_t)(kt * 256);
   const int2 rr = paged_rows(a.c, b);
@@ -203,24 +205,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
     if (!mbar_try_wait(bar, parity)) ok = ok && !fail_sh && wait_mbar(bar, parity);
   };
   float sum = 0.f;
-  if (warp == 10) {
-    uint32_t n = 0;
-    // Under a causal mask alone the first rows see only earlier keys.
-    uint32_t i = !a.m.last && k0 > t0 ? (uint32_t)(k0 - t0) / per : 0;
-    for (; ok; i++) {
-      int32_t lo[4], hi[4], row[4];
-      int32_t ulo = INT32_MAX, uhi = 0, ilo = 0, ihi = INT32_MAX;  // of the union, of the intersection
-      if (i < tiles) {
+  if (warp == kSumWarps + 2) {
+    // A lane has columns lane + 32 e. The next tile's sums are on their way while this one's
+    // wait for their place.
+    struct Cols {
+      uint32_t i;
+      int32_t lo[4], hi[4], row[4], full;
+      float lse[4];
+    };
+    // Token of the tile (past any sequence for a column without a row) and head of each column.
+    uint32_t tok0[4], head[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++) {
+      const uint32_t col = lane + 32 * e, in = col % 64;
+      tok0[e] = in < a.toks * a.group ? (col / 64) * a.toks + in / a.group : 1u << 30;
+      head[e] = kh * a.group + in % a.group;
+    }
+    // The first tile from i on that sees a key, or `tiles`.
+    auto find = [&](uint32_t i, Cols& x) {
+      for (; i < tiles; i++) {
+        int32_t ulo = INT32_MAX, uhi = 0, ilo = 0, ihi = INT32_MAX;  // of the union, of the intersection
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++) {
-          const uint32_t col = lane + 32 * e, in = col % 64, tok = i * per + (col / 64) * a.toks + in / a.group;
+          const uint32_t tok = i * per + tok0[e];
           int2 keys = make_int2(0, 0);
-          row[e] = -1;
-          if (in < a.toks * a.group && tok < (uint32_t)rows) {
-            row[e] = rr.x + (int32_t)tok;
-            keys = paged_keys(a.m, row[e], t0 + (int32_t)tok, len);
+          x.row[e] = -1;
+          if (tok < (uint32_t)rows) {
+            x.row[e] = rr.x + (int32_t)tok;
+            keys = paged_keys(a.m, x.row[e], t0 + (int32_t)tok, len);
           }
-          lo[e] = keys.x, hi[e] = keys.y;
+          x.lo[e] = keys.x, x.hi[e] = keys.y;
           if (keys.x < keys.y) {
             ulo = min(ulo, keys.x);
             uhi = max(uhi, keys.y);
@@ -231,47 +245,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
         ulo = __reduce_min_sync(0xffffffffu, ulo);
         uhi = __reduce_max_sync(0xffffffffu, uhi);
         if (ulo >= k1 || uhi <= k0) continue;
-        ilo = __reduce_max_sync(0xffffffffu, ilo);
-        ihi = __reduce_min_sync(0xffffffffu, ihi);
+        x.full = __reduce_max_sync(0xffffffffu, ilo) <= k0 && __reduce_min_sync(0xffffffffu, ihi) >= k0 + 256;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++)
+          x.lse[e] = x.row[e] < 0 ? -INFINITY
+                                  : __ldg(a.lse + (uint64_t)x.row[e] * a.p.n_heads + head[e]);
+        break;
       }
+      x.i = i;
+    };
+    Cols now, next;
+    // Under a causal mask alone the first rows see only earlier keys.
+    find(!a.m.last && k0 > t0 ? (uint32_t)(k0 - t0) / per : 0, now);
+    for (uint32_t n = 0;; n++) {
       const uint32_t ms = n % NM;
+      if (now.i < tiles) find(now.i + 1, next);
       if (n >= NM) wait(&m_empty[ms], (n / NM - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       WeighMeta& m = meta[ms];
-      if (i < tiles) {
+      if (now.i < tiles) {
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++) {
           const uint32_t col = lane + 32 * e;
-          const uint32_t head = kh * a.group + col % 64 % a.group;
-          m.lse2[col] = row[e] >= 0 ? log2_sum(__ldg(a.lse + (uint64_t)row[e] * a.p.n_heads + head)) : INFINITY;
-          m.lo[col] = lo[e];
-          m.hi[col] = hi[e];
+          m.lse2[col] = log2_sum(now.lse[e]);
+          m.lo[col] = now.lo[e];
+          m.hi[col] = now.hi[e];
           if (GENERAL) {
-            m.t[col] = (float)(t0 + row[e] - rr.x);
-            m.slope[col] = a.m.slopes ? __ldg(a.m.slopes + head) * kLog2e : 0.f;
+            m.t[col] = (float)(t0 + now.row[e] - rr.x);
+            m.slope[col] = a.m.slopes ? __ldg(a.m.slopes + head[e]) * kLog2e : 0.f;
           }
         }
       }
       if (lane == 0) {
-        m.tile = i < tiles ? (int32_t)i : -1;
-        m.full = ilo <= k0 && ihi >= k0 + 256;
+        m.tile = now.i < tiles ? (int32_t)now.i : -1;
+        m.full = now.full;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive_cta(&m_full[ms]);
-      n++;
-      if (i >= tiles) break;
+      if (now.i >= tiles) break;
+      now = next;
     }
-  } else if (warp == 8) {
+  } else if (warp == kSumWarps) {
     // The keys of this CTA, 8 of a page at a time (pages past the length read zeros), then queries.
     if (tiles) {
-      if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&k_full, 2 * G::kK);
+      if (lane == 0) mbar_arrive_expect_tx(&k_full, G::kK);
       __syncwarp();
       if (lane < 16) {
         const int32_t key = k0 + (int32_t)(rank * 128 + 8 * lane);
         const int32_t page = key < len ? paged_page(a.c, b, key) : -1;
         tma_load_5d(smem_u32(smem_k) + lane * G::kGroup, &kmap, key & (int32_t)((1u << a.c.shift) - 1), 0, (int)kh,
-                    page < 0 ? (int32_t)a.c.n_pages : page, in_cta(&k_full, 0));
+                    page < 0 ? (int32_t)a.c.n_pages : page, smem_u32(&k_full));
       }
       __syncwarp();
     }
@@ -294,71 +318,95 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
                     (int)lane, (int)kh, in_cta(&q_full[st], 0));
     }
     if (!ok && lane == 0) fail_sh = 1;
+    if (tiles) (void)wait_mbar(&k_full, 0);
     if (rank == 0) {  // every load of both CTAs lands before they part
-      if (tiles) (void)wait_mbar(&k_full, 0);
       for (uint32_t i = n > NS ? n - NS : 0; i < n; i++) (void)wait_mbar(&q_full[i % NS], (i / NS) & 1);
     }
-  } else if (warp == 9) {
-    const bool leader = rank == 0 && elect_one();
-    if (leader || (rank == 1 && lane == 0)) {
-      const uint32_t kbase = smem_u32(smem_k);
-      if (tiles && leader) wait(&k_full, 0);
-      for (uint32_t n = 0; ok; n++) {
-        const uint32_t ms = n % NM, st = n % NS, buf = n % 4;
-        wait(&m_full[ms], (n / NM) & 1);
-        const int32_t tile = ok ? meta[ms].tile : -1;
-        mbar_arrive_cta(&m_empty[ms]);
-        if (tile < 0) break;
-        if (!leader) continue;
-        if (n >= 4) wait(&s_empty[buf], (n / 4 - 1) & 1);
-        wait(&q_full[st], (n / NS) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t qbase = smem_u32(smem_q) + st * G::kQ;
+  } else if (warp == kSumWarps + 1) {
+    const uint32_t lead = rank == 0 ? elect_one() : 0;
+    if (tiles && rank == 0) wait(&k_there, 0);
+    ok = __all_sync(0xffffffffu, ok);
+    // Whether there is an n-th tile, and it can be issued.
+    auto ready = [&](uint32_t n) -> bool {
+      wait(&m_full[n % NM], (n / NM) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      const bool more = __all_sync(0xffffffffu, ok && meta[n % NM].tile >= 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cta(&m_empty[n % NM]);
+      if (!more || rank != 0) return more;
+      if (n >= NB) wait(&s_empty[n % NB], (n / NB - 1) & 1);
+      wait(&q_full[n % NS], (n / NS) & 1);
+      return ok = __all_sync(0xffffffffu, ok);
+    };
+    bool more = ready(0);
+    for (uint32_t n = 0; more; n++) {
+      if (rank != 0) {
+        more = ready(n + 1);
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t b_lo = desc_lo(smem_u32(smem_q) + n % NS * G::kQ, 16), d = tmem + n % NB * 128;
+      // The waits for the next tile pass while the first half of this one's products is at work.
 #pragma unroll
-        for (uint32_t kk = 0; kk < D / 16; kk++)
-          mma2_ss(tmem + buf * 128, tile_desc(kbase + (kk / 4) * 1024 + (kk % 4) * 32, 16, G::kGroup),
-                  tile_desc(qbase + (kk / 4) * 8192 + (kk % 4) * 32, 16, 1024), idesc16<T>(128, false), kk != 0);
-        commit2(&q_empty[st]);
-        commit2(&s_full[buf]);
+      for (uint32_t kk = 0; kk < D / 16; kk++) {
+        if (kk == D / 32) more = ready(n + 1);
+        mma2_ts(lead, d, tmem + G::kTK + kk * 8, b_lo + (kk / 4) * 512 + (kk % 4) * 2, desc_hi(1024), idesc16<T>(128, false),
+                kk != 0);
       }
-      if (!ok) {
-        fail_sh = 1;
-        report_timeout(a.c.err);
-      }
-      if (leader) {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&drained))
-                     : "memory");
-        (void)wait_mbar(&drained, 0);
-      }
+      commit2(lead, &q_empty[n % NS]);
+      commit2(lead, &s_full[n % NB]);
+    }
+    if (!ok && lane == 0) {
+      fail_sh = 1;
+      report_timeout(a.c.err);
+    }
+    if (rank == 0) {
+      commit_own(lead, &drained);
+      (void)wait_mbar(&drained, 0);
     }
     __syncwarp();
   } else {
-    const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16;
-    const int32_t key = k0 + (int32_t)(rank * 128 + (tid & 127));
+    // Warpgroup wg: columns 32 wg to 32 wg + 31 of every tile.
+    const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16, kl = tid & 127;
+    const int32_t key = k0 + (int32_t)(rank * 128 + kl);
     const float sl = a.m.scale * kLog2e, cap = a.m.cap, pre = GENERAL && cap > 0.f ? a.m.scale / cap : 0.f;
+    if (tiles) {  // the keys into tensor memory, a quarter of head_dim each
+      wait(&k_full, 0);
+      ok = __all_sync(0xffffffffu, ok);
+      uint32_t r[D / 8];
+#pragma unroll
+      for (uint32_t u = 0; u < D / 32; u++) {
+        const uint32_t c = wg * (D / 32) + u;  // 16 bytes of the row
+        const uint4 x = *reinterpret_cast<const uint4*>(smem_k + kl / 8 * G::kGroup + c / 8 * 1024 + kl % 8 * 128 + ((c % 8 ^ kl % 8) << 4));
+        r[4 * u] = x.x, r[4 * u + 1] = x.y, r[4 * u + 2] = x.z, r[4 * u + 3] = x.w;
+      }
+      tm_st<D / 8>(tmem + lanes + G::kTK + wg * (D / 8), r);
+      tm_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(in_cta(&k_there, 0), false);
+    }
     for (uint32_t n = 0;; n++) {
-      const uint32_t ms = n % NM, buf = n % 4;
+      const uint32_t ms = n % NM, buf = n % NB;
       wait(&m_full[ms], (n / NM) & 1);
       ok = __all_sync(0xffffffffu, ok);
       const WeighMeta& m = meta[ms];
       if (!ok || m.tile < 0) break;
-      wait(&s_full[buf], (n / 4) & 1);
+      wait(&s_full[buf], (n / NB) & 1);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      float s[64];
+      float s[32];
       uint32_t* r = reinterpret_cast<uint32_t*>(s);
-      tm_ld32(tmem + lanes + buf * 128 + wg * 64, r);
-      tm_ld32(tmem + lanes + buf * 128 + wg * 64 + 32, r + 32);
-      tm_wait_ld<64>(r);
+      tm_ld32(tmem + lanes + buf * 128 + wg * 32, r);
+      tm_wait_ld<32>(r);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(in_cta(&s_empty[buf], 0), false);
       float2 acc[2] = {{0.f, 0.f}, {0.f, 0.f}};
       const bool full = m.full;
 #pragma unroll
-      for (uint32_t c = 0; c < 64; c += 4) {
-        const uint32_t col = wg * 64 + c;
+      for (uint32_t c = 0; c < 32; c += 4) {
+        const uint32_t col = wg * 32 + c;
         const float4 z = *reinterpret_cast<const float4*>(&m.lse2[col]);
         if constexpr (GENERAL) {
           const float4 t = *reinterpret_cast<const float4*>(&m.t[col]);
@@ -390,13 +438,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
       if (lane == 0) mbar_arrive_cta(&m_empty[ms]);
     }
     if (!ok && lane == 0) fail_sh = 1;
-    if (wg == 1) half_sh[tid & 127] = sum;
-    bar_sync(1, 256);
-    if (wg == 0 && key < len) put_weight(a, b, kh, key, len - rows, sum + half_sh[tid]);
+    if (wg) part_sh[wg - 1][kl] = sum;
+    bar_sync(1, kSumWarps * 32);
+    if (wg == 0 && key < len)
+      put_weight(a, b, kh, key, len - rows, (sum + part_sh[0][kl]) + (part_sh[1][kl] + part_sh[2][kl]));
   }
   __syncwarp();
   cluster_sync();  // nothing of one CTA is used by the other after this
-  if (warp == 9) tmem_dealloc2(tmem);
+  if (warp == kSumWarps + 1) tmem_dealloc2(tmem);
 }
 
 // Queries as (64 elements, head of the group, token, chunk of 64, KV head): a box is one chunk
