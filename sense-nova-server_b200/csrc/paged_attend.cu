@@ -2,25 +2,10 @@
 #include <algorithm>
 #include <string>
 
-#include "paged_tc.cuh"
+#include "paged_attend.cuh"
 
 namespace snl {
 namespace {
-
-struct AttendArgs {
-  PagedView c;
-  PagedMask m;
-  snl_paged_attn_p p;
-  const uint16_t* q;
-  const void* gate;
-  void* out;
-  float* lse;
-  uint32_t group, toks;              // query heads per KV head; tokens of one tile (128 / group)
-  uint32_t slots, n_split, split_len;  // tile slots; parts of the keys and keys of one part
-  float* part;                       // [row][head][part][D], then [row][head][part][max, sum]
-  float2* part_ml;
-  uint32_t vrun;                     // keys of a page that one box of V loads
-};
 
 // Two CTAs of a cluster work as one (cta_group::2): each holds 128 rows of queries, half of
 // every K tile (64 of its 128 keys) and half of every V tile (half of head_dim), so each
@@ -584,6 +569,7 @@ int go_attend(const AttendArgs& a, const CUtensorMap& km, const CUtensorMap& vm,
 
 extern "C" size_t snl_paged_attend_workspace(const snl_paged_cache* c, const snl_paged_batch* b, uint32_t n_heads) {
   if (!c || !b || c->n_kv == 0 || n_heads == 0 || n_heads % c->n_kv || n_heads / c->n_kv > 64) return 0;
+  if (attend_rows_fits(*b, n_heads / c->n_kv)) return std::max<size_t>(16, attend_rows_workspace(*c, *b, n_heads / c->n_kv));
   return part_bytes(plan_attend(*c, *b, n_heads), *c, *b, n_heads);
 }
 
@@ -600,30 +586,31 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
       !paged_strides(p->out_type, p->out_row, p->out_head) ||
       (gate && !paged_strides(p->gate_type, p->gate_row, p->gate_head)))
     return fail(SNL_E_INVALID, w + ": rows must be aligned to 16 bytes");
-  const AttendPlan pl = plan_attend(*c, *b, p->n_heads);
-  if (work_bytes < part_bytes(pl, *c, *b, p->n_heads)) return fail(SNL_E_INVALID, w + ": work is too small");
+  if (work_bytes < snl_paged_attend_workspace(c, b, p->n_heads)) return fail(SNL_E_INVALID, w + ": work is too small");
   if (!work) return fail(SNL_E_INVALID, w + ": null argument");
   if (b->n_rows == 0 || b->n_seqs == 0) return SNL_OK;
   SNL_TRY(paged_error_word(&a.c.err));
-  const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv * 2;
-  if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
-  a.vrun = c->page_size >= 16 ? 16 : 8;
-  CUtensorMap km, vm;
-  SNL_TRY(page_map(&km, *c, c->k, 8, c->head_dim / 64));
-  SNL_TRY(page_map(&vm, *c, c->v, a.vrun, c->head_dim / 128));
   a.p = *p;
   a.q = static_cast<const uint16_t*>(q);
   a.gate = gate;
   a.out = out;
   a.lse = lse;
   a.group = p->n_heads / c->n_kv;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (attend_rows_fits(*b, a.group)) return launch_attend_rows(*c, *b, a, work, s);
+  const AttendPlan pl = plan_attend(*c, *b, p->n_heads);
+  const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv * 2;
+  if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
+  a.vrun = c->page_size >= 16 ? 16 : 8;
+  CUtensorMap km, vm;
+  SNL_TRY(page_map(&km, *c, c->k, 8, c->head_dim / 64));
+  SNL_TRY(page_map(&vm, *c, c->v, a.vrun, c->head_dim / 128));
   a.toks = pl.toks;
   a.slots = pl.slots;
   a.n_split = pl.n_split;
   a.split_len = pl.split_len;
   a.part = static_cast<float*>(work);
   a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)b->n_rows * p->n_heads * pl.n_split * c->head_dim);
-  const cudaStream_t s = (cudaStream_t)stream;
   const bool half = c->type == SNL_T_F16, wide = c->head_dim == 256, gen = p->cap > 0.f || p->slopes;
   const uint32_t g = (uint32_t)grid;
   if (half && wide) SNL_TRY(gen ? (go_attend<__half, 256, true>(a, km, vm, g, s)) : (go_attend<__half, 256, false>(a, km, vm, g, s)));

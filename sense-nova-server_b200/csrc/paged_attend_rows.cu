@@ -1,0 +1,482 @@
+// Attention over the paged cache for single tokens (and two rows a sequence): the work is
+// reading the keys and values once.
+#include <algorithm>
+#include <string>
+
+#include "paged_attend.cuh"
+
+namespace snl {
+namespace {
+
+constexpr uint32_t kRowWarps = 8, kBlock = 64;  // keys of a block: 8 of each warp
+
+// Shared memory: each warp's ring of stages (8 keys of K, then of V, each [64-element chunk]
+// [8 keys][128 bytes], 128-byte swizzled), then each warp's output for up to 8 heads.
+template <int D>
+struct RowGeo {
+  static constexpr uint32_t kGroup = D * 16, kStage = 2 * kGroup;
+  static constexpr uint32_t kStages = D == 256 ? 2 : 5;
+  static constexpr uint32_t kRing = kRowWarps * kStages * kStage;
+  static constexpr uint32_t kSmem = kRing + kRowWarps * 8 * D * 4;
+};
+
+struct RowArgs {
+  AttendArgs a;
+  float* part;      // [CTA][2][group][D], then the same of (max, sum): a CTA's first and last unfinished piece
+  float2* part_ml;
+  int2* span;       // [row][KV head]: first and last CTA
+};
+
+// The keys of a row.
+struct RowKeys {
+  uint32_t b;
+  int32_t lo, hi, t, len;
+};
+__device__ __forceinline__ RowKeys row_keys(const PagedView& c, const PagedMask& m, uint32_t r) {
+  uint32_t b = min(r, c.n_seqs - 1);
+  if ((uint32_t)__ldg(c.start + b) > r || (uint32_t)__ldg(c.start + b + 1) <= r) {  // mostly start[b] = b
+    uint32_t lo = 0, hi = c.n_seqs;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if ((uint32_t)__ldg(c.start + mid) <= r) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+  }
+  const int2 rr = paged_rows(c, b);
+  RowKeys k{b, 0, 0, 0, paged_len(c, b)};
+  k.t = k.len - (rr.y - (int32_t)r);
+  if ((int32_t)r < rr.x || (int32_t)r >= rr.y) return k;
+  const int2 keys = paged_keys(m, r, k.t, k.len);
+  k.lo = keys.x, k.hi = keys.y;
+  return k;
+}
+__device__ __forceinline__ uint32_t row_blocks(const RowKeys& k) {
+  return k.lo < k.hi ? ((uint32_t)k.hi + kBlock - 1) / kBlock - (uint32_t)k.lo / kBlock : 0;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_k16(float d[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {  // rows 8-15 of A are 0
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ void mma_k8(float d[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
+  else
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+// Into this CTA's memory; the box is 8 slots of a head.
+__device__ __forceinline__ void tma_group(uint32_t dst, const CUtensorMap* map, int slot, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(map), "r"(0), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Where a walk over the blocks stands: blocks of (KV head, row) in that order of importance.
+struct Walk {
+  uint64_t left;  // blocks, this one included
+  uint32_t kh, row, blk, end, first;  // block numbers of the row: this one, one past its last, its first
+  RowKeys k;
+};
+__device__ __forceinline__ void enter_row(const RowArgs& A, Walk& w) {
+  w.k = row_keys(A.a.c, A.a.m, w.row);
+  w.first = (uint32_t)w.k.lo / kBlock;
+  w.end = w.first + row_blocks(w.k);
+}
+__device__ __forceinline__ void next_block(const RowArgs& A, Walk& w) {
+  w.left--;
+  w.blk++;
+  while (w.left && w.blk >= w.end) {
+    if (++w.row == A.a.c.n_rows) w.row = 0, w.kh++;
+    enter_row(A, w);
+    w.blk = w.first;
+  }
+}
+
+// The blocks of 64 keys of all (KV head, row) pairs form one line that is cut into equal
+// shares, one for each CTA: every SM reads the same number of bytes whatever the lengths are.
+// A row that ends inside its CTA is written at once; pieces of rows cut by a share's end are
+// left to rows_join_kernel. A warp takes 8 keys of each block through its own ring of TMA
+// boxes: S = Q K^T on m16n8k16 (query heads as rows), O^T += V^T P^T on m16n8k8, whose B
+// operand is the score fragment as it stands.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32, 1)
+    attend_rows_kernel(const __grid_constant__ RowArgs A, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+  using G = RowGeo<D>;
+  constexpr uint32_t NS = G::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t bars[kRowWarps][NS];
+  __shared__ uint32_t scan_sh[kRowWarps], found_sh[2];
+  __shared__ float2 ml_sh[kRowWarps][8];
+  const AttendArgs& a = A.a;
+  pdl_trigger();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023) {
+    report_timeout(a.c.err);
+    return;
+  }
+  if (lane == 0)
+    for (uint32_t s = 0; s < NS; s++) mbar_init(&bars[warp][s], 1);
+  fence_mbar_init();
+  pdl_wait();
+
+  // Blocks before each thread's rows, this CTA's share, and the row that it starts in.
+  const uint32_t per = (a.c.n_rows + kRowWarps * 32 - 1) / (kRowWarps * 32), r0 = min(tid * per, a.c.n_rows),
+                 r1 = min(r0 + per, a.c.n_rows);
+  uint32_t mine = 0;
+  for (uint32_t r = r0; r < r1; r++) mine += row_blocks(row_keys(a.c, a.m, r));
+  uint32_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= (uint32_t)o) upto += v;
+  }
+  if (lane == 31) scan_sh[warp] = upto;
+  __syncthreads();
+  uint32_t total = 0;
+  for (uint32_t i = 0; i < kRowWarps; i++) {
+    if (i < warp) upto += scan_sh[i];
+    total += scan_sh[i];
+  }
+  const uint64_t all = (uint64_t)total * a.c.n_kv, share = (all + gridDim.x - 1) / gridDim.x, g0 = blockIdx.x * share;
+  if (g0 >= all) return;
+  const uint64_t g1 = min(g0 + share, all);
+  {
+    uint32_t off = (uint32_t)(g0 % total);
+    if (off >= upto - mine && off < upto) {
+      off -= upto - mine;
+      uint32_t r = r0;
+      for (;; r++) {
+        const uint32_t n = row_blocks(row_keys(a.c, a.m, r));
+        if (off < n) break;
+        off -= n;
+      }
+      found_sh[0] = r;
+      found_sh[1] = off;
+    }
+  }
+  __syncthreads();
+  Walk now;
+  now.left = g1 - g0;
+  now.kh = (uint32_t)(g0 / total);
+  now.row = found_sh[0];
+  enter_row(A, now);
+  now.blk = now.first + found_sh[1];
+  Walk ahead = now;  // of the loads
+
+  const uint32_t ring = smem_u32(smem) + warp * NS * G::kStage;
+  // Pages of this warp's keys in 32 blocks from `base` on, one a lane.
+  int32_t pages = -1;
+  uint32_t base = 0xFFFFFFFFu, prow = 0xFFFFFFFFu;
+  uint32_t issued = 0, taken = 0;
+  auto active = [&](const Walk& w) {
+    const int32_t key = (int32_t)(w.blk * kBlock + warp * 8);
+    return key + 8 > w.k.lo && key < w.k.hi;
+  };
+  auto issue = [&] {  // the next group that this warp has, if any
+    while (ahead.left) {
+      const bool use = active(ahead);
+      if (use) {
+        if (prow != ahead.row || ahead.blk - base >= 32) {
+          prow = ahead.row;
+          base = ahead.blk;
+          const uint32_t key = (base + lane) * kBlock + warp * 8;
+          pages = (int32_t)key < ahead.k.hi ? paged_page(a.c, ahead.k.b, key) : -1;
+        }
+        const int32_t page = __shfl_sync(0xffffffffu, pages, ahead.blk - base);
+        if (lane == 0) {
+          const uint32_t st = issued % NS, dst = ring + st * G::kStage;
+          const int slot = (int)((ahead.blk * kBlock + warp * 8) & ((1u << a.c.shift) - 1)),
+                    pg = page < 0 ? (int)a.c.n_pages : page;  // past the end: zeros
+          mbar_arrive_expect_tx(&bars[warp][st], G::kStage);
+          tma_group(dst, &kmap, slot, (int)ahead.kh, pg, &bars[warp][st]);
+          tma_group(dst + G::kGroup, &vmap, slot, (int)ahead.kh, pg, &bars[warp][st]);
+        }
+        issued++;
+      }
+      next_block(A, ahead);
+      if (use) return;
+    }
+  };
+  for (uint32_t s = 0; s < NS; s++) issue();
+
+  const uint32_t g = lane >> 2, t = lane & 3;
+  const float flip = a.m.scale < 0.f ? -1.f : 1.f, sl = fmaxf(fabsf(a.m.scale) * kLog2e, 1e-30f) * flip;
+  const float cap = a.m.cap, pre = cap > 0.f ? a.m.scale / cap : 0.f;
+  // ldmatrix: lane L addresses row L % 8 of matrix L / 8, 16 bytes each, four along a row
+  const uint32_t lrow = lane & 7, lsel = lane >> 3;
+  auto lds = [&](uint32_t at, uint32_t c) {  // elements 32 c to 32 c + 31 of the 8 keys
+    return at + (c / 2) * 1024 + lrow * 128 + ((((c & 1) * 4 + lsel) ^ lrow) << 4);
+  };
+  bool ok = true;
+  uint32_t q[D / 16][2];
+  float o[D / 16][4];
+  float m_run = -INFINITY, l_run = 0.f;
+  bool fresh = true;
+  float slope = 0.f;
+  const uint32_t head = g;  // of the group
+  while (now.left) {
+    if (fresh) {  // a new row: its queries (heads past the group are 0)
+      fresh = false;
+#pragma unroll
+      for (int c = 0; c < D / 16; c++) {
+        q[c][0] = q[c][1] = 0;
+        if (head < a.group) {
+          const uint16_t* s = a.q + (uint64_t)now.row * a.p.q_row + (uint64_t)(now.kh * a.group + head) * a.p.q_head + 16 * c + 2 * t;
+          q[c][0] = *reinterpret_cast<const uint32_t*>(s);
+          q[c][1] = *reinterpret_cast<const uint32_t*>(s + 8);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[c][e] = 0.f;
+      }
+      slope = a.m.slopes && head < a.group ? __ldg(a.m.slopes + now.kh * a.group + head) * kLog2e : 0.f;
+      m_run = -INFINITY;
+      l_run = 0.f;
+    }
+    if (active(now)) {
+      const uint32_t st = taken % NS, kat = ring + st * G::kStage, vat = kat + G::kGroup;
+      ok = __all_sync(0xffffffffu, ok && wait_mbar(&bars[warp][st], (taken / NS) & 1));
+      taken++;
+      const int32_t key = (int32_t)(now.blk * kBlock + warp * 8 + 2 * t);
+      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (uint32_t c = 0; c < D / 32; c++) {
+        uint32_t kb[4];
+        ldsm4(kb, lds(kat, c));
+        mma_k16<T>(s0, q[2 * c][0], q[2 * c][1], kb[0], kb[1]);
+        mma_k16<T>(s1, q[2 * c + 1][0], q[2 * c + 1][1], kb[2], kb[3]);
+      }
+      // head g, keys `key` and key + 1
+      float x0 = s0[0] + s1[0], x1 = s0[1] + s1[1];
+      if (cap > 0.f) {
+        x0 = cap * kLog2e * tanh_(x0 * pre);
+        x1 = cap * kLog2e * tanh_(x1 * pre);
+      } else {
+        x0 *= sl;
+        x1 *= sl;
+      }
+      if (slope != 0.f) {
+        x0 -= slope * fabsf((float)(now.k.t - key));
+        x1 -= slope * fabsf((float)(now.k.t - key - 1));
+      }
+      const bool in0 = key >= now.k.lo && key < now.k.hi, in1 = key + 1 >= now.k.lo && key + 1 < now.k.hi;
+      if (!in0) x0 = -INFINITY;
+      if (!in1) x1 = -INFINITY;
+      float mx = fmaxf(x0, x1);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      if (__any_sync(0xffffffffu, mx > m_run + 8.f)) {  // the reference moves only for scores 2^8 above it
+        const float to = mx > m_run + 8.f ? mx : m_run, f = to == m_run ? 1.f : ex2(m_run - to);
+        m_run = to;
+        l_run *= f;
+        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+        for (int c = 0; c < D / 16; c++) o[c][0] *= f0, o[c][1] *= f1, o[c][2] *= f0, o[c][3] *= f1;
+      }
+      const float zero = m_run == -INFINITY ? 0.f : m_run;
+      x0 = ex2(x0 - zero);
+      x1 = ex2(x1 - zero);
+      l_run += x0 + x1;
+      const uint32_t p = pack2(x0, x1, T());
+      // values of keys that the row does not see may be anything: not 0 * that, but 0
+      const uint32_t keep = (in0 ? 0xFFFFu : 0u) | (in1 ? 0xFFFF0000u : 0u);
+#pragma unroll
+      for (uint32_t c = 0; c < D / 32; c++) {
+        uint32_t v[4];
+        ldsm4_t(v, lds(vat, c));
+        mma_k8<T>(o[2 * c], v[0] & keep, v[1] & keep, p);
+        mma_k8<T>(o[2 * c + 1], v[2] & keep, v[3] & keep, p);
+      }
+      fence_proxy_async_smem();  // the stage was read; the next box is written to it after that
+      __syncwarp();
+      issue();
+    }
+    const Walk was = now;
+    next_block(A, now);
+    if (now.left && now.row == was.row && now.kh == was.kh) continue;
+    // The row's piece in this CTA is done: join the warps.
+    fresh = true;
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+    float* mo = reinterpret_cast<float*>(smem + G::kRing);
+#pragma unroll
+    for (int c = 0; c < D / 16; c++) {  // column 2t, 2t + 1: heads; row g, g + 8: elements
+      float* at = mo + (warp * 8 + 2 * t) * D + 16 * c + g;
+      if (2 * t < a.group) at[0] = o[c][0], at[8] = o[c][2];
+      if (2 * t + 1 < a.group) at[D] = o[c][1], at[D + 8] = o[c][3];
+    }
+    if (t == 0) ml_sh[warp][g] = make_float2(m_run, l_run);
+    __syncthreads();
+    const uint64_t g_row = g1 - was.left + 1 - (was.blk - was.first + 1);  // the line's block where the row starts
+    const uint64_t n_row = was.end - was.first;
+    const uint64_t c_first = g_row / share, c_last = (g_row + n_row - 1) / share;
+    const bool whole = c_first == c_last;
+    if (c_first == blockIdx.x && tid == 0)
+      A.span[(uint64_t)was.row * a.c.n_kv + was.kh] = make_int2((int)c_first, (int)c_last);
+    for (uint32_t h = tid / D; h < a.group; h += kRowWarps * 32 / D) {
+      const uint32_t d = tid % D;
+      float top = -INFINITY, l = 0.f, x = 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < kRowWarps; i++) top = fmaxf(top, ml_sh[i][h].x);
+      const float zero = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (uint32_t i = 0; i < kRowWarps; i++) {
+        const float2 ml = ml_sh[i][h];
+        if (ml.y == 0.f) continue;
+        const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - zero);
+        l = fmaf(ml.y, f, l);
+        x = fmaf(mo[(i * 8 + h) * D + d], f, x);
+      }
+      const uint32_t hq = was.kh * a.group + h;
+      if (!whole) {
+        const uint64_t at = ((uint64_t)blockIdx.x * 2 + (c_first == blockIdx.x ? 1 : 0)) * a.group + h;
+        A.part[at * D + d] = x;
+        if (d == 0) A.part_ml[at] = make_float2(top, l);
+        continue;
+      }
+      x = l == 0.f ? 0.f : x / l;
+      auto value = [](const void* p, uint64_t i, uint32_t type) {
+        return type == SNL_T_F32 ? static_cast<const float*>(p)[i]
+               : type == SNL_T_F16 ? __half2float(static_cast<const __half*>(p)[i])
+                                   : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+      };
+      if (a.gate) x *= sigmoidf_(value(a.gate, (uint64_t)was.row * a.p.gate_row + (uint64_t)hq * a.p.gate_head + d, a.p.gate_type));
+      const uint64_t to = (uint64_t)was.row * a.p.out_row + (uint64_t)hq * a.p.out_head + d;
+      if (a.p.out_type == SNL_T_F32) static_cast<float*>(a.out)[to] = x;
+      else if (a.p.out_type == SNL_T_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(x);
+      else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(x);
+      if (a.lse && d == 0)
+        a.lse[(uint64_t)was.row * a.p.n_heads + hq] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
+    }
+    __syncthreads();
+  }
+  if (!ok) {
+    // A wait gave up: this warp's boxes still in flight land before the CTA ends.
+    if (lane == 0) report_timeout(a.c.err);
+    for (uint32_t i = issued > NS ? issued - NS : 0; i < issued; i++) (void)wait_mbar(&bars[warp][i % NS], (i / NS) & 1);
+  }
+}
+
+// Joins the pieces of rows that lie in several shares, and writes rows without keys. One warp
+// per (row, head).
+constexpr uint32_t kJoinWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) rows_join_kernel(const __grid_constant__ RowArgs A) {
+  constexpr int E = D / 32;
+  const AttendArgs& a = A.a;
+  pdl_trigger();
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t item = (uint64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const uint32_t r = (uint32_t)(item / a.p.n_heads), hq = (uint32_t)(item % a.p.n_heads), kh = hq / a.group, h = hq % a.group;
+  pdl_wait();
+  if (r >= a.c.n_rows) return;
+  const RowKeys k = row_keys(a.c, a.m, r);
+  float l = 0.f, zero = 0.f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] = 0.f;
+  if (k.lo < k.hi) {
+    const int2 span = A.span[(uint64_t)r * a.c.n_kv + kh];
+    if (span.x == span.y) return;  // written already
+    auto place = [&](int c) { return ((uint64_t)c * 2 + (c == span.x ? 1 : 0)) * a.group + h; };
+    float top = -INFINITY;
+    for (int c0 = span.x; c0 <= span.y; c0 += 32) {
+      const int c = c0 + (int)lane;
+      if (c <= span.y) top = fmaxf(top, A.part_ml[place(c)].x);
+    }
+    top = warp_max(top);
+    zero = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+    for (int c = span.x; c <= span.y; c++) {
+      const float2 x = A.part_ml[place(c)];
+      float v[E];
+      load_as_float<E>(A.part, place(c) * D + lane * E, SNL_T_F32, v);
+      const float f = x.y == 0.f ? 0.f : x.x == -INFINITY ? 1.f : ex2(x.x - zero);
+      l = fmaf(x.y, f, l);
+#pragma unroll
+      for (int i = 0; i < E; i++) o[i] = x.y == 0.f ? o[i] : fmaf(v[i], f, o[i]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float gate[E];
+  if (a.gate) load_as_float<E>(a.gate, (uint64_t)r * a.p.gate_row + (uint64_t)hq * a.p.gate_head + lane * E, a.p.gate_type, gate);
+#pragma unroll
+  for (int i = 0; i < E; i++) o[i] = l == 0.f ? 0.f : o[i] * (a.gate ? inv * sigmoidf_(gate[i]) : inv);
+  store_from_float<E>(a.out, (uint64_t)r * a.p.out_row + (uint64_t)hq * a.p.out_head + lane * E, a.p.out_type, o);
+  if (a.lse && lane == 0) a.lse[item] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
+}
+
+uint32_t rows_grid(const snl_paged_cache& c, const snl_paged_batch& b) {
+  const uint64_t len = std::min<uint64_t>(b.max_len, (uint64_t)b.table_stride * c.page_size);
+  const uint64_t most = (uint64_t)b.n_rows * c.n_kv * ((len + kBlock - 1) / kBlock + 1);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (uint64_t)std::max(1, sm_count())));
+}
+
+template <typename T, int D>
+int go_rows(const snl_paged_cache& c, const RowArgs& r, uint32_t grid, cudaStream_t s) {
+  CUtensorMap km, vm;
+  SNL_TRY(page_map(&km, c, c.k, 8, D / 64));
+  SNL_TRY(page_map(&vm, c, c.v, 8, D / 64));
+  static bool attr[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr[dev]) {
+    SNL_CUDA_TRY(cudaFuncSetAttribute(attend_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowGeo<D>::kSmem));
+    if (dev >= 0 && dev < 64) attr[dev] = true;
+  }
+  SNL_PDL_LAUNCH("attend_rows_kernel", (attend_rows_kernel<T, D>), dim3(grid), dim3(kRowWarps * 32), (size_t)RowGeo<D>::kSmem, s,
+                 r, km, vm);
+  const uint64_t items = (uint64_t)r.a.c.n_rows * r.a.p.n_heads;
+  SNL_PDL_LAUNCH("rows_join_kernel", rows_join_kernel<D>, dim3((unsigned)((items + kJoinWarps - 1) / kJoinWarps)),
+                 dim3(kJoinWarps * 32), (size_t)0, s, r);
+  return SNL_OK;
+}
+
+}  // namespace
+
+// The query heads of a KV head are rows of one 16-row product whose last 8 are not used; rows
+// beyond two a sequence would read its keys again for each.
+bool attend_rows_fits(const snl_paged_batch& b, uint32_t group) {
+  return group <= 8 && b.n_rows <= 2 * (uint64_t)b.n_seqs && (uint64_t)b.n_rows * (b.max_len / kBlock + 2) < (1ull << 31);
+}
+
+size_t attend_rows_workspace(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t group) {
+  return (size_t)rows_grid(c, b) * 2 * group * (c.head_dim + 2) * sizeof(float) + (size_t)b.n_rows * c.n_kv * sizeof(int2);
+}
+
+int launch_attend_rows(const snl_paged_cache& c, const snl_paged_batch& b, const AttendArgs& a, void* work, cudaStream_t s) {
+  const uint32_t grid = rows_grid(c, b);
+  RowArgs r{};
+  r.a = a;
+  r.part = static_cast<float*>(work);
+  r.part_ml = reinterpret_cast<float2*>(r.part + (size_t)grid * 2 * a.group * c.head_dim);
+  r.span = reinterpret_cast<int2*>(r.part_ml + (size_t)grid * 2 * a.group);
+  if (c.type == SNL_T_F16) return c.head_dim == 256 ? go_rows<__half, 256>(c, r, grid, s) : go_rows<__half, 128>(c, r, grid, s);
+  return c.head_dim == 256 ? go_rows<__nv_bfloat16, 256>(c, r, grid, s) : go_rows<__nv_bfloat16, 128>(c, r, grid, s);
+}
+
+}  // namespace snl
