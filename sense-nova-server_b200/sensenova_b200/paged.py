@@ -19,6 +19,7 @@ ONE, SECTIONS, INTERLEAVED = 0, 1, 2  # which axis of a position turns which pai
 HALVES, ADJACENT = 0, 1  # which elements form a pair
 _TYPES = {"float32": ffi.SNL_T_F32, "float16": ffi.SNL_T_F16, "bfloat16": ffi.SNL_T_BF16}
 _type_of: dict[Any, int] = {}
+_is_int: dict[Any, bool] = {}
 
 
 def _type(t) -> int:
@@ -32,23 +33,30 @@ def _type(t) -> int:
     return code
 
 
+def _fail(what: str):
+    raise SnlError(ffi.SNL_E_INVALID, "paged cache: " + what)
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
-        raise SnlError(ffi.SNL_E_INVALID, "paged cache: " + what)
+        _fail(what)
 
 
-def _ints(t, what: str, *shape: int):
-    """A contiguous tensor of 32-bit integers of that shape; its address."""
-    _need(tuple(t.shape) == shape and str(t.dtype).endswith("int32") and t.is_contiguous(),
-          f"{what} must be contiguous 32-bit integers of shape {shape}")
+def _ints(t, what: str, *shape: int) -> int:
+    """The address of a contiguous tensor of 32-bit integers of that shape."""
+    kind = t.dtype
+    if kind not in _is_int:
+        _is_int[kind] = str(kind).endswith("int32")
+    if not (_is_int[kind] and t.shape == shape and t.is_contiguous()):
+        _fail(f"{what} must be contiguous 32-bit integers of shape {shape}")
     return t.data_ptr()
 
 
-def _floats(t, what: str, *shape: int):
+def _floats(t, what: str, *shape: int) -> int | None:
     if t is None:
         return None
-    _need(tuple(t.shape) == shape and _type(t) == ffi.SNL_T_F32 and t.is_contiguous(),
-          f"{what} must be contiguous float32 of shape {shape}")
+    if not (_type_of.get(t.dtype, -1) == ffi.SNL_T_F32 or _type(t) == ffi.SNL_T_F32) or t.shape != shape or not t.is_contiguous():
+        _fail(f"{what} must be contiguous float32 of shape {shape}")
     return t.data_ptr()
 
 
@@ -84,9 +92,11 @@ class PagedCache:
         self.ref = C.byref(self.c)
 
     def _rows(self, t, what: str, batch: PagedBatch, heads: int) -> tuple[int, int, int]:
-        _need(tuple(t.shape) == (batch.n_rows, heads, self.head_dim) and t.stride(2) == 1,
-              f"{what} must be [{batch.n_rows}, {heads}, {self.head_dim}] with a contiguous last dimension")
-        return t.data_ptr(), t.stride(0), t.stride(1)
+        """Address and row and head strides of [rows, heads, head_dim]."""
+        row, head, one = t.stride() if t.dim() == 3 else (0, 0, 0)
+        if one != 1 or t.shape != (batch.n_rows, heads, self.head_dim):
+            _fail(f"{what} must be [{batch.n_rows}, {heads}, {self.head_dim}] with a contiguous last dimension")
+        return t.data_ptr(), row, head
 
     def append(self, batch: PagedBatch, q, k, v, q_out, pos=None, rope=None, *, axes: int = ONE, pairs: int = HALVES,
                sections=(0, 0, 0), q_norm=None, k_norm=None, eps: float = 1e-6, stream: int = 0) -> None:
@@ -95,44 +105,36 @@ class PagedCache:
         q in the cache's type. pos [rows, 4] 32-bit integers (time, height, width, 0) and
         rope [positions, rot / 2, 2] turn the first rot elements; None turns nothing."""
         d = self.head_dim
-        p = PagedAppendP()
-        kp, p.k_row, p.k_head = self._rows(k, "k", batch, self.n_kv)
-        vp, p.v_row, p.v_head = self._rows(v, "v", batch, self.n_kv)
-        qp = op = None
-        p.in_type = _type(k)
-        _need(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k and v must have one type")
+        kp, k_row, k_head = self._rows(k, "k", batch, self.n_kv)
+        vp, v_row, v_head = self._rows(v, "v", batch, self.n_kv)
+        kind = k.dtype
+        _need(v.dtype == kind and (q is None or q.dtype == kind), "q, k and v must have one type")
+        qp = op = tp = rp = None
+        heads = q_row = q_head = out_row = out_head = rot = n_pos = 0
         if q is not None:
-            p.n_heads = q.shape[1]
-            qp, p.q_row, p.q_head = self._rows(q, "q", batch, q.shape[1])
-            op, p.out_row, p.out_head = self._rows(q_out, "q_out", batch, q.shape[1])
+            heads = q.shape[1]
+            qp, q_row, q_head = self._rows(q, "q", batch, heads)
+            op, out_row, out_head = self._rows(q_out, "q_out", batch, heads)
             _need(_type(q_out) == self.type, "q_out must have the cache's type")
-        tp = rp = None
         if rope is not None:
-            n, half, two = rope.shape
+            n_pos, half, two = rope.shape
             _need(two == 2 and pos is not None, "rope must be [positions, rot / 2, 2] and pos be given")
-            p.rot_dim, p.n_pos = 2 * half, n
-            rp, tp = _floats(rope, "rope", n, half, 2), _ints(pos, "pos", batch.n_rows, 4)
-        p.axes, p.pairs, p.eps = axes, pairs, eps
-        p.sections[0], p.sections[1], p.sections[2] = sections
-        rc = self.lib.snl_paged_append(self.ref, batch.ref, C.byref(p), qp, kp, vp, _floats(q_norm, "q_norm", d),
+            rot = 2 * half
+            rp, tp = _floats(rope, "rope", n_pos, half, 2), _ints(pos, "pos", batch.n_rows, 4)
+        p = PagedAppendP(heads, _type(k), rot, axes, pairs, n_pos, sections, eps, q_row, q_head, k_row, k_head, v_row,
+                         v_head, out_row, out_head)
+        rc = self.lib.snl_paged_append(self.ref, batch.ref, p, qp, kp, vp, _floats(q_norm, "q_norm", d),
                                        _floats(k_norm, "k_norm", d), tp, rp, op, stream)
         if rc:
             ffi.check(rc)
 
     def _attn(self, batch: PagedBatch, q, scale, cap, window, slopes, first, last) -> tuple[PagedAttnP, int]:
-        p = PagedAttnP()
         heads = q.shape[1]
-        qp, p.q_row, p.q_head = self._rows(q, "q", batch, heads)
+        qp, q_row, q_head = self._rows(q, "q", batch, heads)
         _need(_type(q) == self.type, "q must have the cache's type")
-        p.n_heads, p.window, p.cap = heads, window, cap
-        p.scale = self.head_dim ** -0.5 if scale is None else scale
-        if slopes is not None:
-            p.slopes = _floats(slopes, "slopes", heads)
-        if first is not None:
-            p.first = _ints(first, "first", batch.n_rows)
-        if last is not None:
-            p.last = _ints(last, "last", batch.n_rows)
-        return p, qp
+        return PagedAttnP(_floats(slopes, "slopes", heads), None if first is None else _ints(first, "first", batch.n_rows),
+                          None if last is None else _ints(last, "last", batch.n_rows), heads, window,
+                          self.head_dim ** -0.5 if scale is None else scale, cap, 0, 0, q_row, q_head), qp
 
     def attend_workspace(self, batch: PagedBatch, heads: int) -> int:
         """Bytes of scratch that attend needs for such a batch."""
@@ -151,7 +153,7 @@ class PagedCache:
         if gate is not None:
             gp, p.gate_row, p.gate_head = self._rows(gate, "gate", batch, p.n_heads)
             p.gate_type = _type(gate)
-        rc = self.lib.snl_paged_attend(self.ref, batch.ref, C.byref(p), qp, gp, op,
+        rc = self.lib.snl_paged_attend(self.ref, batch.ref, p, qp, gp, op,
                                        _floats(lse, "lse", batch.n_rows, p.n_heads), work.data_ptr(),
                                        work.numel() * work.element_size(), stream)
         if rc:
@@ -162,7 +164,7 @@ class PagedCache:
         """weight = decay * weight + what the rows' attention (with attend's lse) gave each
         slot, per KV head (snl_paged_weigh)."""
         p, qp = self._attn(batch, q, scale, cap, window, slopes, first, last)
-        rc = self.lib.snl_paged_weigh(self.ref, batch.ref, C.byref(p), qp,
+        rc = self.lib.snl_paged_weigh(self.ref, batch.ref, p, qp,
                                       _floats(lse, "lse", batch.n_rows, p.n_heads), decay, stream)
         if rc:
             ffi.check(rc)
@@ -181,7 +183,7 @@ class PagedCache:
             ip = _ints(into, "into", seqs, into.shape[1])
             _need(new_lens is not None, "new_lens is needed with new pages")
         lp = batch.c.len if new_lens is None else _ints(new_lens, "new_lens", seqs)
-        rc = self.lib.snl_paged_evict(self.ref, batch.ref, C.byref(p), _ints(kept, "kept", seqs, self.n_kv, budget), ip,
+        rc = self.lib.snl_paged_evict(self.ref, batch.ref, p, _ints(kept, "kept", seqs, self.n_kv, budget), ip,
                                       lp, stream)
         if rc:
             ffi.check(rc)
