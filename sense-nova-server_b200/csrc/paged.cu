@@ -38,130 +38,166 @@ struct AppendArgs {
 };
 
 constexpr uint32_t kAppendWarps = 8;
+constexpr int append_heads(int d) { return 1024 / d; }  // heads of a warp
 // How a row's elements find their partners: in the lane, a fixed number of lanes away, or
-// through shared memory (halves that do not end with a lane).
+// through shared memory (where a part of a lane's elements turns).
 enum { kTurnNone, kTurnLane, kTurnShuffle, kTurnShared };
 
-// One warp takes `span` of a row's heads (queries, then keys, then values), four at a time: the
-// row's slot, the turn's (cos, sin) and the norm's weights are looked up once for them. A
-// lane holds D / 32 neighbouring elements.
-template <int D, int TURN>
-__global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const __grid_constant__ AppendArgs a, uint32_t span) {
-  constexpr int E = D / 32;
+// One warp takes up to NH query, key or value heads of a row: the row's slot, the turn's (cos,
+// sin) and the norm's weights are looked up once for them, while all their elements are on
+// the way. A lane holds D / 32 neighbouring elements.
+template <int D, int TURN, bool IN32>
+__global__ void __launch_bounds__(kAppendWarps * 32, IN32 ? 3 : 4) append_kernel(const __grid_constant__ AppendArgs a, uint32_t span) {
+  constexpr int E = D / 32, NH = append_heads(D), W = E * (IN32 ? 4 : 2) / 4;  // words of a lane's elements
   __shared__ __align__(16) float rows[TURN == kTurnShared ? kAppendWarps : 1][TURN == kTurnShared ? D : 1];
   pdl_trigger();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t nq = a.p.n_heads, heads = nq + 2 * a.c.n_kv, pieces = (heads + span - 1) / span;
-  const uint64_t item = (uint64_t)blockIdx.x * kAppendWarps + warp;
-  const uint32_t r = (uint32_t)(item / pieces), h0 = (uint32_t)(item % pieces) * span, h1 = min(h0 + span, heads);
+  const uint32_t pq = (a.p.n_heads + span - 1) / span, pk = (a.c.n_kv + span - 1) / span, piece = blockIdx.y;
+  const uint32_t r = blockIdx.x * kAppendWarps + warp;
+  const int what = piece < pq ? 0 : piece < pq + pk ? 1 : 2;  // queries, keys, values
+  const uint32_t h0 = (piece - (what == 0 ? 0 : what == 1 ? pq : pq + pk)) * span;
+  const int n = (int)min(span, (what ? a.c.n_kv : a.p.n_heads) - h0);
   pdl_wait();
   if (r >= a.c.n_rows) return;
 
-  // The slot, for keys and values.
-  int32_t page = -1, t = 0;
-  if (h1 > nq) {
+  const uint64_t step = what == 0 ? a.p.q_head : what == 1 ? a.p.k_head : a.p.v_head;  // elements between heads
+  const uint8_t* src = static_cast<const uint8_t*>(what == 0 ? a.q : what == 1 ? a.k : a.v) +
+                       ((uint64_t)r * (what == 0 ? a.p.q_row : what == 1 ? a.p.k_row : a.p.v_row) + h0 * step + lane * E) *
+                           (IN32 ? 4 : 2);
+  uint32_t raw[NH][W];
+#pragma unroll
+  for (int u = 0; u < NH; u++) {
+    if (u >= n) continue;
+    if constexpr (W == 2) {
+      const uint2 x = __ldg(reinterpret_cast<const uint2*>(src));
+      raw[u][0] = x.x, raw[u][1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const uint4 x = ld_stream16(src + 4 * i);
+        raw[u][i] = x.x, raw[u][i + 1] = x.y, raw[u][i + 2] = x.z, raw[u][i + 3] = x.w;
+      }
+    }
+    src += step * (IN32 ? 4 : 2);
+  }
+
+  uint16_t* dst = a.q_out + (uint64_t)r * a.p.out_row + h0 * a.p.out_head + lane * E;
+  uint64_t to = a.p.out_head;
+  if (what) {  // the row's slot
     const uint32_t b = paged_seq(a.c, r, lane);
     const int2 rr = paged_rows(a.c, b);
-    const int32_t len = paged_len(a.c, b);
-    t = len - (rr.y - (int32_t)r);
-    if ((int32_t)r < rr.x || (int32_t)r >= rr.y || t < 0 || t >= len) report_index(a.c.err);
-    else page = paged_page(a.c, b, t);
+    const int32_t len = paged_len(a.c, b), t = len - (rr.y - (int32_t)r);
+    if ((int32_t)r < rr.x || (int32_t)r >= rr.y || t < 0 || t >= len) {
+      report_index(a.c.err);
+      return;
+    }
+    const int32_t page = paged_page(a.c, b, t);
+    if (page < 0) return;
+    dst = (what == 1 ? a.c.k : a.c.v) + paged_at(a.c, page, h0, t) + lane * E;
+    to = a.c.hs;
   }
   // y = x cos + partner * sin, the sign of the sine by the place in the pair.
   float cs[E], sn[E];
-  bool turned[E];
+  const bool turns = TURN != kTurnNone && what < 2 && lane * E < a.p.rot_dim;  // some of the lane's elements
   const uint32_t half = a.p.rot_dim / 2;
-  const bool adj = a.p.pairs == SNL_ROPE_ADJACENT;
-  if constexpr (TURN != kTurnNone) {
+  if (turns) {
     const uint4 pos = __ldg(a.pos + r);
+    if (max(pos.x, a.p.axes == SNL_ROPE_ONE ? 0u : max(pos.y, pos.z)) >= a.p.n_pos) report_index(a.c.err);
+    const uint32_t last = a.p.n_pos - 1, px = min(pos.x, last), py = min(pos.y, last), pz = min(pos.z, last);
+    const uint32_t e0 = lane * E, s0 = a.p.sections[0], s1 = s0 + a.p.sections[1];
+    const bool adj = TURN == kTurnLane || (TURN == kTurnShared && a.p.pairs == SNL_ROPE_ADJACENT);
+    const bool upper = TURN == kTurnShuffle && e0 >= half;  // the lane holds second places
 #pragma unroll
     for (int i = 0; i < E; i++) {
-      const uint32_t e = lane * E + i;
-      turned[i] = e < a.p.rot_dim;
-      cs[i] = 1.f, sn[i] = 0.f;
-      if (!turned[i]) continue;
-      const bool second = adj ? (e & 1) : e >= half;
-      const uint32_t f = adj ? e / 2 : second ? e - half : e;
-      uint32_t at = pos.x;
-      if (a.p.axes == SNL_ROPE_SECTIONS)
-        at = f < a.p.sections[0] ? pos.x : f < a.p.sections[0] + a.p.sections[1] ? pos.y : pos.z;
-      else if (a.p.axes == SNL_ROPE_INTERLEAVED)
-        at = f % 3 == 1 && f < 3 * a.p.sections[1] ? pos.y : f % 3 == 2 && f < 3 * a.p.sections[2] ? pos.z : pos.x;
-      if (at >= a.p.n_pos) {
-        report_index(a.c.err);
-        at = 0;
+      uint32_t f;
+      bool second;
+      if constexpr (TURN == kTurnShuffle) {
+        f = e0 - (upper ? half : 0) + i, second = upper;
+      } else if constexpr (TURN == kTurnLane) {
+        f = e0 / 2 + i / 2, second = i & 1;
+      } else {
+        cs[i] = 1.f, sn[i] = 0.f;
+        if (e0 + i >= a.p.rot_dim) continue;
+        second = adj ? (i & 1) : e0 + i >= half;
+        f = adj ? (e0 + i) / 2 : second ? e0 + i - half : e0 + i;
+      }
+      uint32_t at = px;
+      if (a.p.axes == SNL_ROPE_SECTIONS) {
+        at = f < s0 ? px : f < s1 ? py : pz;
+      } else if (a.p.axes == SNL_ROPE_INTERLEAVED) {
+        const uint32_t m = f % 3;
+        at = m == 1 && f < 3 * a.p.sections[1] ? py : m == 2 && f < 3 * a.p.sections[2] ? pz : px;
       }
       const float2 v = __ldg(a.rope + (uint64_t)at * half + f);
       cs[i] = v.x;
       sn[i] = second ? v.y : -v.y;
     }
   }
-  float wq[E], wk[E];
+  const float* weights = what == 0 ? a.q_norm : what == 1 ? a.k_norm : nullptr;
+  float norm[E];
+  if (weights) {
+    load_as_float<E>(weights, lane * E, SNL_T_F32, norm);
 #pragma unroll
-  for (int i = 0; i < E; i++) wq[i] = wk[i] = 0.f;
-  if (a.q_norm && h0 < nq) load_as_float<E>(a.q_norm, lane * E, SNL_T_F32, wq);
-  if (a.k_norm && h1 > nq) load_as_float<E>(a.k_norm, lane * E, SNL_T_F32, wk);
+    for (int i = 0; i < E; i++) norm[i] += 1.0f;
+  }
 
-  for (uint32_t hb = h0; hb < h1; hb += 4) {
-    float x[4][E];
+  auto head = [&](int u) {
+    float x[E];
+    if constexpr (IN32) {
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const uint32_t h = hb + u;
-      if (h >= h1) continue;
-      if (h < nq) load_as_float<E>(a.q, (uint64_t)r * a.p.q_row + (uint64_t)h * a.p.q_head + lane * E, a.p.in_type, x[u]);
-      else if (h < nq + a.c.n_kv)
-        load_as_float<E>(a.k, (uint64_t)r * a.p.k_row + (uint64_t)(h - nq) * a.p.k_head + lane * E, a.p.in_type, x[u]);
-      else
-        load_as_float<E>(a.v, (uint64_t)r * a.p.v_row + (uint64_t)(h - nq - a.c.n_kv) * a.p.v_head + lane * E, a.p.in_type, x[u]);
+      for (int i = 0; i < E; i++) x[i] = __uint_as_float(raw[u][i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        const float2 f = a.cache_type == SNL_T_F16 ? unpack2(raw[u][i / 2], __half()) : unpack2(raw[u][i / 2], __nv_bfloat16());
+        x[i] = f.x, x[i + 1] = f.y;
+      }
     }
+    if (weights) {
+      float s = 0.f;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const uint32_t h = hb + u;
-      if (h >= h1) break;
-      const bool is_q = h < nq, is_v = h >= nq + a.c.n_kv;
-      if (!is_v) {
-        if (is_q ? a.q_norm : a.k_norm) {
-          float s = 0.f;
+      for (int i = 0; i < E; i++) s = fmaf(x[i], x[i], s);
+      const float inv = rsqrtf(warp_sum(s) / (float)D + a.p.eps);
 #pragma unroll
-          for (int i = 0; i < E; i++) s = fmaf(x[u][i], x[u][i], s);
-          const float inv = rsqrtf(warp_sum(s) / (float)D + a.p.eps);
+      for (int i = 0; i < E; i++) x[i] = x[i] * inv * norm[i];
+    }
+    if (TURN != kTurnNone && what < 2) {
+      float o[E];
+      if constexpr (TURN == kTurnLane) {
 #pragma unroll
-          for (int i = 0; i < E; i++) x[u][i] = x[u][i] * inv * (1.0f + (is_q ? wq[i] : wk[i]));
-        }
-        if constexpr (TURN != kTurnNone) {
-          float o[E];
-          if constexpr (TURN == kTurnLane) {
+        for (int i = 0; i < E; i++) o[i] = x[i ^ 1];
+      } else if constexpr (TURN == kTurnShuffle) {
+        const uint32_t away = half / E, from = lane < away ? lane + away : lane - away;
 #pragma unroll
-            for (int i = 0; i < E; i++) o[i] = x[u][i ^ 1];
-          } else if constexpr (TURN == kTurnShuffle) {
-            const uint32_t away = half / E, from = lane < away ? lane + away : lane - away;
-#pragma unroll
-            for (int i = 0; i < E; i++) o[i] = __shfl_sync(0xffffffffu, x[u][i], from & 31);
-          } else {
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < E; i += 4)
-              *reinterpret_cast<float4*>(&rows[warp][lane * E + i]) = make_float4(x[u][i], x[u][i + 1], x[u][i + 2], x[u][i + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-              const uint32_t e = lane * E + i;
-              o[i] = rows[warp][e < half ? e + half : e < a.p.rot_dim ? e - half : e];
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < E; i++)
-            if (turned[i]) x[u][i] = fmaf(x[u][i], cs[i], o[i] * sn[i]);
-        }
-      }
-      uint16_t* dst;
-      if (is_q) {
-        dst = a.q_out + (uint64_t)r * a.p.out_row + (uint64_t)h * a.p.out_head;
+        for (int i = 0; i < E; i++) o[i] = __shfl_sync(0xffffffffu, x[i], from & 31);
       } else {
-        if (page < 0) continue;
-        dst = (is_v ? a.c.v : a.c.k) + paged_at(a.c, page, is_v ? h - nq - a.c.n_kv : h - nq, t);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+          *reinterpret_cast<float4*>(&rows[warp][lane * E + i]) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+          const uint32_t e = lane * E + i;
+          o[i] = rows[warp][e >= a.p.rot_dim ? e : a.p.pairs == SNL_ROPE_ADJACENT ? e ^ 1 : e < half ? e + half : e - half];
+        }
       }
-      store_from_float<E>(dst, lane * E, a.cache_type, x[u]);
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < E; i++)
+          if (TURN != kTurnShared || lane * E + i < a.p.rot_dim) x[i] = fmaf(x[i], cs[i], o[i] * sn[i]);
+      }
+    }
+    store_from_float<E>(dst + u * to, 0, a.cache_type, x);
+  };
+  if (n == NH) {  // without a way out between them the heads' sums and turns overlap
+#pragma unroll
+    for (int u = 0; u < NH; u++) head(u);
+  } else {
+#pragma unroll
+    for (int u = 0; u < NH; u++) {
+      if (u >= n) break;
+      head(u);
     }
   }
 }
@@ -541,29 +577,32 @@ extern "C" int snl_paged_append(const snl_paged_cache* c, const snl_paged_batch*
   a.q_out = static_cast<uint16_t*>(q_out);
   a.cache_type = c->type;
   SNL_TRY(paged_error_word(&a.c.err));
-  // Heads of one warp: many rows share the row's look-ups among 8 heads, few rows spread theirs
-  // over the SMs (8 rows of 24 heads: 3 each).
+  // Heads of one warp: with many rows as many as it holds, with few rows they spread over the SMs.
   const uint32_t heads = p->n_heads + 2 * c->n_kv;
   const uint64_t all = (uint64_t)b->n_rows * heads, warps = (uint64_t)std::max(1, sm_count()) * kAppendWarps * 4;
-  const uint32_t span = (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, all / warps));
-  const uint64_t items = (uint64_t)b->n_rows * ((heads + span - 1) / span);
-  if (items > (1ull << 33)) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");
-  const uint32_t e = c->head_dim / 32;
-  const int turn = !p->rot_dim ? kTurnNone : p->pairs == SNL_ROPE_ADJACENT ? kTurnLane
-                   : p->rot_dim / 2 % e == 0 && p->rot_dim / 2 / e <= 16 ? kTurnShuffle : kTurnShared;
+  const uint32_t span = (uint32_t)std::min<uint64_t>(append_heads(c->head_dim), std::max<uint64_t>(1, all / warps));
+  const uint64_t pieces = (p->n_heads + span - 1) / span + 2ull * ((c->n_kv + span - 1) / span);
+  if (pieces > 65535) return fail(SNL_E_UNSUPPORTED, w + ": too many heads");
+  const uint32_t e = c->head_dim / 32;  // elements of a lane: a lane turns whole where they divide rot_dim
+  const int turn = !p->rot_dim ? kTurnNone : p->pairs == SNL_ROPE_ADJACENT && p->rot_dim % e == 0 ? kTurnLane
+                   : p->pairs == SNL_ROPE_HALVES && p->rot_dim / 2 % e == 0 ? kTurnShuffle : kTurnShared;
   auto go = [&](auto kern) -> int {
-    SNL_PDL_LAUNCH("append_kernel", kern, dim3((unsigned)((items + kAppendWarps - 1) / kAppendWarps)), dim3(kAppendWarps * 32),
+    SNL_PDL_LAUNCH("append_kernel", kern, dim3((b->n_rows + kAppendWarps - 1) / kAppendWarps, (unsigned)pieces), dim3(kAppendWarps * 32),
                    (size_t)0, (cudaStream_t)stream, a, span);
     return SNL_OK;
   };
-  auto by_turn = [&](auto d) -> int {
+  auto by_turn = [&](auto d, auto in32) -> int {
     constexpr int D = decltype(d)::value;
-    return turn == kTurnNone      ? go(append_kernel<D, kTurnNone>)
-           : turn == kTurnLane    ? go(append_kernel<D, kTurnLane>)
-           : turn == kTurnShuffle ? go(append_kernel<D, kTurnShuffle>)
-                                  : go(append_kernel<D, kTurnShared>);
+    constexpr bool I = decltype(in32)::value;
+    return turn == kTurnNone      ? go(append_kernel<D, kTurnNone, I>)
+           : turn == kTurnLane    ? go(append_kernel<D, kTurnLane, I>)
+           : turn == kTurnShuffle ? go(append_kernel<D, kTurnShuffle, I>)
+                                  : go(append_kernel<D, kTurnShared, I>);
   };
-  return c->head_dim == 256 ? by_turn(std::integral_constant<int, 256>()) : by_turn(std::integral_constant<int, 128>());
+  auto by_type = [&](auto d) -> int {
+    return p->in_type == SNL_T_F32 ? by_turn(d, std::true_type()) : by_turn(d, std::false_type());
+  };
+  return c->head_dim == 256 ? by_type(std::integral_constant<int, 256>()) : by_type(std::integral_constant<int, 128>());
 }
 
 extern "C" int snl_paged_evict(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_evict_p* p,
