@@ -152,14 +152,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
   if (warp < kSoftWarps) {
     // Queries into shared memory, the sign of the scale folded in.
     const uint32_t flip = a.m.scale < 0.f ? 0x80008000u : 0u;
-    for (uint32_t e = tid; e < G::kQ / 16; e += kSoftWarps * 32) {
-      const uint32_t r = e / (D / 8), u = e % (D / 8), t = r / a.group + rank * a.toks;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r / a.group < a.toks && t < w.toks)
-        x = __ldg(reinterpret_cast<const uint4*>(a.q + (uint64_t)(w.row0 + t) * a.p.q_row +
-                                                 (uint64_t)(kh * a.group + r % a.group) * a.p.q_head + 8 * u));
-      x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
-      *reinterpret_cast<uint4*>(smem_q + (u / 8) * 16384 + r * 128 + ((u % 8 ^ r % 8) << 4)) = x;
+    constexpr uint32_t per = D / 8, batch = 8;  // 16-byte pieces of a row; loads on their way at once
+    for (uint32_t e0 = tid; e0 < G::kQ / 16; e0 += batch * kSoftWarps * 32) {
+      uint4 x[batch];
+#pragma unroll
+      for (uint32_t i = 0; i < batch; i++) {
+        const uint32_t e = e0 + i * kSoftWarps * 32, r = e / per, u = e % per, t0 = r / a.group, t = t0 + rank * a.toks;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (t0 < a.toks && t < w.toks)
+          x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (uint64_t)(w.row0 + t) * a.p.q_row +
+                                                      (uint64_t)(kh * a.group + r - t0 * a.group) * a.p.q_head + 8 * u));
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < batch; i++) {
+        const uint32_t e = e0 + i * kSoftWarps * 32, r = e / per, u = e % per;
+        x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
+        *reinterpret_cast<uint4*>(smem_q + (u / 8) * 16384 + r * 128 + ((u % 8 ^ r % 8) << 4)) = x[i];
+      }
     }
     fence_proxy_async_smem();
   }
@@ -391,7 +400,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
   cluster_sync();  // nothing of one CTA is used by the other after this
   if (warp < kSoftWarps) {
     const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16;
-    const bool live = __any_sync(0xffffffffu, valid);
     // Sums of both halves; the maxima's memory is free after the barrier above.
     max_sh[0][wg][row] = l;
     bar_sync(1 + (warp & 3), 64);
@@ -405,8 +413,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
       else if (a.lse) a.lse[rh] = l == 0.f ? -INFINITY : ((fin == -INFINITY ? 0.f : fin) + log2f(l)) * (1.f / kLog2e);
     }
     const float inv = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    // 32 columns at a time go through the tiles' memory, free now, so that 8 lanes write 32
+    // neighbouring elements of a row: from the accumulator's lanes each would write its own row.
+    float* turn = reinterpret_cast<float*>(smem_k) + warp * 32 * 36;
+    const uint64_t out_at = parts ? (rh * a.n_split + split) * D
+                                  : (uint64_t)(w.row0 + tok) * a.p.out_row + (uint64_t)head * a.p.out_head;
+    const uint64_t gate_at = (uint64_t)(w.row0 + tok) * a.p.gate_row + (uint64_t)head * a.p.gate_head;
+    const uint32_t some_rows = __ballot_sync(0xffffffffu, valid && !(parts && nt == 0));
 #pragma unroll 1
-    for (uint32_t c = wg * (D / 2); live && c < (wg + 1) * (D / 2); c += 32) {
+    for (uint32_t c = wg * (D / 2); some_rows && c < (wg + 1) * (D / 2); c += 32) {
       uint32_t r[32];
       float* o = reinterpret_cast<float*>(r);
       __syncwarp();
@@ -414,8 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
         tm_ld32(tmem + lanes + c, r);
         tm_wait_ld<32>(r);
       }
-      if (!valid || (parts && nt == 0)) continue;
-      if (odd_v) {
+      if (odd_v && valid) {
         for (uint32_t j = j0; j < j0 + nt; j++) {
           if (!masked_tile(j)) continue;
           const int32_t k1 = min(min((int32_t)((j + 1) * KT), keys.y), end);
@@ -433,30 +447,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
           }
         }
       }
-      if (l == 0.f)
 #pragma unroll
-        for (int e = 0; e < 32; e++) o[e] = 0.f;
+      for (int e = 0; e < 32; e += 4)
+        *reinterpret_cast<float4*>(turn + lane * 36 + e) =
+            l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+      __syncwarp();
 #pragma unroll
-      for (int e = 0; e < 32; e++) o[e] *= inv;
-      if (parts) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) store_from_float<4>(a.part, (rh * a.n_split + split) * D + c + e, SNL_T_F32, o + e);
-        continue;
-      }
-      if (a.gate) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          float g[8];
-          load_as_float<8>(a.gate, (uint64_t)(w.row0 + tok) * a.p.gate_row + (uint64_t)head * a.p.gate_head + c + e,
-                           a.p.gate_type, g);
-#pragma unroll
-          for (int f = 0; f < 8; f++) o[e + f] *= sigmoidf_(g[f]);
+      for (uint32_t it = 0; it < 8; it++) {
+        const uint32_t row = it * 4 + lane / 8, col = lane % 8 * 4;
+        const uint64_t to = __shfl_sync(0xffffffffu, out_at, row), from = __shfl_sync(0xffffffffu, gate_at, row);
+        if (!(some_rows >> row & 1)) continue;
+        const float4 x = *reinterpret_cast<const float4*>(turn + row * 36 + col);
+        float v[4] = {x.x, x.y, x.z, x.w};
+        if (parts) {
+          store_from_float<4>(a.part, to + c + col, SNL_T_F32, v);
+          continue;
         }
-      }
+        if (a.gate) {
+          float g[4];
+          load_as_float<4>(a.gate, from + c + col, a.p.gate_type, g);
 #pragma unroll
-      for (int e = 0; e < 32; e += 8)
-        store_from_float<8>(a.out, (uint64_t)(w.row0 + tok) * a.p.out_row + (uint64_t)head * a.p.out_head + c + e,
-                            a.p.out_type, o + e);
+          for (int f = 0; f < 4; f++) v[f] *= sigmoidf_(g[f]);
+        }
+        store_from_float<4>(a.out, to + c + col, a.p.out_type, v);
+      }
     }
     tc_fence_before();
   }
