@@ -8,23 +8,26 @@ namespace snl {
 namespace {
 
 // Two CTAs of a cluster work as one (cta_group::2): each holds 128 rows of queries, half of
-// every K tile (64 of its 128 keys) and half of every V tile (half of head_dim), so each
-// byte of the cache is fetched and held once for 256 rows. One CTA's leader thread issues the
+// every K tile (half of its keys) and half of every V tile (half of head_dim), so each byte
+// of the cache is fetched and held once for 256 rows. One CTA's leader thread issues the
 // MMAs of both.
 
 // Shared and tensor memory of one CTA. A K or V tile's half is [8-key group][64-element
-// chunk][8 keys][128 bytes], 128-byte swizzled (V: 16 keys where the pages hold them); queries are [chunk][128 rows][128 bytes].
-// Tensor memory: the output from column 0, two score tiles (which the probabilities
-// overwrite) from 256.
+// chunk][8 keys][128 bytes], 128-byte swizzled (V: 16 keys where the pages hold them); queries
+// are [chunk][128 rows][128 bytes]. Tensor memory: the output from column 0, then two score
+// tiles, which the probabilities overwrite. At head_dim 256 that is all of an SM's; at 128
+// with tiles of 64 keys it is half, and two CTAs share an SM: one's softmax, start and end
+// run beside the other's products (6 x 1000 rows: 211 us with tiles of 128 keys and one CTA).
 template <int D>
 struct Geo {
-  static constexpr uint32_t KT = 128;            // keys of a tile
-  static constexpr uint32_t kQ = 128 * D * 2;    // bytes of the queries
-  static constexpr uint32_t kTile = 64 * D * 2;  // bytes of half a K tile, of half a V tile
+  static constexpr uint32_t KT = D == 256 ? 128 : 64;  // keys of a tile
+  static constexpr uint32_t kPerSm = D == 256 ? 1 : 2;
+  static constexpr uint32_t kQ = 128 * D * 2;      // bytes of the queries
+  static constexpr uint32_t kTile = KT / 2 * D * 2;  // bytes of half a K tile, of half a V tile
   static constexpr uint32_t kGroupK = D * 16, kGroupV = D * 8;  // bytes of 8 keys
-  static constexpr uint32_t kStagesK = D == 256 ? 2 : 4, kStagesV = D == 256 ? 3 : 6;
+  static constexpr uint32_t kStagesK = D == 256 ? 2 : 4, kStagesV = D == 256 ? 3 : 4;
   static constexpr uint32_t kSmem = kQ + (kStagesK + kStagesV) * kTile;
-  static constexpr uint32_t kS = 256;
+  static constexpr uint32_t kS = D, kCols = D == 256 ? 512 : 256;
 };
 
 // Where a tile of rows lies: sequence, first row, tokens, slot of the first token.
@@ -70,7 +73,7 @@ constexpr float kRefSlack = 8.f;  // log2 that scores may exceed the reference b
 // turn half of a score tile's columns into probabilities each, thread = row. The maximum
 // that the exponentials refer to moves only when a score exceeds it by kRefSlack.
 template <typename T, int D, bool GENERAL>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<D>::kPerSm)
     attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using G = Geo<D>;
@@ -113,7 +116,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     odd_v = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc2(&tmem_sh);
+  if (warp == 9) tmem_alloc2<G::kCols>(&tmem_sh);
   pdl_wait();
   if (warp == 8) {
     const TileInfo w = find_tile(a, slot, lane);
@@ -199,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     // length and pages outside the cache come from a page coordinate past the end, which reads
     // zeros.
     const bool is_k = warp == 8;
-    const uint32_t run = is_k ? 8 : vrun, lanes = is_k ? 8 : KT / vrun, key0 = (is_k ? rank * (KT / 2) : 0) + lane * run;
+    const uint32_t run = is_k ? 8 : vrun, lanes = is_k ? KT / 16 : KT / vrun, key0 = (is_k ? rank * (KT / 2) : 0) + lane * run;
     const uint32_t NS = is_k ? NK : NV;
     uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
     auto page_of = [&](uint32_t i) -> int32_t {
@@ -359,7 +362,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
         }
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
-        tm_st32(tm_s + wg * (NC / 2), r);
+        tm_st<NC / 2>(tm_s + wg * (NC / 2), r);
         tm_wait_st();
       }
       const bool masked = masked_tile(jl - i);
@@ -475,7 +478,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, 1)
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 9) tmem_dealloc2(tmem);
+  if (warp == 9) tmem_dealloc2<G::kCols>(tmem);
 }
 
 // Joins the parts of a row: one warp per (row, head), over the parts that its keys touch.
@@ -540,7 +543,8 @@ AttendPlan plan_attend(const snl_paged_cache& c, const snl_paged_batch& b, uint3
   pl.slots = b.n_rows / (2 * pl.toks) + b.n_seqs;
   const uint64_t max_len = std::min<uint64_t>(b.max_len, (uint64_t)b.table_stride * c.page_size);
   const uint64_t units = (uint64_t)std::min<uint64_t>(pl.slots, b.n_rows) * c.n_kv;
-  const double per_key = c.head_dim == 256 ? 0.011 : 0.006, sms = std::max(1, sm_count() / 2);
+  const bool wide = c.head_dim == 256;
+  const double per_key = wide ? 0.011 : 0.014, sms = std::max(1, wide ? sm_count() / 2 : sm_count());
   double best = 1e30;
   pl.n_split = 1;
   for (uint32_t n = 1; n <= 64; n++) {

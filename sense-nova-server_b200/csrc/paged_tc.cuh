@@ -93,12 +93,17 @@ __device__ __forceinline__ void commit_own(uint32_t lead, uint64_t* bar) {
       "r"(lead)
       : "memory");
 }
+// Pairs of CTAs that hold tensor memory on one SM and wait for more on the other must not meet:
+// kernels that take all 512 columns also take so much shared memory that no other such CTA
+// fits beside them.
+template <uint32_t COLS>
 __device__ __forceinline__ void tmem_alloc2(uint32_t* dst) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "n"(COLS) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
+template <uint32_t COLS>
 __device__ __forceinline__ void tmem_dealloc2(uint32_t base) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLS) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

@@ -133,7 +133,7 @@ struct WeighGeo {
   static constexpr uint32_t kK = 128 * D * 2, kGroup = D * 16;
   static constexpr uint32_t kQ = 64 * D * 2;
   static constexpr uint32_t kStages = 4, kMeta = 4, kBufs = 3, kTK = 384;
-  static constexpr uint32_t kSmem = kK + kStages * kQ;
+  static constexpr uint32_t kSmem = D == 256 ? kK + kStages * kQ : 160 * 1024;  // one CTA an SM, and none that holds tensor memory
 };
 constexpr uint32_t kSumWarps = 16, kWeighThreads = (kSumWarps + 3) * 32;  // 16: the exponentials bound the sums
 
@@ -188,7 +188,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
     fail_sh = 0;
     fence_mbar_init();
   }
-  if (warp == kSumWarps + 1) tmem_alloc2(&tmem_sh);
+  if (warp == kSumWarps + 1) tmem_alloc2<512>(&tmem_sh);
   pdl_wait();
   const int32_t len = paged_len(a.c, b), k0 = (int32_t)(kt * 256);
   const int2 rr = paged_rows(a.c, b);
@@ -445,7 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
   }
   __syncwarp();
   cluster_sync();  // nothing of one CTA is used by the other after this
-  if (warp == kSumWarps + 1) tmem_dealloc2(tmem);
+  if (warp == kSumWarps + 1) tmem_dealloc2<512>(tmem);
 }
 
 // Queries as (64 elements, head of the group, token, chunk of 64, KV head): a box is one chunk
