@@ -4,18 +4,17 @@
 #include <string>
 
 #include "paged_attend.cuh"
+#include "paged_rows.cuh"
 
 namespace snl {
 namespace {
-
-constexpr uint32_t kRowWarps = 8, kBlock = 64;  // keys of a block: 8 of each warp
 
 // Shared memory: each warp's ring of stages (8 keys of K, then of V, each [64-element chunk]
 // [8 keys][128 bytes], 128-byte swizzled), then each warp's output for up to 8 heads.
 template <int D>
 struct RowGeo {
   static constexpr uint32_t kGroup = D * 16, kStage = 2 * kGroup;
-  static constexpr uint32_t kStages = D == 256 ? 2 : 5;
+  static constexpr uint32_t kStages = 2, kPerSm = D == 256 ? 1 : 2;
   static constexpr uint32_t kRing = kRowWarps * kStages * kStage;
   static constexpr uint32_t kSmem = kRing + kRowWarps * 8 * D * 4;
 };
@@ -55,47 +54,6 @@ __device__ __forceinline__ uint32_t row_blocks(const RowKeys& k) {
   return k.lo < k.hi ? ((uint32_t)k.hi + kBlock - 1) / kBlock - (uint32_t)k.lo / kBlock : 0;
 }
 
-template <typename T>
-__device__ __forceinline__ void mma_k16(float d[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {  // rows 8-15 of A are 0
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1));
-}
-template <typename T>
-__device__ __forceinline__ void mma_k8(float d[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(b0));
-  else
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(b0));
-}
-__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t r[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-// Into this CTA's memory; the box is 8 slots of a head.
-__device__ __forceinline__ void tma_group(uint32_t dst, const CUtensorMap* map, int slot, int head, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], [%6];" ::"r"(
-          dst),
-      "l"(map), "r"(0), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // Where a walk over the blocks stands: blocks of (KV head, row) in that order of importance.
 struct Walk {
   uint64_t left;  // blocks, this one included
@@ -124,7 +82,7 @@ __device__ __forceinline__ void next_block(const RowArgs& A, Walk& w) {
 // boxes: S = Q K^T on m16n8k16 (query heads as rows), O^T += V^T P^T on m16n8k8, whose B
 // operand is the score fragment as it stands.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32, 1)
+__global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
     attend_rows_kernel(const __grid_constant__ RowArgs A, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   using G = RowGeo<D>;
@@ -228,11 +186,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
   const uint32_t g = lane >> 2, t = lane & 3;
   const float flip = a.m.scale < 0.f ? -1.f : 1.f, sl = fmaxf(fabsf(a.m.scale) * kLog2e, 1e-30f) * flip;
   const float cap = a.m.cap, pre = cap > 0.f ? a.m.scale / cap : 0.f;
-  // ldmatrix: lane L addresses row L % 8 of matrix L / 8, 16 bytes each, four along a row
-  const uint32_t lrow = lane & 7, lsel = lane >> 3;
-  auto lds = [&](uint32_t at, uint32_t c) {  // elements 32 c to 32 c + 31 of the 8 keys
-    return at + (c / 2) * 1024 + lrow * 128 + ((((c & 1) * 4 + lsel) ^ lrow) << 4);
-  };
   bool ok = true;
   uint32_t q[D / 16][2];
   float o[D / 16][4];
@@ -267,9 +220,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
 #pragma unroll
       for (uint32_t c = 0; c < D / 32; c++) {
         uint32_t kb[4];
-        ldsm4(kb, lds(kat, c));
-        mma_k16<T>(s0, q[2 * c][0], q[2 * c][1], kb[0], kb[1]);
-        mma_k16<T>(s1, q[2 * c + 1][0], q[2 * c + 1][1], kb[2], kb[3]);
+        ldsm4(kb, box_at(kat, c, lane));
+        mma_k16<T>(s0, q[2 * c][0], 0, q[2 * c][1], 0, kb[0], kb[1]);  // rows 8-15 are not used
+        mma_k16<T>(s1, q[2 * c + 1][0], 0, q[2 * c + 1][1], 0, kb[2], kb[3]);
       }
       // head g, keys `key` and key + 1
       float x0 = s0[0] + s1[0], x1 = s0[1] + s1[1];
@@ -308,7 +261,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
 #pragma unroll
       for (uint32_t c = 0; c < D / 32; c++) {
         uint32_t v[4];
-        ldsm4_t(v, lds(vat, c));
+        ldsm4_t(v, box_at(vat, c, lane));
         mma_k8<T>(o[2 * c], v[0] & keep, v[1] & keep, p);
         mma_k8<T>(o[2 * c + 1], v[2] & keep, v[3] & keep, p);
       }
@@ -433,7 +386,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) rows_join_kernel(const __grid
 uint32_t rows_grid(const snl_paged_cache& c, const snl_paged_batch& b) {
   const uint64_t len = std::min<uint64_t>(b.max_len, (uint64_t)b.table_stride * c.page_size);
   const uint64_t most = (uint64_t)b.n_rows * c.n_kv * ((len + kBlock - 1) / kBlock + 1);
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (uint64_t)std::max(1, sm_count())));
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (uint64_t)std::max(1, sm_count()) * (c.head_dim == 256 ? RowGeo<256>::kPerSm : RowGeo<128>::kPerSm)));
 }
 
 template <typename T, int D>

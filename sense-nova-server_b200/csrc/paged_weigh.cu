@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <string>
 
-#include "paged_tc.cuh"
+#include "paged_rows.cuh"
 
 namespace snl {
 namespace {
@@ -30,95 +30,223 @@ __device__ __forceinline__ float log2_sum(float lse) { return lse == -INFINITY ?
 
 // ---- few rows: one pass over the keys ------------------------------------------------------
 
-constexpr uint32_t kWeighWarps = 8, kWeighGroups = 4;  // 8-key groups of one warp
+template <int D>
+struct WeighRowGeo {
+  static constexpr uint32_t kStage = D * 16;  // 8 keys
+  static constexpr uint32_t kStages = D == 256 ? 3 : 6, kPerSm = 2;  // a group's chain of steps is long: two CTAs an SM
+  static constexpr uint32_t kSmem = kRowWarps * kStages * kStage;
+};
 
-// One warp takes 8 keys (of one page) at a time, a lane D / 32 elements of each; the products
-// with 4 heads at once are 32 sums over the lanes, folded so that each lane ends with one.
+// Where a walk over the blocks of (KV head, sequence) stands.
+struct WeighWalk {
+  uint64_t left;
+  uint32_t kh, b, blk, end;
+  int32_t len, lo, hi;  // keys that some row sees
+  int2 rows;
+};
+__device__ __forceinline__ void enter_seq(const WeighArgs& a, WeighWalk& w) {
+  w.len = paged_len(a.c, w.b);
+  w.rows = paged_rows(a.c, w.b);
+  w.end = ((uint32_t)w.len + kBlock - 1) / kBlock;
+  w.lo = INT32_MAX, w.hi = 0;
+  for (int32_t r = w.rows.x; r < w.rows.y; r++) {
+    const int2 keys = paged_keys(a.m, r, w.len - (w.rows.y - r), w.len);
+    if (keys.x < keys.y) w.lo = min(w.lo, keys.x), w.hi = max(w.hi, keys.y);
+  }
+}
+__device__ __forceinline__ void next_block(const WeighArgs& a, WeighWalk& w) {
+  w.left--;
+  w.blk++;
+  while (w.left && w.blk >= w.end) {
+    if (++w.b == a.c.n_seqs) w.b = 0, w.kh++;
+    enter_seq(a, w);
+    w.blk = 0;
+  }
+}
+
+// The blocks of 64 keys of all (KV head, sequence) pairs form one line that is cut into equal
+// shares, one for each CTA. A warp takes 8 keys of each block through its own ring of TMA
+// boxes: S = Q K^T on m16n8k16 with the heads of two rows as the 16 rows, so a key's sum over
+// heads and rows is one over the lanes of its column.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWeighWarps * 32, 2) weigh_rows_kernel(const __grid_constant__ WeighArgs a) {
-  constexpr int E = D / 32, W = E / 2;
+__global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
+    weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ CUtensorMap kmap) {
+  using G = WeighRowGeo<D>;
+  constexpr uint32_t NS = G::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t bars[kRowWarps][NS];
+  __shared__ uint32_t scan_sh[kRowWarps], found_sh[2];
   pdl_trigger();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023) {
+    report_timeout(a.c.err);
+    return;
+  }
+  if (lane == 0)
+    for (uint32_t s = 0; s < NS; s++) mbar_init(&bars[warp][s], 1);
+  fence_mbar_init();
   pdl_wait();
-  const uint32_t lane = threadIdx.x & 31, kh = blockIdx.y, b = blockIdx.z;
-  const int32_t len = paged_len(a.c, b);
-  const int32_t key0 = (int32_t)((blockIdx.x * kWeighWarps + (threadIdx.x >> 5)) * kWeighGroups * 8);
-  if (key0 >= len) return;
-  const int2 rr = paged_rows(a.c, b);
-  auto load = [&](int32_t key, uint32_t (&x)[8][W]) -> int32_t {
-    const int32_t page = key < len ? paged_page(a.c, b, key) : -1;
+
+  // Blocks before each thread's sequences, this CTA's share, and the sequence that it starts in.
+  const uint32_t per = (a.c.n_seqs + kRowWarps * 32 - 1) / (kRowWarps * 32), b0 = min(tid * per, a.c.n_seqs),
+                 b1 = min(b0 + per, a.c.n_seqs);
+  auto blocks = [&](uint32_t b) { return ((uint32_t)paged_len(a.c, b) + kBlock - 1) / kBlock; };
+  uint32_t mine = 0;
+  for (uint32_t b = b0; b < b1; b++) mine += blocks(b);
+  uint32_t upto = mine;
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-#pragma unroll
-      for (int e = 0; e < W; e++) x[k][e] = 0;
-      if (page < 0 || key + k >= len) continue;
-      const uint16_t* s = a.c.k + paged_at(a.c, page, kh, key + k) + lane * E;
-      if constexpr (E == 8) {
-        const uint4 v = ld_stream16(s);
-        x[k][0] = v.x, x[k][1] = v.y, x[k][2] = v.z, x[k][3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(s);
-        x[k][0] = v.x, x[k][1] = v.y;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= (uint32_t)o) upto += v;
+  }
+  if (lane == 31) scan_sh[warp] = upto;
+  __syncthreads();
+  uint32_t total = 0;
+  for (uint32_t i = 0; i < kRowWarps; i++) {
+    if (i < warp) upto += scan_sh[i];
+    total += scan_sh[i];
+  }
+  const uint64_t all = (uint64_t)total * a.c.n_kv, share = (all + gridDim.x - 1) / gridDim.x, g0 = blockIdx.x * share;
+  if (g0 >= all) return;
+  const uint64_t g1 = min(g0 + share, all);
+  {
+    uint32_t off = (uint32_t)(g0 % total);
+    if (off >= upto - mine && off < upto) {
+      off -= upto - mine;
+      uint32_t b = b0;
+      for (;; b++) {
+        const uint32_t n = blocks(b);
+        if (off < n) break;
+        off -= n;
       }
+      found_sh[0] = b;
+      found_sh[1] = off;
     }
-    return page;
+  }
+  __syncthreads();
+  WeighWalk now;
+  now.left = g1 - g0;
+  now.kh = (uint32_t)(g0 / total);
+  now.b = found_sh[0];
+  enter_seq(a, now);
+  now.blk = found_sh[1];
+  WeighWalk ahead = now;  // of the loads
+
+  const uint32_t ring = smem_u32(smem) + warp * NS * G::kStage;
+  int32_t pages = -1;  // of this warp's keys in 32 blocks from `base` on, one a lane
+  uint32_t base = 0xFFFFFFFFu, pseq = 0xFFFFFFFFu, issued = 0, taken = 0;
+  auto active = [&](const WeighWalk& w) {
+    const int32_t key = (int32_t)(w.blk * kBlock + warp * 8);
+    return key + 8 > w.lo && key < w.hi;
   };
-  uint32_t x[8][W], next[8][W];
-  load(key0, x);
-  for (uint32_t n = 0; n < kWeighGroups; n++) {
-    const int32_t key = key0 + (int32_t)n * 8, mine = key + (int32_t)(lane & 7);
-    if (key >= len) return;
-    if (n + 1 < kWeighGroups) load(key + 8, next);
-    float sum = 0.f;
-    for (int32_t r = rr.x; r < rr.y; r++) {
-      const int32_t t = len - (rr.y - r);
-      const int2 keys = paged_keys(a.m, r, t, len);
-      if (key + 8 <= keys.x || key >= keys.y) continue;
-      for (uint32_t g = 0; g < a.group; g += 4) {
-        float v[32];
+  auto issue = [&] {  // the next group that this warp has to read, if any
+    while (ahead.left) {
+      const bool use = active(ahead);
+      if (use) {
+        if (pseq != ahead.b || ahead.blk - base >= 32) {
+          pseq = ahead.b;
+          base = ahead.blk;
+          const uint32_t key = (base + lane) * kBlock + warp * 8;
+          pages = (int32_t)key < ahead.len ? paged_page(a.c, ahead.b, key) : -1;
+        }
+        const int32_t page = __shfl_sync(0xffffffffu, pages, ahead.blk - base);
+        if (lane == 0) {
+          const uint32_t st = issued % NS;
+          mbar_arrive_expect_tx(&bars[warp][st], G::kStage);
+          tma_group(ring + st * G::kStage, &kmap, (int)((ahead.blk * kBlock + warp * 8) & ((1u << a.c.shift) - 1)),
+                    (int)ahead.kh, page < 0 ? (int)a.c.n_pages : page, &bars[warp][st]);
+        }
+        issued++;
+      }
+      next_block(a, ahead);
+      if (use) return;
+    }
+  };
+  for (uint32_t s = 0; s < NS; s++) issue();
+
+  const uint32_t g = lane >> 2, t = lane & 3;
+  const float cap = a.m.cap;
+  bool ok = true, fresh = true;
+  uint32_t q[D / 16][4];
+  float z[2] = {0.f, 0.f}, slope = 0.f;
+  auto load_rows = [&](int32_t r0) {  // rows r0 and r0 + 1: this lane's head g of each
+    const uint32_t head = now.kh * a.group + g;
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
-          float q[E];
-          if (g + h < a.group) {
-            load_as_float<E>(a.q, (uint64_t)r * a.p.q_row + (uint64_t)(kh * a.group + g + h) * a.p.q_head + lane * E,
-                             std::is_same<T, __half>::value ? SNL_T_F16 : SNL_T_BF16, q);
-          } else {
+    for (int e = 0; e < 2; e++) {
+      const bool there = g < a.group && r0 + e < now.rows.y;
+      const uint16_t* s = a.q + (uint64_t)(r0 + e) * a.p.q_row + (uint64_t)head * a.p.q_head + 2 * t;
 #pragma unroll
-            for (int e = 0; e < E; e++) q[e] = 0.f;
+      for (int c = 0; c < D / 16; c++) {
+        q[c][e] = there ? *reinterpret_cast<const uint32_t*>(s + 16 * c) : 0;
+        q[c][2 + e] = there ? *reinterpret_cast<const uint32_t*>(s + 16 * c + 8) : 0;
+      }
+      z[e] = there ? log2_sum(__ldg(a.lse + (uint64_t)(r0 + e) * a.p.n_heads + head)) : INFINITY;
+    }
+    slope = a.m.slopes && g < a.group ? __ldg(a.m.slopes + head) : 0.f;
+  };
+  while (now.left) {
+    if (fresh) load_rows(now.rows.x);
+    fresh = false;
+    const int32_t key0 = (int32_t)(now.blk * kBlock + warp * 8), key = key0 + 2 * (int32_t)t;
+    if (key0 < now.len) {
+      // The old weights of the lane's two keys come beside the scores.
+      const int32_t old_len = now.len - (now.rows.y - now.rows.x), page = paged_page(a.c, now.b, key0);
+      float2* at = reinterpret_cast<float2*>(a.c.weight + paged_weight_at(a.c, max(page, 0), now.kh, key));
+      float2 w = make_float2(0.f, 0.f);
+      if (g == 0 && page >= 0) w = *at;
+      float sum0 = 0.f, sum1 = 0.f;
+      if (active(now)) {
+        const uint32_t st = taken % NS, box = ring + st * G::kStage;
+        ok = __all_sync(0xffffffffu, ok && wait_mbar(&bars[warp][st], (taken / NS) & 1));
+        taken++;
+        for (int32_t r0 = now.rows.x; r0 < now.rows.y; r0 += 2) {
+          if (now.rows.y - now.rows.x > 2) load_rows(r0);  // a sequence of more rows than most
+          float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (uint32_t c = 0; c < D / 32; c++) {
+            uint32_t kb[4];
+            ldsm4(kb, box_at(box, c, lane));
+            mma_k16<T>(s0, q[2 * c][0], q[2 * c][1], q[2 * c][2], q[2 * c][3], kb[0], kb[1]);
+            mma_k16<T>(s1, q[2 * c + 1][0], q[2 * c + 1][1], q[2 * c + 1][2], q[2 * c + 1][3], kb[2], kb[3]);
           }
 #pragma unroll
-          for (int k = 0; k < 8; k++) {
-            float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int e = 0; e < W; e++) s = fma2(unpack2(x[k][e], T()), make_float2(q[2 * e], q[2 * e + 1]), s);
-            v[h * 8 + k] = s.x + s.y;
+          for (int e = 0; e < 4; e++) {  // row r0 + e / 2, key + e % 2
+            const int32_t r = r0 + e / 2, k = key + e % 2, pos = now.len - (now.rows.y - r);
+            if (r >= now.rows.y || g >= a.group) continue;
+            const int2 keys = paged_keys(a.m, r, pos, now.len);
+            if (k < keys.x || k >= keys.y) continue;
+            float s = (s0[e] + s1[e]) * a.m.scale;
+            if (cap > 0.f) s = cap * tanh_(s / cap);
+            if (a.m.slopes) s -= slope * fabsf((float)(pos - k));
+            const float p = ex2(fmaf(s, kLog2e, -z[e / 2]));
+            if (e % 2) sum1 += p;
+            else sum0 += p;
           }
         }
+        fence_proxy_async_smem();  // the stage was read; the next box is written to it after that
+        __syncwarp();
+        issue();
+      }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const bool up = lane & o;
-#pragma unroll
-          for (int i = 0; i < o; i++) {
-            const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-        }
-        // lane 8 h + k: head g + h, key + k
-        const uint32_t h = g + lane / 8, head = kh * a.group + h;
-        if (h < a.group && mine >= keys.x && mine < keys.y) {
-          float s = v[0] * a.m.scale;
-          if (a.m.cap > 0.f) s = a.m.cap * tanh_(s / a.m.cap);
-          if (a.m.slopes) s -= __ldg(a.m.slopes + head) * fabsf((float)(t - mine));
-          sum += ex2(fmaf(s, kLog2e, -log2_sum(__ldg(a.lse + (uint64_t)r * a.p.n_heads + head))));
-        }
+      for (int o = 4; o < 32; o <<= 1) {
+        sum0 += __shfl_xor_sync(0xffffffffu, sum0, o);
+        sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
+      }
+      if (g == 0 && page >= 0) {
+        w.x = a.decay != 0.f && key < old_len ? fmaf(w.x, a.decay, sum0) : sum0;
+        w.y = a.decay != 0.f && key + 1 < old_len ? fmaf(w.y, a.decay, sum1) : sum1;
+        if (key + 1 < now.len) *at = w;
+        else if (key < now.len) at->x = w.x;
       }
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-    if (lane < 8 && mine < len) put_weight(a, b, kh, mine, len - (rr.y - rr.x), sum);
-#pragma unroll
-    for (int k = 0; k < 8; k++)
-#pragma unroll
-      for (int e = 0; e < W; e++) x[k][e] = next[k][e];
+    const uint32_t b = now.b, kh = now.kh;
+    next_block(a, now);
+    fresh = now.b != b || now.kh != kh;
+  }
+  if (!ok) {
+    // A wait gave up: this warp's boxes still in flight land before the CTA ends.
+    if (lane == 0) report_timeout(a.c.err);
+    for (uint32_t i = issued > NS ? issued - NS : 0; i < issued; i++) (void)wait_mbar(&bars[warp][i % NS], (i / NS) & 1);
   }
 }
 
@@ -466,12 +594,26 @@ int query_map(CUtensorMap* map, const snl_paged_cache& c, const snl_paged_batch&
 
 template <typename T, int D>
 int go_weigh(const snl_paged_cache& c, const snl_paged_batch& b, const WeighArgs& a, cudaStream_t s) {
-  // Few rows a sequence: the keys are read once and the products are few. From about 3 rows on
-  // the tensor cores' passes are the shorter ones.
-  if (b.n_rows <= 2 * (uint64_t)b.n_seqs) {
-    const uint32_t per = kWeighWarps * kWeighGroups * 8;
-    SNL_PDL_LAUNCH("weigh_rows_kernel", (weigh_rows_kernel<T, D>), dim3((a.c.max_len + per - 1) / per, c.n_kv, b.n_seqs),
-                   dim3(kWeighWarps * 32), (size_t)0, s, a);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < 64, general = a.m.cap > 0.f || a.m.slopes;
+  auto allow = [&](auto kern, bool* done, uint32_t smem) -> int {
+    if (known && done[dev]) return SNL_OK;
+    SNL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (known) done[dev] = true;
+    return SNL_OK;
+  };
+  // Few rows a sequence: the keys are read once and the products are few (two rows of up to 8
+  // heads are one tile of them).
+  if (a.group <= 8 && b.n_rows <= 2 * (uint64_t)b.n_seqs && (uint64_t)b.n_seqs * (a.c.max_len / kBlock + 1) < (1ull << 31)) {
+    static bool attr[64] = {};
+    SNL_TRY(allow(weigh_rows_kernel<T, D>, attr, WeighRowGeo<D>::kSmem));
+    CUtensorMap km;
+    SNL_TRY(page_map(&km, c, c.k, 8, D / 64));
+    const uint64_t most = (uint64_t)b.n_seqs * c.n_kv * ((a.c.max_len + kBlock - 1) / kBlock);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(most, (uint64_t)std::max(1, sm_count()) * WeighRowGeo<D>::kPerSm);
+    SNL_PDL_LAUNCH("weigh_rows_kernel", (weigh_rows_kernel<T, D>), dim3(grid), dim3(kRowWarps * 32),
+                   (size_t)WeighRowGeo<D>::kSmem, s, a, km);
     return SNL_OK;
   }
   CUtensorMap km, qm;
@@ -479,19 +621,13 @@ int go_weigh(const snl_paged_cache& c, const snl_paged_batch& b, const WeighArgs
   SNL_TRY(query_map(&qm, c, b, a.p, a.q, a.group, a.toks));
   const uint64_t grid = 2ull * c.n_kv * b.n_seqs * ((a.c.max_len + 255) / 256);
   if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, "snl_paged_weigh: too many keys");
-  auto go = [&](auto kern, bool& done) -> int {
-    if (!done) SNL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WeighGeo<D>::kSmem));
-    done = true;
+  static bool attr[2][64] = {};
+  auto go = [&](auto kern, bool* done) -> int {
+    SNL_TRY(allow(kern, done, WeighGeo<D>::kSmem));
     SNL_PDL_LAUNCH("weigh_tile_kernel", kern, dim3((unsigned)grid), dim3(kWeighThreads), (size_t)WeighGeo<D>::kSmem, s, a, km, qm);
     return SNL_OK;
   };
-  static bool attr[2][64] = {};
-  bool none = false;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const bool known = dev >= 0 && dev < 64, general = a.m.cap > 0.f || a.m.slopes;
-  return general ? go(weigh_tile_kernel<T, D, true>, known ? attr[1][dev] : none)
-                 : go(weigh_tile_kernel<T, D, false>, known ? attr[0][dev] : none);
+  return general ? go(weigh_tile_kernel<T, D, true>, attr[1]) : go(weigh_tile_kernel<T, D, false>, attr[0]);
 }
 
 }  // namespace
@@ -509,6 +645,7 @@ extern "C" int snl_paged_weigh(const snl_paged_cache* c, const snl_paged_batch* 
   if (!c->weight) return fail(SNL_E_INVALID, w + ": the cache has no weights");
   if (!(decay >= 0.f) || decay > 3e38f) return fail(SNL_E_INVALID, w + ": decay must be finite and not negative");
   if (!paged_aligned(q)) return fail(SNL_E_INVALID, w + ": q rows must be aligned to 16 bytes");
+  if (!paged_aligned(c->weight)) return fail(SNL_E_INVALID, w + ": the weights must be aligned to 16 bytes");
   if (b->n_seqs == 0 || a.c.max_len == 0) return SNL_OK;
   SNL_TRY(paged_error_word(&a.c.err));
   a.p = *p;
