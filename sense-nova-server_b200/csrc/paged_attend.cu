@@ -87,7 +87,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   __shared__ volatile int fail_sh;
   __shared__ int odd_v;
   pdl_trigger();
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
+  const uint32_t tid = threadIdx.x, warp = same_in_warp(tid >> 5), lane = tid & 31, rank = same_in_warp(cluster_rank());
   const uint32_t kh = (blockIdx.x / 2) % a.c.n_kv, unit = (blockIdx.x / 2) / a.c.n_kv;
   const uint32_t split = unit % a.n_split, slot = a.slots - 1 - unit / a.n_split;
   uint8_t *smem_k = smem_q + G::kQ, *smem_v = smem_k + NK * G::kTile;
@@ -125,7 +125,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_sh;
+  const uint32_t tmem = same_in_warp(tmem_sh);
   const TileInfo w = info_sh;  // of the cluster: up to 2 a.toks tokens
 
   // Row of this thread (both warpgroups hold all 128): token and head, its keys.
@@ -190,7 +190,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   // scores would outgrow the reference at every tile of the other order.
   const int32_t c0 = (int32_t)(split * a.split_len);
   const int32_t beg = max(lo0 == INT32_MAX ? 0 : lo0, c0), end = min(hi1, c0 + (int32_t)a.split_len);
-  const uint32_t j0 = beg < end ? (uint32_t)beg / KT : 0, nt = beg < end ? ((uint32_t)end + KT - 1) / KT - j0 : 0, jl = j0 + nt - 1;
+  const uint32_t j0 = same_in_warp(beg < end ? (uint32_t)beg / KT : 0);
+  const uint32_t nt = same_in_warp(beg < end ? ((uint32_t)end + KT - 1) / KT - j0 : 0), jl = j0 + nt - 1;
   // Tiles with a key that some row of the cluster does not see.
   auto masked_tile = [&](uint32_t j) { return (int32_t)(j * KT) < lo1 || (int32_t)(j * KT + KT) > hi0; };
 

@@ -14,7 +14,7 @@ struct WeighArgs {
   const uint16_t* q;
   const float* lse;
   float decay;
-  uint32_t group, toks;  // query heads per KV head; tokens of half a query tile (64 / group)
+  uint32_t group, toks;  // query heads per KV head; tokens of half a query tile (32 / group, at least 1)
 };
 
 // The new weight of a slot: sums start at 0 for the step's own slots.
@@ -252,23 +252,24 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
 
 // ---- many rows: S^T = K Q^T on the tensor cores ---------------------------------------------
 
-// Shared memory of one CTA: its 128 keys [8-key group][64-element chunk][8 keys][128 bytes],
-// and stages of half a query tile [chunk][64 rows][128 bytes]. Tensor memory: three tiles of
-// 128 keys x 128 (token, head) rows, and from column 384 the keys, the products' A operand
-// (from shared memory it and the queries would take the whole of its bandwidth).
+// Shared memory of one CTA: stages of half a query tile [chunk][32 rows][128 bytes], the last
+// four of them in the place of its 128 keys [8-key group][64-element chunk][8 keys][128 bytes],
+// which are there first and move to tensor memory. Tensor memory, half of an SM's: two tiles of
+// 128 keys x 64 (token, head) rows, and from column 128 the keys, the products' A operand.
+// Two CTAs share an SM: the sums' latencies of one pass beside the other's products.
 template <int D>
 struct WeighGeo {
   static constexpr uint32_t kK = 128 * D * 2, kGroup = D * 16;
-  static constexpr uint32_t kQ = 64 * D * 2;
-  static constexpr uint32_t kStages = 4, kMeta = 4, kBufs = 3, kTK = 384;
-  static constexpr uint32_t kSmem = D == 256 ? kK + kStages * kQ : 160 * 1024;  // one CTA an SM, and none that holds tensor memory
+  static constexpr uint32_t kQ = 32 * D * 2;
+  static constexpr uint32_t kStages = 6, kMeta = 8, kBufs = 2, kTK = 128;
+  static constexpr uint32_t kSmem = D == 256 ? 2 * kQ + kK : 80 * 1024;  // at most two CTAs an SM
 };
-constexpr uint32_t kSumWarps = 16, kWeighThreads = (kSumWarps + 3) * 32;  // 16: the exponentials bound the sums
+constexpr uint32_t kSumWarps = 8, kWeighThreads = (kSumWarps + 3) * 32, kCols = 64;
 
-// What the sums need of a query tile's 128 rows (read 16 bytes at a time).
+// What the sums need of a query tile's 64 rows (read 16 bytes at a time).
 struct alignas(16) WeighMeta {
-  float lse2[128], t[128], slope[128];
-  int32_t lo[128], hi[128];
+  float lse2[kCols], t[kCols], slope[kCols];
+  int32_t lo[kCols], hi[kCols];
   int32_t tile;  // -1: no more tiles
   int32_t full;  // every row sees every key of the cluster
 };
@@ -278,22 +279,22 @@ struct alignas(16) WeighMeta {
 // the rows needs no exchange. The last warp lists the query tiles that see the keys, with what
 // each row needs; one loads their queries by TMA, one of the first CTA issues the products.
 template <typename T, int D, bool GENERAL>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 2)
     weigh_tile_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap qmap) {
   using G = WeighGeo<D>;
   constexpr uint32_t NS = G::kStages, NM = G::kMeta, NB = G::kBufs;
-  extern __shared__ __align__(1024) uint8_t smem_k[];
-  uint8_t* smem_q = smem_k + G::kK;
+  extern __shared__ __align__(1024) uint8_t smem_q[];
+  uint8_t* smem_k = smem_q + 2 * G::kQ;
   __shared__ WeighMeta meta[NM];
-  __shared__ uint64_t k_full, q_full[NS], q_empty[NS], m_full[NM], m_empty[NM], s_full[G::kBufs], s_empty[G::kBufs], k_there, drained;
+  __shared__ uint64_t k_full, q_full[NS], q_empty[NS], m_full[NM], m_empty[NM], s_full[G::kBufs], s_empty[G::kBufs], k_there, k_moved, drained;
   __shared__ uint32_t tmem_sh;
-  __shared__ float part_sh[3][128];
+  __shared__ float part_sh[128];
   __shared__ volatile int fail_sh;
   pdl_trigger();
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
+  const uint32_t tid = threadIdx.x, warp = same_in_warp(tid >> 5), lane = tid & 31, rank = same_in_warp(cluster_rank());
   const uint32_t cl = blockIdx.x / 2, kh = cl % a.c.n_kv, b = cl / a.c.n_kv % a.c.n_seqs, kt = cl / a.c.n_kv / a.c.n_seqs;
-  if (smem_u32(smem_k) & 1023) {  // the swizzle needs it; the same for every CTA
+  if (smem_u32(smem_q) & 1023) {  // the swizzle needs it; the same for every CTA
     report_timeout(a.c.err);
     return;
   }
@@ -312,21 +313,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
       mbar_init(&s_empty[s], 2 * kSumWarps);  // of both CTAs
     }
     mbar_init(&k_there, 2 * kSumWarps);
+    mbar_init(&k_moved, kSumWarps);
     mbar_init(&drained, 1);
     fail_sh = 0;
     fence_mbar_init();
   }
-  if (warp == kSumWarps + 1) tmem_alloc2<512>(&tmem_sh);
+  if (warp == kSumWarps + 1) tmem_alloc2<256>(&tmem_sh);
   pdl_wait();
   const int32_t len = paged_len(a.c, b), k0 = (int32_t)(kt * 256);
   const int2 rr = paged_rows(a.c, b);
   const int32_t rows = rr.y - rr.x, t0 = len - rows;
-  const uint32_t per = 2 * a.toks, tiles = k0 < len ? ((uint32_t)rows + per - 1) / per : 0;
+  // A half tile is toks whole tokens; of more than 32 heads, half of one token's.
+  const bool wide = a.group > 32;
+  const uint32_t per = wide ? 1 : 2 * a.toks, tiles = k0 < len ? ((uint32_t)rows + per - 1) / per : 0;
   const int32_t k1 = min(k0 + 256, len);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_sh;
+  const uint32_t tmem = same_in_warp(tmem_sh);
   cluster_sync();
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -334,27 +338,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
   };
   float sum = 0.f;
   if (warp == kSumWarps + 2) {
-    // A lane has columns lane + 32 e. The next tile's sums are on their way while this one's
+    // A lane has column `lane` of both halves. The next tile's sums are on their way while this one's
     // wait for their place.
     struct Cols {
       uint32_t i;
-      int32_t lo[4], hi[4], row[4], full;
-      float lse[4];
+      int32_t lo[2], hi[2], row[2], full;
+      float lse[2];
     };
     // Token of the tile (past any sequence for a column without a row) and head of each column.
-    uint32_t tok0[4], head[4];
+    uint32_t tok0[2], head[2];
 #pragma unroll
-    for (uint32_t e = 0; e < 4; e++) {
-      const uint32_t col = lane + 32 * e, in = col % 64;
-      tok0[e] = in < a.toks * a.group ? (col / 64) * a.toks + in / a.group : 1u << 30;
-      head[e] = kh * a.group + in % a.group;
+    for (uint32_t e = 0; e < 2; e++) {
+      if (wide) {
+        tok0[e] = e * 32 + lane < a.group ? 0 : 1u << 30;
+        head[e] = kh * a.group + e * 32 + lane;
+      } else {
+        tok0[e] = lane < a.toks * a.group ? e * a.toks + lane / a.group : 1u << 30;
+        head[e] = kh * a.group + lane % a.group;
+      }
     }
     // The first tile from i on that sees a key, or `tiles`.
     auto find = [&](uint32_t i, Cols& x) {
       for (; i < tiles; i++) {
         int32_t ulo = INT32_MAX, uhi = 0, ilo = 0, ihi = INT32_MAX;  // of the union, of the intersection
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) {
+        for (uint32_t e = 0; e < 2; e++) {
           const uint32_t tok = i * per + tok0[e];
           int2 keys = make_int2(0, 0);
           x.row[e] = -1;
@@ -375,7 +383,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
         if (ulo >= k1 || uhi <= k0) continue;
         x.full = __reduce_max_sync(0xffffffffu, ilo) <= k0 && __reduce_min_sync(0xffffffffu, ihi) >= k0 + 256;
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++)
+        for (uint32_t e = 0; e < 2; e++)
           x.lse[e] = x.row[e] < 0 ? -INFINITY
                                   : __ldg(a.lse + (uint64_t)x.row[e] * a.p.n_heads + head[e]);
         break;
@@ -394,7 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
       WeighMeta& m = meta[ms];
       if (now.i < tiles) {
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) {
+        for (uint32_t e = 0; e < 2; e++) {
           const uint32_t col = lane + 32 * e;
           m.lse2[col] = log2_sum(now.lse[e]);
           m.lo[col] = now.lo[e];
@@ -436,14 +444,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cta(&m_empty[ms]);
       if (tile < 0) break;
+      if (n == 2) wait(&k_moved, 0);  // the stages from here on are the keys' place
       if (n >= NS) wait(&q_empty[st], (n / NS - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&q_full[st], 2 * (D / 64) * a.toks * a.group * 128);
+      if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&q_full[st], 2 * (D / 64) * (wide ? 32 : a.toks * a.group) * 128);
       __syncwarp();
       if (lane < D / 64)  // (64 elements, head of the group, token, chunk, KV head)
-        tma_load_5d(smem_u32(smem_q) + st * G::kQ + lane * 8192, &qmap, 0, rr.x + tile * (int32_t)per + (int32_t)(rank * a.toks),
-                    (int)lane, (int)kh, in_cta(&q_full[st], 0));
+        tma_query(smem_u32(smem_q) + st * G::kQ + lane * 4096, &qmap, wide ? (int)(rank * 32) : 0,
+                  rr.x + tile * (int32_t)per + (wide ? 0 : (int32_t)(rank * a.toks)), (int)lane, (int)kh, in_cta(&q_full[st], 0));
     }
     if (!ok && lane == 0) fail_sh = 1;
     if (tiles) (void)wait_mbar(&k_full, 0);
@@ -473,12 +482,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
         continue;
       }
       tc_fence_after();
-      const uint32_t b_lo = desc_lo(smem_u32(smem_q) + n % NS * G::kQ, 16), d = tmem + n % NB * 128;
+      const uint32_t b_lo = __reduce_max_sync(0xffffffffu, desc_lo(smem_u32(smem_q) + n % NS * G::kQ, 16)),
+                     d = __reduce_max_sync(0xffffffffu, tmem + n % NB * kCols);  // into uniform registers
       // The waits for the next tile pass while the first half of this one's products is at work.
 #pragma unroll
       for (uint32_t kk = 0; kk < D / 16; kk++) {
         if (kk == D / 32) more = ready(n + 1);
-        mma2_ts(lead, d, tmem + G::kTK + kk * 8, b_lo + (kk / 4) * 512 + (kk % 4) * 2, desc_hi(1024), idesc16<T>(128, false),
+        mma2_ts(lead, d, tmem + G::kTK + kk * 8, b_lo + (kk / 4) * 256 + (kk % 4) * 2, desc_hi(1024), idesc16<T>(kCols, false),
                 kk != 0);
       }
       commit2(lead, &q_empty[n % NS]);
@@ -498,20 +508,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
     const uint32_t wg = warp >> 2, lanes = ((warp & 3) * 32) << 16, kl = tid & 127;
     const int32_t key = k0 + (int32_t)(rank * 128 + kl);
     const float sl = a.m.scale * kLog2e, cap = a.m.cap, pre = GENERAL && cap > 0.f ? a.m.scale / cap : 0.f;
-    if (tiles) {  // the keys into tensor memory, a quarter of head_dim each
+    if (tiles) {  // the keys into tensor memory, half of head_dim each
       wait(&k_full, 0);
       ok = __all_sync(0xffffffffu, ok);
-      uint32_t r[D / 8];
 #pragma unroll
-      for (uint32_t u = 0; u < D / 32; u++) {
-        const uint32_t c = wg * (D / 32) + u;  // 16 bytes of the row
-        const uint4 x = *reinterpret_cast<const uint4*>(smem_k + kl / 8 * G::kGroup + c / 8 * 1024 + kl % 8 * 128 + ((c % 8 ^ kl % 8) << 4));
-        r[4 * u] = x.x, r[4 * u + 1] = x.y, r[4 * u + 2] = x.z, r[4 * u + 3] = x.w;
+      for (uint32_t c0 = 0; c0 < D / 16; c0 += 8) {  // 16-byte pieces of the row
+        uint32_t r[32];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++) {
+          const uint32_t c = wg * (D / 16) + c0 + u;
+          const uint4 x = *reinterpret_cast<const uint4*>(smem_k + kl / 8 * G::kGroup + c / 8 * 1024 + kl % 8 * 128 + ((c % 8 ^ kl % 8) << 4));
+          r[4 * u] = x.x, r[4 * u + 1] = x.y, r[4 * u + 2] = x.z, r[4 * u + 3] = x.w;
+        }
+        tm_st32(tmem + lanes + G::kTK + wg * (D / 4) + c0 * 4, r);
       }
-      tm_st<D / 8>(tmem + lanes + G::kTK + wg * (D / 8), r);
+      fence_proxy_async_smem();  // the keys' place is read; boxes of queries are written to it next
       tm_wait_st();
       tc_fence_before();
       __syncwarp();
+      if (lane == 0) mbar_arrive_cta(&k_moved);
       if (lane == 0) arrive_cluster(in_cta(&k_there, 0), false);
     }
     for (uint32_t n = 0;; n++) {
@@ -525,7 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
       tc_fence_after();
       float s[32];
       uint32_t* r = reinterpret_cast<uint32_t*>(s);
-      tm_ld32(tmem + lanes + buf * 128 + wg * 32, r);
+      tm_ld32(tmem + lanes + buf * kCols + wg * 32, r);
       tm_wait_ld<32>(r);
       tc_fence_before();
       __syncwarp();
@@ -566,14 +581,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 1)
       if (lane == 0) mbar_arrive_cta(&m_empty[ms]);
     }
     if (!ok && lane == 0) fail_sh = 1;
-    if (wg) part_sh[wg - 1][kl] = sum;
+    if (wg) part_sh[kl] = sum;
     bar_sync(1, kSumWarps * 32);
-    if (wg == 0 && key < len)
-      put_weight(a, b, kh, key, len - rows, (sum + part_sh[0][kl]) + (part_sh[1][kl] + part_sh[2][kl]));
+    if (wg == 0 && key < len) put_weight(a, b, kh, key, len - rows, sum + part_sh[kl]);
   }
   __syncwarp();
   cluster_sync();  // nothing of one CTA is used by the other after this
-  if (warp == kSumWarps + 1) tmem_dealloc2<512>(tmem);
+  if (warp == kSumWarps + 1) tmem_dealloc2<256>(tmem);
 }
 
 // Queries as (64 elements, head of the group, token, chunk of 64, KV head): a box is one chunk
@@ -585,7 +599,7 @@ int query_map(CUtensorMap* map, const snl_paged_cache& c, const snl_paged_batch&
   const cuuint64_t dims[5] = {64, group, b.n_rows, c.head_dim / 64, c.n_kv};
   const cuuint64_t str[4] = {group > 1 ? p.q_head * 2 : 128, b.n_rows > 1 ? p.q_row * 2 : 128, 128,
                              c.n_kv > 1 ? p.q_head * group * 2 : 128};
-  const cuuint32_t box[5] = {64, group, toks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+  const cuuint32_t box[5] = {64, std::min(group, 32u), toks, 1, 1}, one[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(map, c.type == SNL_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                          const_cast<void*>(q), dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -653,7 +667,7 @@ extern "C" int snl_paged_weigh(const snl_paged_cache* c, const snl_paged_batch* 
   a.lse = lse;
   a.decay = decay;
   a.group = p->n_heads / c->n_kv;
-  a.toks = 64 / a.group;
+  a.toks = std::max(1u, 32 / a.group);
   const cudaStream_t s = (cudaStream_t)stream;
   if (c->type == SNL_T_F16) return c->head_dim == 256 ? go_weigh<__half, 256>(*c, *b, a, s) : go_weigh<__half, 128>(*c, *b, a, s);
   return c->head_dim == 256 ? go_weigh<__nv_bfloat16, 256>(*c, *b, a, s) : go_weigh<__nv_bfloat16, 128>(*c, *b, a, s);
