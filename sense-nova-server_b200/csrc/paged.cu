@@ -247,14 +247,14 @@ __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* sh, uint32
 }
 
 // One CTA per (KV head, sequence): the n-th largest key of the candidates by four 8-bit radix
-// passes (equal digits of a warp are counted by one addition: weights crowd in few
-// exponents), then the kept slots in slot order, 4096 at a time. A thread takes four
+// passes (weights crowd in few exponents: eight counts of each digit, by lane, on banks of
+// their own), then the kept slots in slot order, 4096 at a time. A thread takes four
 // neighbouring slots, which lie in one page. The weights are read once where their keys fit
 // shared memory.
 template <bool HELD>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t held[];
-  __shared__ uint32_t hist[256], warp_n[32], s_digit, s_need;
+  __shared__ uint32_t hist[8][260], warp_n[32], s_digit, s_need;
   pdl_trigger();
   pdl_wait();
   const uint32_t kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   const uint32_t take = a.p.budget - a.p.sink - a.p.recent;
   uint32_t cut = 0, need = take;  // the keys' common prefix so far, and how many of it are taken
   for (int shift = 24; take && shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+    for (uint32_t i = tid; i < 8 * 260; i += kSelectThreads) hist[0][i] = 0;
     __syncthreads();
     for (int32_t base = 0; base < len; base += kSelectKeys) {
       const int32_t t = base + 4 * (int32_t)tid;
@@ -294,17 +294,21 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
       const uint32_t ks[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const bool in = ks[e] && (shift == 24 || ks[e] >> (shift + 8) == cut >> (shift + 8));
-        const uint32_t d = in ? (ks[e] >> shift) & 255 : 256;
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
-        if (in && lane == (uint32_t)__ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
+        if (ks[e] && (shift == 24 || ks[e] >> (shift + 8) == cut >> (shift + 8))) atomicAdd(&hist[lane & 7][(ks[e] >> shift) & 255], 1u);
       }
+    }
+    __syncthreads();
+    if (tid < 256) {
+      uint32_t s = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) s += hist[i][tid];
+      hist[0][tid] = s;
     }
     __syncthreads();
     if (tid < 32) {  // the digit at which the sum from the top reaches `need`: 8 digits a lane
       uint32_t n[8], s = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) s += n[e] = hist[255 - 8 * lane - e];
+      for (int e = 0; e < 8; e++) s += n[e] = hist[0][255 - 8 * lane - e];
       uint32_t upto = s;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

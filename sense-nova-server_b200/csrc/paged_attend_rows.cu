@@ -32,8 +32,17 @@ struct RowKeys {
   int32_t lo, hi, t, len;
 };
 __device__ __forceinline__ RowKeys row_keys(const PagedView& c, const PagedMask& m, uint32_t r) {
-  uint32_t b = min(r, c.n_seqs - 1);
-  if ((uint32_t)__ldg(c.start + b) > r || (uint32_t)__ldg(c.start + b + 1) <= r) {  // mostly start[b] = b
+  uint32_t b = min(r, c.n_seqs - 1);  // mostly start[b] = b
+  const int32_t s0 = __ldg(c.start + b), s1 = __ldg(c.start + b + 1), n = __ldg(c.len + b);
+  const int32_t first = m.first ? __ldg(m.first + r) : 0;
+  if (s0 == (int32_t)r && s1 == (int32_t)r + 1 && s1 <= (int32_t)c.n_rows && n > 0 && n <= c.max_len) {
+    // the sequence's only row, at its last slot, which no `last` can pass: nothing more to look up
+    RowKeys k{b, m.window ? max(first, n - m.window) : first, n, n - 1, n};
+    k.lo = max(k.lo, 0);
+    if (k.lo >= k.hi) k.lo = k.hi = 0;
+    return k;
+  }
+  if (s0 > (int32_t)r || s1 <= (int32_t)r) {
     uint32_t lo = 0, hi = c.n_seqs;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
@@ -348,12 +357,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) rows_join_kernel(const __grid
   const uint32_t r = (uint32_t)(item / a.p.n_heads), hq = (uint32_t)(item % a.p.n_heads), kh = hq / a.group, h = hq % a.group;
   pdl_wait();
   if (r >= a.c.n_rows) return;
+  const int2 span = A.span[(uint64_t)r * a.c.n_kv + kh];  // not set for a row without keys
   const RowKeys k = row_keys(a.c, a.m, r);
   float l = 0.f, zero = 0.f, o[E];
 #pragma unroll
   for (int i = 0; i < E; i++) o[i] = 0.f;
   if (k.lo < k.hi) {
-    const int2 span = A.span[(uint64_t)r * a.c.n_kv + kh];
     if (span.x == span.y) return;  // written already
     auto place = [&](int c) { return ((uint64_t)c * 2 + (c == span.x ? 1 : 0)) * a.group + h; };
     float top = -INFINITY;

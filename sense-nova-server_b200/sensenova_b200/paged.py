@@ -55,7 +55,7 @@ def _ints(t, what: str, *shape: int) -> int:
 def _floats(t, what: str, *shape: int) -> int | None:
     if t is None:
         return None
-    if not (_type_of.get(t.dtype, -1) == ffi.SNL_T_F32 or _type(t) == ffi.SNL_T_F32) or t.shape != shape or not t.is_contiguous():
+    if _type(t) != 0 or t.shape != shape or not t.is_contiguous():
         _fail(f"{what} must be contiguous float32 of shape {shape}")
     return t.data_ptr()
 
@@ -93,8 +93,11 @@ class PagedCache:
 
     def _rows(self, t, what: str, batch: PagedBatch, heads: int) -> tuple[int, int, int]:
         """Address and row and head strides of [rows, heads, head_dim]."""
-        row, head, one = t.stride() if t.dim() == 3 else (0, 0, 0)
-        if one != 1 or t.shape != (batch.n_rows, heads, self.head_dim):
+        if t.shape == (batch.n_rows, heads, self.head_dim):
+            row, head, one = t.stride()
+        else:
+            one = 0
+        if one != 1:
             _fail(f"{what} must be [{batch.n_rows}, {heads}, {self.head_dim}] with a contiguous last dimension")
         return t.data_ptr(), row, head
 
