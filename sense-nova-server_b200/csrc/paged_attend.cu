@@ -290,8 +290,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
     const uint32_t ready[2] = {in_cta(&p_ready[0], 0), in_cta(&p_ready[1], 0)};
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = __all_sync(0xffffffffu, ok && (mbar_try_wait(bar, parity) || (!fail_sh && wait_mbar(bar, parity))));
-      if (!ok) fail_sh = 1;
+      if (!mbar_try_wait(bar, parity)) {
+        ok = ok && !fail_sh && wait_mbar(bar, parity);
+        if (!ok) fail_sh = 1;
+      }
+      __syncwarp();
     };
     // Tiles with a key that some row of this warp (one without keys counts) does not see.
     const bool some = keys.x < keys.y;
@@ -326,7 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
         }
         float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (uint32_t c = 4; c < NC; c++) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+        for (uint32_t c = 4; c < NC; c += 2) m4[(c / 2) & 3] = fmaxf(fmaxf(m4[(c / 2) & 3], s[c]), s[c + 1]);
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if constexpr (!GENERAL) mx *= sl;
         // The tile's maximum from both halves; after this barrier both have read their scores, which
