@@ -260,6 +260,51 @@ def test_bad_indices_are_reported(lib):
     assert lib.snl_device_error(1) == 4 and torch.equal(got[20:], want[20:])
 
 
+@pytest.mark.parametrize("d,rows", [(128, 1), (256, 1), (128, 3), (256, 3)])
+def test_attend_many_sequences(d, rows):
+    """More sequences than one look at 32 boundaries finds, lengths of every kind."""
+    lens = [max(rows, (i * 37) % 90) if i % 11 else 0 for i in range(260)]
+    p = Problem(lens, [min(n, rows) for n in lens], 8, 2, d, 8, seed=d + rows)
+    check_attend(p)
+    check_attend(p, **masks_of(p, window=20, slopes=True))
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_attend_uneven_rows(d):
+    """At most two rows a sequence on the average, many in one; two rows in each."""
+    check_attend(Problem([300, 70, 5, 90, 64, 1, 33], [9, 1, 0, 1, 1, 1, 1], 8, 2, d, seed=1))
+    check_attend(Problem([300, 70, 5, 900], [2, 2, 2, 2], 8, 1, d, seed=2), window=200)
+    check_attend(Problem([40, 130], [2, 1], 6, 2, d, seed=3), cap=9.0)
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_attend_zero_scale(rows):
+    """Equal scores: the mean of the values."""
+    p = Problem([333], [rows], 4, 1, seed=19)
+    check_attend(p, scale=0.0)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attend_generous_bounds(rows):
+    """max_len and the table's rows far past the lengths: parts that no sequence reaches."""
+    p = Problem([200, 64, 900], [rows] * 3, 8, 2, seed=20, width=3000, max_len=40000)
+    check_attend(p)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_pages_inside_a_wider_pool(rows):
+    """k and v as the halves of one tensor per page, two layers deep."""
+    p = Problem([200, 77], [rows, rows], 8, 2, 256, 16, seed=21, weight=True)
+    want, lse = run_attend(p)
+    pool = torch.full((p.k.shape[0], 2, 2, 2, 16, 264), math.nan, dtype=F16, device="cuda")
+    k, v = pool[:, 1, 0, :, :, :256], pool[:, 1, 1, :, :, :256]
+    k.copy_(p.k), v.copy_(p.v)
+    p.k, p.v = k, v
+    got, z = run_attend(p)
+    assert torch.equal(got, want) and torch.equal(z, lse)
+    check_weigh(p)
+
+
 # ---- append --------------------------------------------------------------------------------
 
 
@@ -389,6 +434,29 @@ def test_weigh_hides_what_is_not_seen():
     assert not p.weight[pg, :, sl].isnan().any()
 
 
+@pytest.mark.parametrize("heads", [33, 40, 17, 64])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_weigh_large_groups(heads, rows):
+    """Heads of one KV head that do not divide a tile, or fill more than half of one."""
+    check_weigh(Problem([150, 300], [rows, 21 if rows > 1 else 1], heads, 1, 128, seed=heads, weight=True))
+
+
+@pytest.mark.parametrize("d,rows", [(128, 1), (256, 1), (128, 3), (256, 3)])
+def test_weigh_many_sequences(d, rows):
+    lens = [max(rows, (i * 37) % 90) if i % 11 else 0 for i in range(150)]
+    check_weigh(Problem(lens, [min(n, rows) for n in lens], 8, 2, d, 8, seed=d + rows, weight=True), 0.5)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_weigh_uneven_rows(d):
+    check_weigh(Problem([300, 70, 5, 90, 64, 1, 33], [9, 1, 0, 1, 1, 1, 1], 8, 2, d, seed=1, weight=True))
+    check_weigh(Problem([300, 70, 5, 900], [2, 2, 2, 2], 8, 1, d, seed=2, weight=True), window=200, cap=20.0)
+
+
+def test_weigh_long():
+    check_weigh(Problem([3000, 2100], [700, 1], 8, 2, 256, 64, seed=22, weight=True), 0.9)
+
+
 def test_weigh_sums_to_the_rows():
     """Every row hands out a weight of one per head."""
     p = Problem([700], [90], 8, 2, seed=14, weight=True)
@@ -460,6 +528,19 @@ def test_evict_ties_and_odd_weights(values, in_place):
         p.weight = torch.stack([x, x - 0.5, x * 1e-42, torch.full_like(x, math.inf), torch.full_like(x, -math.inf),
                                 torch.full_like(x, math.nan)])[pick, *torch.meshgrid(*[torch.arange(n, device="cuda") for n in x.shape], indexing="ij")]
     check_evict(p, 350, 2, 30, in_place)
+
+
+@pytest.mark.parametrize("budget", [1000, 57000])
+def test_evict_long(budget):
+    """More candidates than shared memory holds keys of."""
+    p = Problem([60000], [1], 2, 1, 128, 64, seed=23, weight=True, spare=-(-budget // 64))
+    check_evict(p, budget, 4, 64, False)
+
+
+def test_evict_many_sequences():
+    lens = [(i * 53) % 200 for i in range(70)]
+    p = Problem(lens, [min(n, 1) for n in lens], 4, 2, 128, 8, seed=24, weight=True, spare=70 * 8)
+    check_evict(p, 60, 2, 10, False)
 
 
 # ---- together --------------------------------------------------------------------------------
