@@ -124,7 +124,9 @@ class PagedCache:
             _need(two == 2 and pos is not None, "rope must be [positions, rot / 2, 2] and pos be given")
             rot = 2 * half
             rp, tp = _floats(rope, "rope", n_pos, half, 2), _ints(pos, "pos", batch.n_rows, 4)
-        p = PagedAppendP(heads, _type(k), rot, axes, pairs, n_pos, sections, eps, q_row, q_head, k_row, k_head, v_row,
+        if len(sections) != 3:
+            _fail("sections must be the numbers of pairs of the three axes")
+        p = PagedAppendP(heads, _type(k), rot, axes, pairs, n_pos, tuple(sections), eps, q_row, q_head, k_row, k_head, v_row,
                          v_head, out_row, out_head)
         rc = self.lib.snl_paged_append(self.ref, batch.ref, p, qp, kp, vp, _floats(q_norm, "q_norm", d),
                                        _floats(k_norm, "k_norm", d), tp, rp, op, stream)

@@ -624,3 +624,25 @@ def test_matches_the_contiguous_cache(lib):
     assert torch.equal(p.v[pg, :, sl], vc.view(n, kv, 256))
     out, _ = run_attend(p, q_out, per[:, :, 256:], out_dtype=F32)
     assert (out.view(n, -1) - want).abs().max() < 4e-3 * want.abs().max()
+
+
+def test_serving_example(lib, capsys):
+    """The example's prompts, eviction and tokens; chunks of a prompt give what one chunk does."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(paged.__file__).resolve().parent.parent / "examples"))
+    import paged_serving as ex
+
+    out, layer = ex.serve(budget=192, steps=3)
+    assert layer.lens == [195, 48, 132] and layer.seen == [303, 48, 132] and out.isfinite().all()
+    assert sorted(layer.free + [p for t in layer.tables for p in t]) == list(range(128))
+    again, _ = ex.serve(budget=192, steps=3)
+    assert torch.equal(out, again)
+    x = torch.randn(200, 256, device="cuda")
+    a, b = (ex.PagedLayer(ex.small(), pages=32) for _ in range(2))
+    whole = a.step([a.add()], [x])
+    s = b.add()
+    parts = torch.cat([b.step([s], [x[i:j]]) for i, j in ((0, 150), (150, 151), (151, 200))])
+    # values of order 1; the projections' rows come from two kernels (1e-4), attention rounds to 2^-11
+    assert (whole - parts).abs().max() < 5e-3 * whole.abs().max()

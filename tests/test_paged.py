@@ -83,6 +83,7 @@ def test_append_refusals(lib):
     refused("SNL_E_INVALID", "pos must be", a, batch, q, k, k, q, pos[:, :3], rope)
     refused("SNL_E_INVALID", "add up to rot_dim / 2", a, batch, q, k, k, q, pos, rope, axes=paged.SECTIONS,
             sections=(11, 11, 11))
+    refused("SNL_E_INVALID", "three axes", a, batch, q, k, k, q, pos, rope, sections=[11, 21])
     refused("SNL_E_INVALID", "unknown rotary layout", a, batch, q, k, k, q, pos, rope, axes=3)
     refused("SNL_E_UNSUPPORTED", "invalid rotary dim", a, batch, q, k, k, q, pos, torch.zeros(10, 129, 2))
     refused("SNL_E_INVALID", "q_norm must be", a, batch, q, k, k, q, q_norm=torch.zeros(128))
