@@ -281,7 +281,8 @@ size_t snl_sample_scratch_bytes(void);
  * see is bounded there: a page number outside the cache, a length over max_len or the
  * table's pages, a start array that leaves [0, n_rows], a position outside the rotary table. Such an
  * entry is not read or written, its results are undefined, and bit 2 (value 4) of
- * snl_device_error() is set. */
+ * snl_device_error() is set. Sequences may share pages that a call only reads (a common
+ * prefix); the slots that append, weigh or evict write belong to one sequence. */
 
 /* Element types of q, k, v, gate and out. */
 enum { SNL_T_F32 = 0, SNL_T_F16 = 1, SNL_T_BF16 = 2 };

@@ -591,7 +591,7 @@ int go_attend(const AttendArgs& a, const CUtensorMap& km, const CUtensorMap& vm,
 
 extern "C" size_t snl_paged_attend_workspace(const snl_paged_cache* c, const snl_paged_batch* b, uint32_t n_heads) {
   if (!c || !b || c->n_kv == 0 || n_heads == 0 || n_heads % c->n_kv || n_heads / c->n_kv > 64) return 0;
-  if (attend_rows_fits(*b, n_heads / c->n_kv)) return std::max<size_t>(16, attend_rows_workspace(*c, *b, n_heads / c->n_kv));
+  if (attend_rows_fits(*c, *b, n_heads / c->n_kv)) return std::max<size_t>(16, attend_rows_workspace(*c, *b, n_heads / c->n_kv));
   return part_bytes(plan_attend(*c, *b, n_heads), *c, *b, n_heads);
 }
 
@@ -619,7 +619,7 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
   a.lse = lse;
   a.group = p->n_heads / c->n_kv;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (attend_rows_fits(*b, a.group)) return launch_attend_rows(*c, *b, a, work, s);
+  if (attend_rows_fits(*c, *b, a.group)) return launch_attend_rows(*c, *b, a, work, s);
   const AttendPlan pl = plan_attend(*c, *b, p->n_heads);
   const uint64_t grid = (uint64_t)pl.slots * pl.n_split * c->n_kv * 2;
   if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, w + ": too many rows");

@@ -21,7 +21,7 @@ struct AttendArgs {
 };
 
 // One or two rows a sequence (paged_attend_rows.cu).
-bool attend_rows_fits(const snl_paged_batch& b, uint32_t group);
+bool attend_rows_fits(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t group);
 size_t attend_rows_workspace(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t group);
 int launch_attend_rows(const snl_paged_cache& c, const snl_paged_batch& b, const AttendArgs& a, void* work, cudaStream_t s);
 

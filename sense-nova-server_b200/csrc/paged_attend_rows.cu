@@ -420,10 +420,17 @@ int go_rows(const snl_paged_cache& c, const RowArgs& r, uint32_t grid, cudaStrea
 
 }  // namespace
 
-// The query heads of a KV head are rows of one 16-row product whose last 8 are not used; rows
-// beyond two a sequence would read its keys again for each.
-bool attend_rows_fits(const snl_paged_batch& b, uint32_t group) {
-  return group <= 8 && b.n_rows <= 2 * (uint64_t)b.n_seqs && (uint64_t)b.n_rows * (b.max_len / kBlock + 2) < (1ull << 31);
+// The query heads of a KV head are rows of one 16-row product whose last 8 are not used. A
+// second row of a sequence reads its keys again here, where a tile of the other kernel holds
+// all rows: at head_dim 256 and 27 rows of 16 sequences of up to 32768 keys 212 us against 182
+// (single rows 193 against 243), at 13 rows of 8 of up to 2048 keys 24 against 26, and 2 rows of
+// one 17 against 21; at head_dim 128 and 104 rows of 64 sequences of up to 4096 keys 129
+// against 161.
+bool attend_rows_fits(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t group) {
+  const uint64_t blocks = (uint64_t)b.n_rows * (b.max_len / kBlock + 2);
+  const bool small = blocks * c.n_kv <= 8192, wide = c.head_dim == 256;
+  return group <= 8 && blocks < (1ull << 31) &&
+         (wide && !small ? 4ull * b.n_rows <= 5ull * b.n_seqs : b.n_rows <= 2ull * b.n_seqs);
 }
 
 size_t attend_rows_workspace(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t group) {

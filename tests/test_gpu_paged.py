@@ -117,8 +117,9 @@ def test_attend_masks(mask, d, rows):
     check_attend(p, **masks_of(p, **MASKS[mask]))
 
 
-def test_attend_nothing_seen():
-    p = Problem([200, 40], [70, 1], seed=3)
+@pytest.mark.parametrize("rows", [[70, 1], [1, 1]])
+def test_attend_nothing_seen(rows):
+    p = Problem([200, 40], rows, seed=3)
     out, lse = run_attend(p, first=torch.full((p.n,), 2**31 - 1, dtype=torch.int32, device="cuda"))
     assert (out == 0).all() and torch.isneginf(lse).all()
 
@@ -209,8 +210,9 @@ def test_attend_same_bits_every_time(rows):
         assert torch.equal(a, b) and torch.equal(z, y)
 
 
-def test_attend_other_stream_and_graph():
-    p = Problem([1500, 64], [1, 1], 8, 2, seed=10)
+@pytest.mark.parametrize("d,rows", [(256, 1), (256, 40), (128, 40)])
+def test_attend_other_stream_and_graph(d, rows):
+    p = Problem([1500, 64], [rows, rows], 8, 2, d, seed=10)
     a, _ = run_attend(p)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
@@ -274,6 +276,7 @@ def test_attend_uneven_rows(d):
     """At most two rows a sequence on the average, many in one; two rows in each."""
     check_attend(Problem([300, 70, 5, 90, 64, 1, 33], [9, 1, 0, 1, 1, 1, 1], 8, 2, d, seed=1))
     check_attend(Problem([300, 70, 5, 900], [2, 2, 2, 2], 8, 1, d, seed=2), window=200)
+    check_attend(Problem([30000, 21000], [2, 1], 32, 8, d, 64, seed=25))  # more blocks than the few-row kernel takes at 256
     check_attend(Problem([40, 130], [2, 1], 6, 2, d, seed=3), cap=9.0)
 
 
