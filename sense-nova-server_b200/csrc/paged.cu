@@ -45,7 +45,9 @@ enum { kTurnNone, kTurnLane, kTurnShuffle, kTurnShared };
 
 // One warp takes up to NH query, key or value heads of a row: the row's slot, the turn's (cos,
 // sin) and the norm's weights are looked up once for them, while all their elements are on
-// the way. A lane holds D / 32 neighbouring elements.
+// the way. A lane holds D / 32 neighbouring elements. Two chunks of up to 4096 rows of 16 + 8
+// heads: 43 us (184 MB, 4.3 TB/s, 0.66 of a copy's rate; 116 us with a warp for each head,
+// whose look-ups were most of its instructions); 8 rows are one launch's latency.
 template <int D, int TURN, bool IN32>
 __global__ void __launch_bounds__(kAppendWarps * 32, IN32 ? 3 : 4) append_kernel(const __grid_constant__ AppendArgs a, uint32_t span) {
   constexpr int E = D / 32, NH = append_heads(D), W = E * (IN32 ? 4 : 2) / 4;  // words of a lane's elements
@@ -250,7 +252,8 @@ __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* sh, uint32
 // passes (weights crowd in few exponents: eight counts of each digit, by lane, on banks of
 // their own), then the kept slots in slot order, 4096 at a time. A thread takes four
 // neighbouring slots, which lie in one page. The weights are read once where their keys fit
-// shared memory.
+// shared memory. 32 lists of up to 16384 weights take 22 us, the copy of their 4096 kept slots
+// 43 us (269 MB in all).
 template <bool HELD>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t held[];

@@ -67,7 +67,9 @@ __device__ __forceinline__ void next_block(const WeighArgs& a, WeighWalk& w) {
 // The blocks of 64 keys of all (KV head, sequence) pairs form one line that is cut into equal
 // shares, one for each CTA. A warp takes 8 keys of each block through its own ring of TMA
 // boxes: S = Q K^T on m16n8k16 with the heads of two rows as the 16 rows, so a key's sum over
-// heads and rows is one over the lanes of its column.
+// heads and rows is one over the lanes of its column. 8 tokens over up to 16384 keys: 36 us
+// (142 MB, 3.9 TB/s, 0.61 of a copy's rate: the chain of a group's steps, not the bytes;
+// 52 with one CTA an SM, 72 with products on the FMA units).
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
     weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ CUtensorMap kmap) {
@@ -276,8 +278,11 @@ struct alignas(16) WeighMeta {
 
 // A cluster = (256 keys of a sequence and KV head), a CTA 128 of them, thread = key: the
 // scores of a query tile come with a key's row in one lane of tensor memory, so its sum over
-// the rows needs no exchange. The last warp lists the query tiles that see the keys, with what
-// each row needs; one loads their queries by TMA, one of the first CTA issues the products.
+// the rows needs no exchange, and its order is fixed. The last warp lists the query tiles that
+// see the keys, with what each row needs; one loads their queries by TMA, one of the first CTA
+// issues the products. 2048 rows of 16 heads over 8192 keys: 152 us (790 TFLOP/s), the tensor
+// pipe active 41% and the special-function unit 42% of the time: both wait on the hand-over
+// between them, and 128 clusters are 1.7 for each pair of SMs.
 template <typename T, int D, bool GENERAL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 2)
     weigh_tile_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ CUtensorMap kmap,
