@@ -380,8 +380,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
         tm_st<NC / 2>(tm_s + wg * (NC / 2), r);
         tm_wait_st();
       }
-      const bool masked = masked_tile(jl - i);
-      if (masked) {
+      bool mended = false;
+      if (masked_tile(jl - i)) {
         // A row's probability for a key that it does not see is 0, but 0 * NaN is not: values that
         // are not finite leave the tile, and reach the rows that see them at the end.
         ok = __all_sync(0xffffffffu, ok && wait_cluster(&v_landed, landed & 1));
@@ -398,6 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
             if (b0 | b1 | b2 | b3) {
               const int32_t key = (int32_t)((jl - i) * KT + e * 16 / (vrun * D) * vrun + e * 16 % (vrun * 128) / 128);
               odd = odd || (key >= lo0 && key < hi1);
+              mended = true;
               tile[e] = make_uint4(x.x & ~b0, x.y & ~b1, x.z & ~b2, x.w & ~b3);
             }
           }
@@ -405,12 +406,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
             odd_v = 1;
             asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(in_cta(&odd_v, rank ^ 1)) : "memory");
           }
-          fence_proxy_async_smem();
+          mended = __any_sync(0xffffffffu, mended);  // seldom: the MMAs read what was written then
+          if (mended) fence_proxy_async_smem();
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_cluster(ready[i & 1], masked);
+      if (lane == 0) arrive_cluster(ready[i & 1], mended);
     }
     if (nt) wait(&pv_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1);
   }
