@@ -90,7 +90,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   using G = Geo<D>;
   constexpr uint32_t KT = G::KT, NK = G::kStagesK, NV = G::kStagesV;
   extern __shared__ __align__(1024) uint8_t smem_q[];
-  __shared__ uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_ready[2], pv_done[2], v_landed, drained;
+  __shared__ uint64_t k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_ready[2], pv_done[2], v_landed, q_ready, drained;
   __shared__ uint32_t tmem_sh;
   __shared__ TileInfo info_sh;
   __shared__ int32_t lohi[4][kSoftWarps / 2];  // per warp: least and largest lo, least and largest hi
@@ -122,11 +122,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
       mbar_init(&pv_done[s], 1);
     }
     mbar_init(&v_landed, 1);
+    mbar_init(&q_ready, 2 * kSoftWarps);
     mbar_init(&drained, 1);
     fail_sh = 0;
     odd_v = 0;
     fence_mbar_init();
   }
+  __syncwarp();
+  cluster_arrive();  // the barriers of this CTA are there
   if (warp == 9) tmem_alloc2<G::kCols>(&tmem_sh);
   pdl_wait();
   if (warp == 8) {
@@ -143,6 +146,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   const uint32_t row = tid & 127, tok0 = row / a.group, head = kh * a.group + row % a.group;
   const uint32_t tok = tok0 + rank * a.toks;
   const bool mine = warp < kSoftWarps && tok0 < a.toks, valid = mine && tok < w.toks;
+  // Queries into shared memory, the sign of the scale folded in; the first of them are on their
+  // way while the rows' keys are looked up, all of them while the first tiles come.
+  // 16-byte pieces of a row; loads on their way at once
+  constexpr uint32_t per = D / 8, batch = 8, batches = G::kQ / 16 / (batch * kSoftWarps * 32);
+  uint4 x[batch];
+  auto fetch_q = [&](uint32_t n) {
+#pragma unroll
+    for (uint32_t i = 0; i < batch; i++) {
+      const uint32_t e = tid + (n * batch + i) * kSoftWarps * 32, r = e / per, u = e % per, t0 = r / a.group, t = t0 + rank * a.toks;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (t0 < a.toks && t < w.toks)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (uint64_t)(w.row0 + t) * a.p.q_row +
+                                                    (uint64_t)(kh * a.group + r - t0 * a.group) * a.p.q_head + 8 * u));
+    }
+  };
+  if (warp < kSoftWarps) fetch_q(0);
   int2 keys = make_int2(0, 0);
   if (valid) keys = paged_keys(a.m, w.row0 + tok, w.t0 + (int32_t)tok, w.len);
   if (warp < kSoftWarps / 2) {
@@ -163,31 +182,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
     }
   }
   const float sl = fmaxf(fabsf(a.m.scale) * kLog2e, 1e-30f);  // not 0: -inf of a masked score has to stay
+  cluster_wait();  // the other CTA's barriers are there
+  __syncthreads();
   if (warp < kSoftWarps) {
-    // Queries into shared memory, the sign of the scale folded in.
     const uint32_t flip = a.m.scale < 0.f ? 0x80008000u : 0u;
-    constexpr uint32_t per = D / 8, batch = 8;  // 16-byte pieces of a row; loads on their way at once
-    for (uint32_t e0 = tid; e0 < G::kQ / 16; e0 += batch * kSoftWarps * 32) {
-      uint4 x[batch];
+#pragma unroll
+    for (uint32_t n = 0; n < batches; n++) {
+      if (n) fetch_q(n);
 #pragma unroll
       for (uint32_t i = 0; i < batch; i++) {
-        const uint32_t e = e0 + i * kSoftWarps * 32, r = e / per, u = e % per, t0 = r / a.group, t = t0 + rank * a.toks;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (t0 < a.toks && t < w.toks)
-          x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (uint64_t)(w.row0 + t) * a.p.q_row +
-                                                      (uint64_t)(kh * a.group + r - t0 * a.group) * a.p.q_head + 8 * u));
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < batch; i++) {
-        const uint32_t e = e0 + i * kSoftWarps * 32, r = e / per, u = e % per;
+        const uint32_t e = tid + (n * batch + i) * kSoftWarps * 32, r = e / per, u = e % per;
         x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
         *reinterpret_cast<uint4*>(smem_q + (u / 8) * 16384 + r * 128 + ((u % 8 ^ r % 8) << 4)) = x[i];
       }
     }
     fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) arrive_cluster(in_cta(&q_ready, 0), true);
   }
-  __syncthreads();
-  cluster_sync();  // barriers and queries of both CTAs are there
   int32_t lo0 = lohi[0][0], lo1 = lohi[1][0], hi0 = lohi[2][0], hi1 = lohi[3][0];
 #pragma unroll
   for (uint32_t i = 1; i < kSoftWarps / 2; i++) {
@@ -265,7 +277,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
         commit2(lead, &k_empty[st]);
         commit2(lead, &s_full[i & 1]);
       };
-      if (nt) scores(0);
+      if (nt) {
+        ok = __all_sync(0xffffffffu, wait_cluster(&q_ready, 0));
+        if (ok) scores(0);
+      }
       for (uint32_t i = 0; ok && i < nt; i++) {
         if (i + 1 < nt) scores(i + 1);
         const uint32_t st = i % NV;
@@ -472,25 +487,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
         *reinterpret_cast<float4*>(turn + lane * 36 + e) =
             l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
       __syncwarp();
+      // Gates are loaded ahead of the stores, which no later load may pass: as many as registers hold.
+      auto put = [&](auto gated) {
+        constexpr bool with_gate = decltype(gated)::value;
+        constexpr uint32_t ahead = !with_gate ? 1 : D == 256 ? 8 : 2;
+        uint4 g4[ahead];
 #pragma unroll
-      for (uint32_t it = 0; it < 8; it++) {
-        const uint32_t row = it * 4 + lane / 8, col = lane % 8 * 4;
-        const uint64_t to = __shfl_sync(0xffffffffu, out_at, row), from = __shfl_sync(0xffffffffu, gate_at, row);
-        if (!(some_rows >> row & 1)) continue;
-        const float4 x = *reinterpret_cast<const float4*>(turn + row * 36 + col);
-        float v[4] = {x.x, x.y, x.z, x.w};
-        if (parts) {
-          store_from_float<4>(a.part, to + c + col, SNL_T_F32, v);
-          continue;
-        }
-        if (a.gate) {
-          float g[4];
-          load_as_float<4>(a.gate, from + c + col, a.p.gate_type, g);
+        for (uint32_t it = 0; it < 8; it++) {
+          if (with_gate && it % ahead == 0) {
 #pragma unroll
-          for (int f = 0; f < 4; f++) v[f] *= sigmoidf_(g[f]);
+            for (uint32_t i = 0; i < ahead; i++) {
+              const uint32_t row = (it + i) * 4 + lane / 8;
+              const uint64_t from = __shfl_sync(0xffffffffu, gate_at, row) + c + lane % 8 * 4;
+              g4[i] = make_uint4(0, 0, 0, 0);
+              if (!(some_rows >> row & 1)) continue;
+              if (a.p.gate_type == SNL_T_F32) {
+                g4[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.gate) + from));
+              } else {
+                const uint2 h = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.gate) + from));
+                g4[i].x = h.x, g4[i].y = h.y;
+              }
+            }
+          }
+          const uint32_t row = it * 4 + lane / 8, col = lane % 8 * 4;
+          const uint64_t to = __shfl_sync(0xffffffffu, out_at, row);
+          if (!(some_rows >> row & 1)) continue;
+          const float4 y = *reinterpret_cast<const float4*>(turn + row * 36 + col);
+          float v[4] = {y.x, y.y, y.z, y.w};
+          if constexpr (with_gate) {
+            float g[4];
+            load_as_float<4>(&g4[it % ahead], 0, a.p.gate_type, g);
+#pragma unroll
+            for (int f = 0; f < 4; f++) v[f] *= sigmoidf_(g[f]);
+          } else if (parts) {
+            store_from_float<4>(a.part, to + c + col, SNL_T_F32, v);
+            continue;
+          }
+          store_from_float<4>(a.out, to + c + col, a.p.out_type, v);
         }
-        store_from_float<4>(a.out, to + c + col, a.p.out_type, v);
-      }
+      };
+      if (a.gate && !parts) put(std::true_type());
+      else put(std::false_type());
     }
     tc_fence_before();
   }
