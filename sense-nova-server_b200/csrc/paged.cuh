@@ -25,13 +25,13 @@ struct PagedView {
 
 __device__ __forceinline__ void report_index(int* err) { atomicOr(err, kPagedBadIndex); }
 
-// Length of sequence b, in [0, max_len].
-__device__ __forceinline__ int32_t paged_len(const PagedView& c, uint32_t b) {
-  const int32_t n = __ldg(c.len + b);
+// Length of sequence b, in [0, max_len]; n is what the batch says.
+__device__ __forceinline__ int32_t paged_length(const PagedView& c, int32_t n) {
   if (n >= 0 && n <= c.max_len) return n;
   report_index(c.err);
   return n < 0 ? 0 : c.max_len;
 }
+__device__ __forceinline__ int32_t paged_len(const PagedView& c, uint32_t b) { return paged_length(c, __ldg(c.len + b)); }
 
 // Page of slot t (t in [0, max_len)) of sequence b, or -1 for a number outside the cache.
 __device__ __forceinline__ int32_t paged_page(const PagedView& c, uint32_t b, uint32_t t) {
@@ -47,14 +47,16 @@ __device__ __forceinline__ uint64_t paged_weight_at(const PagedView& c, int32_t 
   return (((uint64_t)page * c.n_kv + head) << c.shift) + (t & ((1u << c.shift) - 1));
 }
 
-// Rows [r0, r1) of sequence b, within [0, n_rows].
-__device__ __forceinline__ int2 paged_rows(const PagedView& c, uint32_t b) {
-  int32_t r0 = __ldg(c.start + b), r1 = __ldg(c.start + b + 1);
+// Rows [r0, r1) of a sequence, within [0, n_rows].
+__device__ __forceinline__ int2 paged_rows(const PagedView& c, int32_t r0, int32_t r1) {
   if (r0 < 0 || r1 < r0 || r1 > (int32_t)c.n_rows) {
     report_index(c.err);
     return make_int2(0, 0);
   }
   return make_int2(r0, r1);
+}
+__device__ __forceinline__ int2 paged_rows(const PagedView& c, uint32_t b) {
+  return paged_rows(c, __ldg(c.start + b), __ldg(c.start + b + 1));
 }
 
 // The sequence that owns row r: the last b with start[b] <= r. All lanes of the warp call
@@ -81,14 +83,17 @@ struct PagedMask {
   int32_t window;  // 0: none
   float scale, cap;
 };
-__device__ __forceinline__ int2 paged_keys(const PagedMask& m, uint32_t r, int32_t t, int32_t len) {
-  int32_t lo = m.first ? __ldg(m.first + r) : 0;
+__device__ __forceinline__ int2 paged_interval(const PagedMask& m, int32_t first, int32_t last, int32_t t, int32_t len) {
+  int32_t lo = first;
   if (m.window) lo = max(lo, t + 1 - m.window);
   lo = max(lo, 0);
   int32_t hi = t + 1;
-  if (m.last) hi = max(hi, __ldg(m.last + r));
+  if (m.last) hi = max(hi, last);
   hi = min(hi, len);
   return t >= 0 && lo < hi ? make_int2(lo, hi) : make_int2(0, 0);
+}
+__device__ __forceinline__ int2 paged_keys(const PagedMask& m, uint32_t r, int32_t t, int32_t len) {
+  return paged_interval(m, m.first ? __ldg(m.first + r) : 0, m.last ? __ldg(m.last + r) : 0, t, len);
 }
 
 template <typename T>

@@ -41,7 +41,7 @@ struct TileInfo {
 __device__ __forceinline__ TileInfo find_tile(const AttendArgs& a, uint32_t s, uint32_t lane) {
   const uint32_t per = 2 * a.toks;
   uint32_t lo = 0, hi = a.c.n_seqs;
-  while (hi - lo > 1) {
+  while (hi - lo > 32) {
     const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
     const bool le = at < hi && (at == lo || (uint32_t)__ldg(a.c.start + at) / per + at <= s);
     const uint32_t n = __popc(__ballot_sync(0xffffffffu, le));
@@ -49,15 +49,22 @@ __device__ __forceinline__ TileInfo find_tile(const AttendArgs& a, uint32_t s, u
     hi = min(hi, below + step);
     lo = below;
   }
+  // Of up to 32 sequences all that is needed is fetched at once.
+  const uint32_t at = min(lo + lane, hi - 1);
+  const int32_t from = __ldg(a.c.start + at), to = __ldg(a.c.start + at + 1), n_at = __ldg(a.c.len + at);
+  const bool le = lo + lane < hi && (lane == 0 || (uint32_t)from / per + at <= s);
+  const uint32_t pick = max(__popc(__ballot_sync(0xffffffffu, le)), 1) - 1;
+  lo += pick;
   TileInfo w{lo, 0, 0, 0, 0};
-  const int2 rr = paged_rows(a.c, lo);
+  const int2 rr = paged_rows(a.c, __shfl_sync(0xffffffffu, from, pick), __shfl_sync(0xffffffffu, to, pick));
+  const int32_t len = paged_length(a.c, __shfl_sync(0xffffffffu, n_at, pick));
   const uint32_t base = (uint32_t)rr.x / per + lo;
   if (s < base) return w;
   const uint32_t off = (s - base) * per;
   if (off >= (uint32_t)(rr.y - rr.x)) return w;
   w.row0 = rr.x + off;
   w.toks = min(per, (uint32_t)(rr.y - rr.x) - off);
-  w.len = paged_len(a.c, lo);
+  w.len = len;
   w.t0 = w.len - (rr.y - rr.x) + (int32_t)off;
   return w;
 }
@@ -146,15 +153,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   const uint32_t row = tid & 127, tok0 = row / a.group, head = kh * a.group + row % a.group;
   const uint32_t tok = tok0 + rank * a.toks;
   const bool mine = warp < kSoftWarps && tok0 < a.toks, valid = mine && tok < w.toks;
+  // The row's interval, and that of the same row of the other CTA: both walk the same tiles.
+  const uint32_t tok1 = tok0 + (rank ^ 1) * a.toks, most = w.toks ? w.toks - 1 : 0;
+  const uint32_t ra = w.row0 + min(tok, most), rb = w.row0 + min(tok1, most);
+  int32_t first0 = 0, first1 = 0, last0 = 0, last1 = 0;
+  if (a.m.first && warp < kSoftWarps) first0 = __ldg(a.m.first + ra), first1 = __ldg(a.m.first + rb);
+  if (a.m.last && warp < kSoftWarps) last0 = __ldg(a.m.last + ra), last1 = __ldg(a.m.last + rb);
   // Queries into shared memory, the sign of the scale folded in; the first of them are on their
   // way while the rows' keys are looked up, all of them while the first tiles come.
   // 16-byte pieces of a row; loads on their way at once
   constexpr uint32_t per = D / 8, batch = 8, batches = G::kQ / 16 / (batch * kSoftWarps * 32);
+  const uint32_t by_group = 65535 / a.group + 1;  // r * by_group >> 16 is r / group: r < 128, group <= 64
   uint4 x[batch];
   auto fetch_q = [&](uint32_t n) {
 #pragma unroll
     for (uint32_t i = 0; i < batch; i++) {
-      const uint32_t e = tid + (n * batch + i) * kSoftWarps * 32, r = e / per, u = e % per, t0 = r / a.group, t = t0 + rank * a.toks;
+      const uint32_t e = tid + (n * batch + i) * kSoftWarps * 32, r = e / per, u = e % per, t0 = r * by_group >> 16, t = t0 + rank * a.toks;
       x[i] = make_uint4(0, 0, 0, 0);
       if (t0 < a.toks && t < w.toks)
         x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (uint64_t)(w.row0 + t) * a.p.q_row +
@@ -163,12 +177,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   };
   if (warp < kSoftWarps) fetch_q(0);
   int2 keys = make_int2(0, 0);
-  if (valid) keys = paged_keys(a.m, w.row0 + tok, w.t0 + (int32_t)tok, w.len);
+  if (valid) keys = paged_interval(a.m, first0, last0, w.t0 + (int32_t)tok, w.len);
   if (warp < kSoftWarps / 2) {
-    // The same row of the other CTA too: both walk the same tiles.
-    const uint32_t tok1 = tok0 + (rank ^ 1) * a.toks;
     int2 k1 = make_int2(0, 0);
-    if (mine && tok1 < w.toks) k1 = paged_keys(a.m, w.row0 + tok1, w.t0 + (int32_t)tok1, w.len);
+    if (mine && tok1 < w.toks) k1 = paged_interval(a.m, first1, last1, w.t0 + (int32_t)tok1, w.len);
     const bool s0 = keys.x < keys.y, s1 = k1.x < k1.y;
     const int32_t lo0 = min(s0 ? keys.x : INT32_MAX, s1 ? k1.x : INT32_MAX), lo1 = max(s0 ? keys.x : 0, s1 ? k1.x : 0);
     const int32_t hi0 = min(s0 ? keys.y : INT32_MAX, s1 ? k1.y : INT32_MAX), hi1 = max(s0 ? keys.y : 0, s1 ? k1.y : 0);
