@@ -562,6 +562,7 @@ extern "C" int snl_paged_append(const snl_paged_cache* c, const snl_paged_batch*
   if (p->rot_dim && (!pos || !rope || p->n_pos == 0)) return fail(SNL_E_INVALID, w + ": null positions or rotary table");
   if (p->axes > SNL_ROPE_INTERLEAVED || p->pairs > SNL_ROPE_ADJACENT)
     return fail(SNL_E_INVALID, w + ": unknown rotary layout");
+  if (!(p->eps >= 0.f) || p->eps > 3e38f) return fail(SNL_E_INVALID, w + ": eps must be finite and not negative");
   if (p->axes == SNL_ROPE_SECTIONS &&
       (uint64_t)p->sections[0] + p->sections[1] + p->sections[2] != p->rot_dim / 2)
     return fail(SNL_E_INVALID, w + ": the sections must add up to rot_dim / 2");

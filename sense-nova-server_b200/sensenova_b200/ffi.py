@@ -219,10 +219,10 @@ SIGNATURES = {
     "snl_argmax": (i32, [vp, u32, u32, vp, vp]),
     "snl_argmax_noalloc": (i32, [vp, u32, u32, vp, vp]),
     "snl_rope_table": (i32, [C.c_double, u32, u32, vp, vp]),
-    "snl_paged_append": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedAppendP), *[vp] * 9]),
-    "snl_paged_attend": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedAttnP), *[vp] * 5, sz, vp]),
+    "snl_paged_append": (i32, [P(PagedCacheC), P(PagedBatchC), vp, *[vp] * 9]),
+    "snl_paged_attend": (i32, [P(PagedCacheC), P(PagedBatchC), vp, *[vp] * 5, sz, vp]),
     "snl_paged_attend_workspace": (sz, [P(PagedCacheC), P(PagedBatchC), u32]),
-    "snl_paged_weigh": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedAttnP), vp, vp, C.c_float, vp]),
+    "snl_paged_weigh": (i32, [P(PagedCacheC), P(PagedBatchC), vp, vp, vp, C.c_float, vp]),
     "snl_paged_evict": (i32, [P(PagedCacheC), P(PagedBatchC), P(PagedEvictP), vp, vp, vp, vp]),
     "snl_synth_quant": (i32, [u64, C.c_char_p, i32, sz, sz, vp, vp, vp]),
     "snl_synth_f32": (i32, [u64, C.c_char_p, u32, sz, C.c_float, C.c_float, vp, vp]),

@@ -10,16 +10,21 @@ is done. SnlError says what a call refuses; snl_device_error() what only the dev
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Any
 
 from . import ffi
-from .ffi import PagedAppendP, PagedAttnP, PagedBatchC, PagedCacheC, PagedEvictP, SnlError
+from .ffi import PagedBatchC, PagedCacheC, PagedEvictP, SnlError
 
 ONE, SECTIONS, INTERLEAVED = 0, 1, 2  # which axis of a position turns which pair
 HALVES, ADJACENT = 0, 1  # which elements form a pair
 _TYPES = {"float32": ffi.SNL_T_F32, "float16": ffi.SNL_T_F16, "bfloat16": ffi.SNL_T_BF16}
 _type_of: dict[Any, int] = {}
 _is_int: dict[Any, bool] = {}
+# snl_paged_append_p and snl_paged_attn_p, packed anew for each call: 0.15 us where a ctypes
+# structure of as many fields takes 1.4 us to make, most of what a small call costs here.
+_APPEND = struct.Struct("@9If8Q").pack
+_ATTN = struct.Struct("@3Q2I2f2I6Q").pack
 
 
 def _type(t) -> int:
@@ -111,7 +116,8 @@ class PagedCache:
         kp, k_row, k_head = self._rows(k, "k", batch, self.n_kv)
         vp, v_row, v_head = self._rows(v, "v", batch, self.n_kv)
         kind = k.dtype
-        _need(v.dtype == kind and (q is None or q.dtype == kind), "q, k and v must have one type")
+        if v.dtype != kind or (q is not None and q.dtype != kind):
+            _fail("q, k and v must have one type")
         qp = op = tp = rp = None
         heads = q_row = q_head = out_row = out_head = rot = n_pos = 0
         if q is not None:
@@ -126,20 +132,30 @@ class PagedCache:
             rp, tp = _floats(rope, "rope", n_pos, half, 2), _ints(pos, "pos", batch.n_rows, 4)
         if len(sections) != 3:
             _fail("sections must be the numbers of pairs of the three axes")
-        p = PagedAppendP(heads, _type(k), rot, axes, pairs, n_pos, tuple(sections), eps, q_row, q_head, k_row, k_head, v_row,
-                         v_head, out_row, out_head)
+        try:
+            p = _APPEND(heads, _type(k), rot, axes, pairs, n_pos, *sections, eps, q_row, q_head, k_row, k_head, v_row, v_head,
+                        out_row, out_head)
+        except struct.error as e:
+            _fail(f"append's numbers: {e}")
         rc = self.lib.snl_paged_append(self.ref, batch.ref, p, qp, kp, vp, _floats(q_norm, "q_norm", d),
                                        _floats(k_norm, "k_norm", d), tp, rp, op, stream)
         if rc:
             ffi.check(rc)
 
-    def _attn(self, batch: PagedBatch, q, scale, cap, window, slopes, first, last) -> tuple[PagedAttnP, int]:
-        heads = q.shape[1]
-        qp, q_row, q_head = self._rows(q, "q", batch, heads)
-        _need(_type(q) == self.type, "q must have the cache's type")
-        return PagedAttnP(_floats(slopes, "slopes", heads), None if first is None else _ints(first, "first", batch.n_rows),
-                          None if last is None else _ints(last, "last", batch.n_rows), heads, window,
-                          self.head_dim ** -0.5 if scale is None else scale, cap, 0, 0, q_row, q_head), qp
+    def _query(self, batch: PagedBatch, q) -> tuple[int, int, int]:
+        at = self._rows(q, "q", batch, q.shape[1])
+        if _type(q) != self.type:
+            _fail("q must have the cache's type")
+        return at
+
+    def _attn(self, batch: PagedBatch, heads, scale, cap, window, slopes, first, last, *types_and_strides: int) -> bytes:
+        """snl_paged_attn_p; types_and_strides: gate's and out's type, and q's, gate's and out's strides."""
+        try:
+            return _ATTN(_floats(slopes, "slopes", heads) or 0, 0 if first is None else _ints(first, "first", batch.n_rows),
+                         0 if last is None else _ints(last, "last", batch.n_rows), heads, window,
+                         self.head_dim ** -0.5 if scale is None else scale, cap, *types_and_strides)
+        except (struct.error, OverflowError) as e:
+            _fail(f"the attention's numbers: {e}")
 
     def attend_workspace(self, batch: PagedBatch, heads: int) -> int:
         """Bytes of scratch that attend needs for such a batch."""
@@ -151,15 +167,17 @@ class PagedCache:
         cache's type, out and gate like it in any type, lse [rows, heads] f32, work a
         contiguous tensor of scratch bytes. first, last [rows] int32 and slopes [heads] f32
         are the masks and the distance bias; scale is 1 / sqrt(d) unless given."""
-        p, qp = self._attn(batch, q, scale, cap, window, slopes, first, last)
-        op, p.out_row, p.out_head = self._rows(out, "out", batch, p.n_heads)
-        p.out_type = _type(out)
-        gp = None
+        heads = q.shape[1]
+        qp, q_row, q_head = self._query(batch, q)
+        op, out_row, out_head = self._rows(out, "out", batch, heads)
+        gp, gate_type, gate_row, gate_head = None, 0, 0, 0
         if gate is not None:
-            gp, p.gate_row, p.gate_head = self._rows(gate, "gate", batch, p.n_heads)
-            p.gate_type = _type(gate)
+            gp, gate_row, gate_head = self._rows(gate, "gate", batch, heads)
+            gate_type = _type(gate)
+        p = self._attn(batch, heads, scale, cap, window, slopes, first, last, gate_type, _type(out), q_row, q_head,
+                       gate_row, gate_head, out_row, out_head)
         rc = self.lib.snl_paged_attend(self.ref, batch.ref, p, qp, gp, op,
-                                       _floats(lse, "lse", batch.n_rows, p.n_heads), work.data_ptr(),
+                                       _floats(lse, "lse", batch.n_rows, heads), work.data_ptr(),
                                        work.numel() * work.element_size(), stream)
         if rc:
             ffi.check(rc)
@@ -168,9 +186,11 @@ class PagedCache:
               window: int = 0, slopes=None, first=None, last=None, stream: int = 0) -> None:
         """weight = decay * weight + what the rows' attention (with attend's lse) gave each
         slot, per KV head (snl_paged_weigh)."""
-        p, qp = self._attn(batch, q, scale, cap, window, slopes, first, last)
+        heads = q.shape[1]
+        qp, q_row, q_head = self._query(batch, q)
+        p = self._attn(batch, heads, scale, cap, window, slopes, first, last, 0, 0, q_row, q_head, 0, 0, 0, 0)
         rc = self.lib.snl_paged_weigh(self.ref, batch.ref, p, qp,
-                                      _floats(lse, "lse", batch.n_rows, p.n_heads), decay, stream)
+                                      _floats(lse, "lse", batch.n_rows, heads), decay, stream)
         if rc:
             ffi.check(rc)
 

@@ -136,3 +136,12 @@ def test_batch_and_cache_shapes(lib):
 def test_struct_sizes(lib):
     assert [C.sizeof(s) for s in (ffi.PagedCacheC, ffi.PagedBatchC, ffi.PagedAppendP, ffi.PagedAttnP, ffi.PagedEvictP)] == \
         [72, 40, 104, 96, 16]
+
+
+def test_numbers_that_no_field_holds(lib):
+    cache, batch, q = make()
+    for kw in (dict(window=-1), dict(window=1 << 32), dict(window=1.5), dict(scale=1e39), dict(cap="soft")):
+        refused("SNL_E_INVALID", "the attention's numbers|scale must be finite", attend, cache, batch, q, **kw)
+    new = torch.zeros(3, 2, 256)
+    for kw in (dict(axes=-1), dict(sections=(1 << 32, 0, 0)), dict(sections=(0, -1, 0)), dict(eps=1e39)):
+        refused("SNL_E_INVALID", "append's numbers|eps must be finite", cache.append, batch, None, new, new, None, **kw)
