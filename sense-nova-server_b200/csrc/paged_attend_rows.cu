@@ -24,6 +24,7 @@ struct RowArgs {
   float* part;      // [CTA][2][group][D], then the same of (max, sum): a CTA's first and last unfinished piece
   float2* part_ml;
   int2* span;       // [row][KV head]: first and last CTA
+  uint32_t cluster;  // CTAs of a row and KV head (attend_short_kernel)
 };
 
 // The keys of a row.
@@ -84,6 +85,27 @@ __device__ __forceinline__ void next_block(const RowArgs& A, Walk& w) {
   }
 }
 
+// One element of the output: x gated, and with the first of a head its log-sum-exp.
+__device__ __forceinline__ void put_element(const AttendArgs& a, uint32_t row, uint32_t head, uint32_t d, float x, float l, float zero) {
+  auto value = [](const void* p, uint64_t i, uint32_t type) {
+    return type == SNL_T_F32 ? static_cast<const float*>(p)[i]
+           : type == SNL_T_F16 ? __half2float(static_cast<const __half*>(p)[i])
+                               : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  };
+  if (a.gate && l != 0.f) x *= sigmoidf_(value(a.gate, (uint64_t)row * a.p.gate_row + (uint64_t)head * a.p.gate_head + d, a.p.gate_type));
+  const uint64_t to = (uint64_t)row * a.p.out_row + (uint64_t)head * a.p.out_head + d;
+  if (a.p.out_type == SNL_T_F32) static_cast<float*>(a.out)[to] = x;
+  else if (a.p.out_type == SNL_T_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(x);
+  if (a.lse && d == 0) a.lse[(uint64_t)row * a.p.n_heads + head] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
+}
+constexpr uint32_t kRowCluster = 8;  // at most
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+
 // The blocks of 64 keys of all (KV head, row) pairs form one line that is cut into equal
 // shares, one for each CTA: every SM reads the same number of bytes whatever the lengths are.
 // A row that ends inside its CTA is written at once; pieces of rows cut by a share's end are
@@ -93,18 +115,19 @@ __device__ __forceinline__ void next_block(const RowArgs& A, Walk& w) {
 //
 // Bound by memory: 16 tokens of 16 heads of 256 over up to 32768 keys 189 us (1.19 GB, 6.3
 // TB/s, 0.97 of a copy's rate; 243 with the tiles of attend_kernel), 64 of 32 heads of 128 over
-// up to 4096 keys with capped scores 82 us (5.5 TB/s; 113 with one CTA an SM). One token over
-// 517 keys takes two launches' latency, 13 us a call.
-template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
-    attend_rows_kernel(const __grid_constant__ RowArgs A, const __grid_constant__ CUtensorMap kmap,
-                       const __grid_constant__ CUtensorMap vmap) {
+// up to 4096 keys with capped scores 82 us (5.5 TB/s; 113 with one CTA an SM).
+//
+// CLUSTER: a cluster of 1 to 8 CTAs takes each (KV head, row) instead, an equal share of its
+// blocks each, and joins them through shared memory: one launch in place of two, for short rows.
+template <typename T, int D, bool CLUSTER>
+__device__ __forceinline__ void attend_rows(const RowArgs& A, const CUtensorMap& kmap, const CUtensorMap& vmap) {
   using G = RowGeo<D>;
   constexpr uint32_t NS = G::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t bars[kRowWarps][NS];
   __shared__ uint32_t scan_sh[kRowWarps], found_sh[2];
-  __shared__ float2 ml_sh[kRowWarps][8];
+  __shared__ float2 ml_sh[kRowWarps][8], own_ml[8];
+  float* mo = reinterpret_cast<float*>(smem + G::kRing);  // [warp][8 heads][D]
   const AttendArgs& a = A.a;
   pdl_trigger();
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -117,48 +140,63 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
   fence_mbar_init();
   pdl_wait();
 
-  // Blocks before each thread's rows, this CTA's share, and the row that it starts in.
-  const uint32_t per = (a.c.n_rows + kRowWarps * 32 - 1) / (kRowWarps * 32), r0 = min(tid * per, a.c.n_rows),
-                 r1 = min(r0 + per, a.c.n_rows);
-  uint32_t mine = 0;
-  for (uint32_t r = r0; r < r1; r++) mine += row_blocks(row_keys(a.c, a.m, r));
-  uint32_t upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= (uint32_t)o) upto += v;
-  }
-  if (lane == 31) scan_sh[warp] = upto;
-  __syncthreads();
-  uint32_t total = 0;
-  for (uint32_t i = 0; i < kRowWarps; i++) {
-    if (i < warp) upto += scan_sh[i];
-    total += scan_sh[i];
-  }
-  const uint64_t all = (uint64_t)total * a.c.n_kv, share = (all + gridDim.x - 1) / gridDim.x, g0 = blockIdx.x * share;
-  if (g0 >= all) return;
-  const uint64_t g1 = min(g0 + share, all);
-  {
-    uint32_t off = (uint32_t)(g0 % total);
-    if (off >= upto - mine && off < upto) {
-      off -= upto - mine;
-      uint32_t r = r0;
-      for (;; r++) {
-        const uint32_t n = row_blocks(row_keys(a.c, a.m, r));
-        if (off < n) break;
-        off -= n;
-      }
-      found_sh[0] = r;
-      found_sh[1] = off;
-    }
-  }
-  __syncthreads();
   Walk now;
-  now.left = g1 - g0;
-  now.kh = (uint32_t)(g0 / total);
-  now.row = found_sh[0];
-  enter_row(A, now);
-  now.blk = now.first + found_sh[1];
+  uint32_t total = 0;
+  uint64_t share = 0, g1 = 0;
+  if constexpr (CLUSTER) {
+    now.row = blockIdx.x / A.cluster / a.c.n_kv;
+    now.kh = blockIdx.x / A.cluster % a.c.n_kv;
+    enter_row(A, now);
+    const uint32_t n = now.end - now.first, part = blockIdx.x % A.cluster, from = (uint32_t)((uint64_t)n * part / A.cluster);
+    now.left = (uint32_t)((uint64_t)n * (part + 1) / A.cluster) - from;
+    now.blk = now.first + from;
+    for (uint32_t i = tid; i < a.group * D; i += kRowWarps * 32) mo[i] = 0.f;
+    if (tid < 8) own_ml[tid] = make_float2(-INFINITY, 0.f);
+    __syncthreads();
+  } else {
+    // Blocks before each thread's rows, this CTA's share, and the row that it starts in.
+    const uint32_t per = (a.c.n_rows + kRowWarps * 32 - 1) / (kRowWarps * 32), r0 = min(tid * per, a.c.n_rows),
+                   r1 = min(r0 + per, a.c.n_rows);
+    uint32_t mine = 0;
+    for (uint32_t r = r0; r < r1; r++) mine += row_blocks(row_keys(a.c, a.m, r));
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= (uint32_t)o) upto += v;
+    }
+    if (lane == 31) scan_sh[warp] = upto;
+    __syncthreads();
+    for (uint32_t i = 0; i < kRowWarps; i++) {
+      if (i < warp) upto += scan_sh[i];
+      total += scan_sh[i];
+    }
+    const uint64_t all = (uint64_t)total * a.c.n_kv;
+    share = (all + gridDim.x - 1) / gridDim.x;
+    const uint64_t g0 = blockIdx.x * share;
+    if (g0 >= all) return;
+    g1 = min(g0 + share, all);
+    {
+      uint32_t off = (uint32_t)(g0 % total);
+      if (off >= upto - mine && off < upto) {
+        off -= upto - mine;
+        uint32_t r = r0;
+        for (;; r++) {
+          const uint32_t n = row_blocks(row_keys(a.c, a.m, r));
+          if (off < n) break;
+          off -= n;
+        }
+        found_sh[0] = r;
+        found_sh[1] = off;
+      }
+    }
+    __syncthreads();
+    now.left = g1 - g0;
+    now.kh = (uint32_t)(g0 / total);
+    now.row = found_sh[0];
+    enter_row(A, now);
+    now.blk = now.first + found_sh[1];
+  }
   Walk ahead = now;  // of the loads
 
   const uint32_t ring = smem_u32(smem) + warp * NS * G::kStage;
@@ -290,7 +328,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
     fresh = true;
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    float* mo = reinterpret_cast<float*>(smem + G::kRing);
 #pragma unroll
     for (int c = 0; c < D / 16; c++) {  // column 2t, 2t + 1: heads; row g, g + 8: elements
       float* at = mo + (warp * 8 + 2 * t) * D + 16 * c + g;
@@ -299,12 +336,16 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
     }
     if (t == 0) ml_sh[warp][g] = make_float2(m_run, l_run);
     __syncthreads();
-    const uint64_t g_row = g1 - was.left + 1 - (was.blk - was.first + 1);  // the line's block where the row starts
-    const uint64_t n_row = was.end - was.first;
-    const uint64_t c_first = g_row / share, c_last = (g_row + n_row - 1) / share;
-    const bool whole = c_first == c_last;
-    if (c_first == blockIdx.x && tid == 0)
-      A.span[(uint64_t)was.row * a.c.n_kv + was.kh] = make_int2((int)c_first, (int)c_last);
+    uint64_t c_first = 0;
+    bool whole = false;
+    if constexpr (!CLUSTER) {
+      const uint64_t g_row = g1 - was.left + 1 - (was.blk - was.first + 1);  // the line's block where the row starts
+      const uint64_t n_row = was.end - was.first, c_last = (g_row + n_row - 1) / share;
+      c_first = g_row / share;
+      whole = c_first == c_last;
+      if (c_first == blockIdx.x && tid == 0)
+        A.span[(uint64_t)was.row * a.c.n_kv + was.kh] = make_int2((int)c_first, (int)c_last);
+    }
     for (uint32_t h = tid / D; h < a.group; h += kRowWarps * 32 / D) {
       const uint32_t d = tid % D;
       float top = -INFINITY, l = 0.f, x = 0.f;
@@ -319,26 +360,18 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
         l = fmaf(ml.y, f, l);
         x = fmaf(mo[(i * 8 + h) * D + d], f, x);
       }
-      const uint32_t hq = was.kh * a.group + h;
+      if constexpr (CLUSTER) {
+        mo[h * D + d] = x;  // this thread alone read it
+        if (d == 0) own_ml[h] = make_float2(top, l);
+        continue;
+      }
       if (!whole) {
         const uint64_t at = ((uint64_t)blockIdx.x * 2 + (c_first == blockIdx.x ? 1 : 0)) * a.group + h;
         A.part[at * D + d] = x;
         if (d == 0) A.part_ml[at] = make_float2(top, l);
         continue;
       }
-      x = l == 0.f ? 0.f : x / l;
-      auto value = [](const void* p, uint64_t i, uint32_t type) {
-        return type == SNL_T_F32 ? static_cast<const float*>(p)[i]
-               : type == SNL_T_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                                   : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-      };
-      if (a.gate) x *= sigmoidf_(value(a.gate, (uint64_t)was.row * a.p.gate_row + (uint64_t)hq * a.p.gate_head + d, a.p.gate_type));
-      const uint64_t to = (uint64_t)was.row * a.p.out_row + (uint64_t)hq * a.p.out_head + d;
-      if (a.p.out_type == SNL_T_F32) static_cast<float*>(a.out)[to] = x;
-      else if (a.p.out_type == SNL_T_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(x);
-      else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(x);
-      if (a.lse && d == 0)
-        a.lse[(uint64_t)was.row * a.p.n_heads + hq] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
+      put_element(a, was.row, was.kh * a.group + h, d, l == 0.f ? 0.f : x / l, l, zero);
     }
     __syncthreads();
   }
@@ -347,6 +380,48 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
     if (lane == 0) report_timeout(a.c.err);
     for (uint32_t i = issued > NS ? issued - NS : 0; i < issued; i++) (void)wait_mbar(&bars[warp][i % NS], (i / NS) & 1);
   }
+  if constexpr (CLUSTER) {  // each CTA joins its part of the row's elements
+    cluster_sync();
+    const uint32_t n = a.group * D / A.cluster, part = blockIdx.x % A.cluster;
+    for (uint32_t i = part * n + tid; i < (part + 1) * n; i += kRowWarps * 32) {
+      float2 ml[kRowCluster];
+      float x[kRowCluster], top = -INFINITY;
+#pragma unroll
+      for (uint32_t r = 0; r < kRowCluster; r++) {
+        ml[r] = make_float2(-INFINITY, 0.f);
+        x[r] = 0.f;
+        if (r >= A.cluster) continue;
+        ml[r].x = ld_cluster(in_cta(&own_ml[i / D].x, r));
+        ml[r].y = ld_cluster(in_cta(&own_ml[i / D].y, r));
+        x[r] = ld_cluster(in_cta(&mo[i], r));
+        top = fmaxf(top, ml[r].x);
+      }
+      const float zero = top == -INFINITY ? 0.f : top;
+      float l = 0.f, sum = 0.f;
+#pragma unroll
+      for (uint32_t r = 0; r < kRowCluster; r++) {
+        if (ml[r].y == 0.f) continue;
+        const float f = ml[r].x == -INFINITY ? 1.f : ex2(ml[r].x - zero);
+        l = fmaf(ml[r].y, f, l);
+        sum = fmaf(x[r], f, sum);
+      }
+      put_element(a, now.row, now.kh * a.group + i / D, i % D, l == 0.f ? 0.f : sum / l, l, zero);
+    }
+    cluster_sync();  // no CTA ends while another reads its memory
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
+    attend_rows_kernel(const __grid_constant__ RowArgs A, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+  attend_rows<T, D, false>(A, kmap, vmap);
+}
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32, RowGeo<D>::kPerSm)
+    attend_short_kernel(const __grid_constant__ RowArgs A, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap) {
+  attend_rows<T, D, true>(A, kmap, vmap);
 }
 
 // Joins the pieces of rows that lie in several shares, and writes rows without keys. One warp
@@ -409,11 +484,46 @@ int go_rows(const snl_paged_cache& c, const RowArgs& r, uint32_t grid, cudaStrea
   SNL_TRY(page_map(&km, c, c.k, 8, D / 64));
   SNL_TRY(page_map(&vm, c, c.v, 8, D / 64));
   static bool attr[64] = {};
+  static int room[64][4] = {};  // clusters of 1, 2, 4 and 8 CTAs that the GPU runs at once
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !attr[dev]) {
+  if (dev < 0 || dev >= 64) return fail(SNL_E_UNSUPPORTED, "snl_paged_attend: device number");
+  if (!attr[dev]) {
     SNL_CUDA_TRY(cudaFuncSetAttribute(attend_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowGeo<D>::kSmem));
-    if (dev >= 0 && dev < 64) attr[dev] = true;
+    SNL_CUDA_TRY(cudaFuncSetAttribute(attend_short_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowGeo<D>::kSmem));
+    for (uint32_t i = 0; i < 4; i++) {
+      cudaLaunchAttribute at{};
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim.x = 1u << i;
+      at.val.clusterDim.y = at.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(1u << i);
+      cfg.blockDim = dim3(kRowWarps * 32);
+      cfg.dynamicSmemBytes = RowGeo<D>::kSmem;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      SNL_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, attend_short_kernel<T, D>, &cfg));
+      room[dev][i] = n;
+    }
+    attr[dev] = true;
+  }
+  // The largest clusters of which one wave holds all rows, up to 512 keys for each CTA. Against
+  // equal shares, one to 16 rows of one length, and of lengths from an eighth of the longest up: up
+  // to 512 keys a CTA all gain (head_dim 256: 1 row of 517 keys 12.0 -> 8.5 us, of 4096 18.5 -> 15.0; 8 of
+  // 1024 14.9 -> 11.4; 16 of up to 1024 19.0 -> 15.4), with 1024 uneven rows lose (8 of up to 8192 29 -> 40).
+  constexpr uint32_t kShortKeys = 512;
+  const uint64_t pairs = (uint64_t)r.a.c.n_rows * c.n_kv;
+  int i = 3;
+  while (i >= 0 && pairs > (uint64_t)room[dev][i]) i--;
+  if (i >= 0 && (uint32_t)r.a.c.max_len <= kShortKeys << i) {
+    RowArgs brief = r;
+    brief.cluster = 1u << i;
+    const cudaError_t e = launch_pdl_clusters(attend_short_kernel<T, D>, brief.cluster, dim3((unsigned)pairs * brief.cluster),
+                                              dim3(kRowWarps * 32), (size_t)RowGeo<D>::kSmem, s, brief, km, vm);
+    if (e != cudaSuccess) return cuda_fail(e, "attend_short_kernel");
+    count_launch();
+    return SNL_OK;
   }
   SNL_PDL_LAUNCH("attend_rows_kernel", (attend_rows_kernel<T, D>), dim3(grid), dim3(kRowWarps * 32), (size_t)RowGeo<D>::kSmem, s,
                  r, km, vm);

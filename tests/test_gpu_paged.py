@@ -649,3 +649,31 @@ def test_serving_example(lib, capsys):
     parts = torch.cat([b.step([s], [x[i:j]]) for i, j in ((0, 150), (150, 151), (151, 200))])
     # values of order 1; the projections' rows come from two kernels (1e-4), attention rounds to 2^-11
     assert (whole - parts).abs().max() < 5e-3 * whole.abs().max()
+
+
+# A batch for far longer sequences: single rows go by equal shares of all blocks instead of a cluster each.
+WIDE = dict(width=20000 // 8, max_len=20000)
+
+
+@pytest.mark.parametrize("heads,kv,d,page,layout,dtype", [s for s in SHAPES if s[0] // s[1] <= 8])
+@pytest.mark.parametrize("lens", [[1], [129], [7, 300, 64, 1], [600, 0, 63, 64, 65, 8, 9] * 3])
+def test_attend_one_row_by_equal_shares(heads, kv, d, page, layout, dtype, lens):
+    check_attend(Problem(lens, [min(n, 1) for n in lens], heads, kv, d, page, layout, dtype, seed=len(lens), **WIDE))
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("by_shares", [False, True])
+def test_attend_one_row_masks(mask, d, by_shares):
+    p = Problem([300, 150, 77, 2000], [1, 1, 1, 1], 8, 2, d, 16, seed=d, **(WIDE if by_shares else {}))
+    gate = torch.randn(p.n, p.heads, p.d, device="cuda", generator=torch.Generator("cuda").manual_seed(d))
+    check_attend(p, gate=gate, out_dtype=F32, **masks_of(p, **MASKS[mask]))
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 7, 9, 18, 37, 75, 150])
+@pytest.mark.parametrize("heads,d", [(8, 256), (32, 128)])
+def test_attend_one_row_clusters(n, heads, d):
+    """Clusters of 8, 4, 2 and 1 CTAs, and more rows than one wave holds."""
+    p = Problem([(17 * i) % 480 + 1 for i in range(n)], [1] * n, heads, heads // 4, d, 16, seed=n)
+    check_attend(p)
+    assert all(torch.equal(a, b) for a, b in zip(run_attend(p), run_attend(p)))
