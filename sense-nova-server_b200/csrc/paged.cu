@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <string>
 
-#include "paged.cuh"
+#include "paged_tc.cuh"
 
 namespace snl {
 namespace {
@@ -212,7 +212,7 @@ struct EvictArgs {
   int32_t* kept;
   const int32_t* into;
   int32_t* new_len;
-  uint32_t head_dim;
+  uint32_t head_dim, cluster;  // CTAs that select from one list
 };
 
 // Order-preserving map of a weight to an unsigned key: NaN as -inf, -0 as +0.
@@ -248,26 +248,29 @@ __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* sh, uint32
   return s - v + (warp ? before : 0);
 }
 
-// One CTA per (KV head, sequence): the n-th largest key of the candidates by four 8-bit radix
+// One CTA, or a cluster of them, per (KV head, sequence): the n-th largest key of the candidates by four 8-bit radix
 // passes (weights crowd in few exponents: eight counts of each digit, by lane, on banks of
 // their own), then the kept slots in slot order, 4096 at a time. A thread takes four
 // neighbouring slots, which lie in one page. The weights are read once where their keys fit
 // shared memory. 32 lists of up to 16384 weights take 22 us, the copy of their 4096 kept slots
 // 43 us (269 MB in all).
-template <bool HELD>
+template <bool HELD, bool MANY>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t held[];
-  __shared__ uint32_t hist[8][260], warp_n[32], s_digit, s_need;
+  __shared__ uint32_t hist[8][260], sums[2][256], warp_n[32], s_digit, s_need, own_n[2];
   pdl_trigger();
+  const uint32_t cs = MANY ? a.cluster : 1, part = blockIdx.x % cs, kh = blockIdx.x / cs, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  if (tid < 2) own_n[tid] = 0;
+  if (tid == 0) s_digit = s_need = 0;
   pdl_wait();
-  const uint32_t kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
   const int32_t len = paged_len(a.c, b), budget = (int32_t)a.p.budget;
   int32_t* kept = a.kept + ((uint64_t)b * a.c.n_kv + kh) * a.p.budget;
   if (len <= budget) {
-    for (int32_t i = tid; i < budget; i += kSelectThreads) kept[i] = i < len ? i : -1;
+    for (int32_t i = part * kSelectThreads + tid; i < budget; i += cs * kSelectThreads) kept[i] = i < len ? i : -1;
     return;
   }
   const int32_t t0 = (int32_t)a.p.sink, t1 = len - (int32_t)a.p.recent;  // the candidates
+  const int32_t own = (int32_t)(((uint32_t)len + 4 * cs - 1) / (4 * cs)) * 4, from = (int32_t)part * own, end = min(len, from + own);  // this CTA's slots
   // Keys of slots t to t + 3 (t a multiple of 4): 0 for what is no candidate, which no weight maps to.
   auto fetch = [&](int32_t t) -> uint4 {
     uint4 k = make_uint4(0, 0, 0, 0);
@@ -281,17 +284,17 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
     if (t + 3 >= t0 && t + 3 < t1) k.w = weight_key(w.w);
     return k;
   };
-  auto keys_at = [&](int32_t t) -> uint4 { return HELD ? *reinterpret_cast<const uint4*>(held + t) : fetch(t); };
+  auto keys_at = [&](int32_t t) -> uint4 { return HELD ? *reinterpret_cast<const uint4*>(held + (t - from)) : fetch(t); };
   const uint32_t take = a.p.budget - a.p.sink - a.p.recent;
   uint32_t cut = 0, need = take;  // the keys' common prefix so far, and how many of it are taken
   for (int shift = 24; take && shift >= 0; shift -= 8) {
     for (uint32_t i = tid; i < 8 * 260; i += kSelectThreads) hist[0][i] = 0;
     __syncthreads();
-    for (int32_t base = 0; base < len; base += kSelectKeys) {
+    for (int32_t base = from; base < end; base += kSelectKeys) {
       const int32_t t = base + 4 * (int32_t)tid;
       uint4 k = make_uint4(0, 0, 0, 0);
-      if (t < len) {
-        if (HELD && shift == 24) *reinterpret_cast<uint4*>(held + t) = k = fetch(t);
+      if (t < end) {
+        if (HELD && shift == 24) *reinterpret_cast<uint4*>(held + (t - from)) = k = fetch(t);
         else k = keys_at(t);
       }
       const uint32_t ks[4] = {k.x, k.y, k.z, k.w};
@@ -305,7 +308,15 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
       uint32_t s = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) s += hist[i][tid];
-      hist[0][tid] = s;
+      (MANY ? sums[(shift >> 3) & 1] : hist[0])[tid] = s;
+    }
+    if constexpr (MANY) {  // over the cluster; the next pass writes the other sums, so one meeting a pass
+      cluster_sync();
+      if (tid < 256) {
+        uint32_t s = 0;
+        for (uint32_t r = 0; r < cs; r++) s += ld_cluster_u32(in_cta(&sums[(shift >> 3) & 1][tid], r));
+        hist[0][tid] = s;
+      }
     }
     __syncthreads();
     if (tid < 32) {  // the digit at which the sum from the top reaches `need`: 8 digits a lane
@@ -336,14 +347,38 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   }
   // Kept: what must be, what lies above the cut, and of its equals the first `need`.
   uint32_t sure = 0, ties = 0;  // before this stretch
-  for (int32_t base = 0; base < len; base += kSelectKeys) {
+  if constexpr (MANY) {
+    for (int32_t t = from + 4 * (int32_t)tid; t < end; t += kSelectKeys) {
+      const uint4 k = take ? keys_at(t) : make_uint4(0, 0, 0, 0);
+      const uint32_t ks[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const bool must = t + e < len && (t + e < t0 || t + e >= t1), is_sure = must || (take && ks[e] > cut);
+        sure += is_sure;
+        ties += !is_sure && take && ks[e] == cut;
+      }
+    }
+    sure = __reduce_add_sync(0xffffffffu, sure);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) {
+      atomicAdd(&own_n[0], sure);
+      atomicAdd(&own_n[1], ties);
+    }
+    cluster_sync();
+    sure = ties = 0;
+    for (uint32_t r = 0; r < part; r++) {
+      sure += ld_cluster_u32(in_cta(&own_n[0], r));
+      ties += ld_cluster_u32(in_cta(&own_n[1], r));
+    }
+  }
+  for (int32_t base = from; base < end; base += kSelectKeys) {
     const int32_t t = base + 4 * (int32_t)tid;
-    const uint4 k = take && t < len ? keys_at(t) : make_uint4(0, 0, 0, 0);
+    const uint4 k = take && t < end ? keys_at(t) : make_uint4(0, 0, 0, 0);
     const uint32_t ks[4] = {k.x, k.y, k.z, k.w};
     uint32_t mine = 0;  // sure ones, ties << 16
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const bool must = t + e < len && (t + e < t0 || t + e >= t1);
+      const bool must = t < end && t + e < len && (t + e < t0 || t + e >= t1);
       mine += must || (take && ks[e] > cut) ? 1u : take && ks[e] == cut ? 1u << 16 : 0u;
     }
     uint32_t all;
@@ -351,7 +386,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
     uint32_t s = sure + (before & 0xFFFF), q = ties + (before >> 16);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const bool must = t + e < len && (t + e < t0 || t + e >= t1);
+      const bool must = t < end && t + e < len && (t + e < t0 || t + e >= t1);
       const bool is_sure = must || (take && ks[e] > cut), tie = !is_sure && take && ks[e] == cut;
       const uint32_t at = s + min(q, need);
       if ((is_sure || (tie && q < need)) && at < a.p.budget) kept[at] = t + e;
@@ -361,6 +396,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
     sure += all & 0xFFFF;
     ties += all >> 16;
   }
+  if constexpr (MANY) cluster_sync();  // no CTA ends while another reads its counts
 }
 
 constexpr uint32_t kMoveThreads = 256, kMoveRows = 8 * 32;  // rows of one step: 8 per group of 8 threads
@@ -634,21 +670,30 @@ extern "C" int snl_paged_evict(const snl_paged_cache* c, const snl_paged_batch* 
   a.head_dim = c->head_dim;
   SNL_TRY(paged_error_word(&a.c.err));
   const cudaStream_t s = (cudaStream_t)stream;
-  const dim3 sel(c->n_kv, b->n_seqs);
-  if ((uint32_t)a.c.max_len <= kSelectHeld) {
-    static bool attr[64] = {};
+  // CTAs of a list: 4096 slots for each, and no more CTAs than the SMs hold, two each (32 lists of
+  // 16384 slots, with the copy of 1024: 28 us with one, 24 with 2, 21 with 4, 23 with 8; of 65536
+  // 90, 40, 37, 32; 128 lists of 16384 48, 43, 53, 86).
+  const uint64_t lists = (uint64_t)c->n_kv * b->n_seqs;
+  a.cluster = 8;
+  while (a.cluster > 1 && ((uint32_t)a.c.max_len < 4096 * a.cluster || lists * a.cluster > 2ull * sm_count())) a.cluster /= 2;
+  const dim3 sel(c->n_kv * a.cluster, b->n_seqs);
+  const uint32_t own = (uint32_t)(((uint64_t)a.c.max_len + 4 * a.cluster - 1) / (4 * a.cluster)) * 4;
+  auto select = [&](auto kern, bool held, bool* done) -> int {
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !attr[dev]) {
-      SNL_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kSelectHeld * sizeof(uint32_t))));
-      if (dev >= 0 && dev < 64) attr[dev] = true;
+    if (held && (dev < 0 || dev >= 64 || !done[dev])) {
+      SNL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSelectHeld * sizeof(uint32_t))));
+      if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    const size_t smem = ((size_t)a.c.max_len + 3) / 4 * 16;
-    SNL_PDL_LAUNCH("evict_select_kernel", evict_select_kernel<true>, sel, dim3(kSelectThreads), smem, s, a);
-  } else {
-    SNL_PDL_LAUNCH("evict_select_kernel", evict_select_kernel<false>, sel, dim3(kSelectThreads), (size_t)0, s, a);
-  }
+    const cudaError_t e = launch_pdl_clusters(kern, a.cluster, sel, dim3(kSelectThreads), held ? own * sizeof(uint32_t) : 0, s, a);
+    if (e != cudaSuccess) return cuda_fail(e, "evict_select_kernel");
+    count_launch();
+    return SNL_OK;
+  };
+  static bool attr[2][64] = {};
+  const bool many = a.cluster > 1;
+  if (own <= kSelectHeld) SNL_TRY(many ? select(evict_select_kernel<true, true>, true, attr[1]) : select(evict_select_kernel<true, false>, true, attr[0]));
+  else SNL_TRY(many ? select(evict_select_kernel<false, true>, false, nullptr) : select(evict_select_kernel<false, false>, false, nullptr));
   if (!into) {
     SNL_PDL_LAUNCH("evict_shift_kernel", evict_shift_kernel, dim3(2 * (c->head_dim * 2 / 128) + 1, c->n_kv, b->n_seqs),
                    dim3(kMoveThreads), (size_t)0, s, a);

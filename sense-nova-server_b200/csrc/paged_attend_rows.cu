@@ -100,11 +100,7 @@ __device__ __forceinline__ void put_element(const AttendArgs& a, uint32_t row, u
   if (a.lse && d == 0) a.lse[(uint64_t)row * a.p.n_heads + head] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
 }
 constexpr uint32_t kRowCluster = 8;  // at most
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float x;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
-  return x;
-}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) { return __uint_as_float(ld_cluster_u32(addr)); }
 
 // The blocks of 64 keys of all (KV head, row) pairs form one line that is cut into equal
 // shares, one for each CTA: every SM reads the same number of bytes whatever the lengths are.

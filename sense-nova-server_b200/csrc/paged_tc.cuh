@@ -156,6 +156,12 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity) {
     if (clock64() - t0 > (1ll << 28)) return false;
   return true;
 }
+// A variable of the CTA whose address in_cta() gave.
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t x;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+  return x;
+}
 // Boxes into this CTA, counted on a barrier that may be the other CTA's: slots of a page, or
 // one chunk of the queries of some tokens.
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int slot, int chunk, int head, int page,

@@ -677,3 +677,22 @@ def test_attend_one_row_clusters(n, heads, d):
     p = Problem([(17 * i) % 480 + 1 for i in range(n)], [1] * n, heads, heads // 4, d, 16, seed=n)
     check_attend(p)
     assert all(torch.equal(a, b) for a, b in zip(run_attend(p), run_attend(p)))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,budget,sink,recent", [
+    ([8192, 8191, 700], 300, 4, 32), ([16384, 16389, 4096, 1], 5000, 0, 0), ([33000], 20000, 20000, 0),
+    ([40001], 7, 3, 4), ([16400], 16399, 5, 9000),
+])
+def test_evict_by_clusters(lens, budget, sink, recent, in_place):
+    """Lists long enough for 2, 4 or 8 CTAs; few distinct weights, so that equal ones lie in all of them."""
+    p = Problem(lens, [min(n, 1) for n in lens], 4, 2, 128, 16, seed=budget, weight=True,
+                spare=len(lens) * -(-min(budget, max(lens)) // 16))
+    p.weight.copy_((p.weight * 50).floor())
+    check_evict(p, budget, sink, recent, in_place)
+
+
+def test_evict_very_long():
+    """More candidates than the shared memory of eight CTAs holds keys of."""
+    p = Problem([400000], [1], 1, 1, 128, 256, seed=29, weight=True, spare=20)
+    check_evict(p, 5000, 4, 64, False)
