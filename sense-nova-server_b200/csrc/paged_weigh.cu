@@ -167,10 +167,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
   for (uint32_t s = 0; s < NS; s++) issue();
 
   const uint32_t g = lane >> 2, t = lane & 3;
-  const float cap = a.m.cap;
+  const float cap = a.m.cap, sl = a.m.scale * kLog2e, pre = cap > 0.f ? a.m.scale / cap : 0.f;
   bool ok = true, fresh = true;
   uint32_t q[D / 16][4];
-  float z[2] = {0.f, 0.f}, slope = 0.f;
+  float z[2], slope = 0.f;
+  int2 keys[2];    // what a row sees, of its keys from the lane's first key of block 0 on
+  float gap[2];    // from that key to the row's own slot
   auto load_rows = [&](int32_t r0) {  // rows r0 and r0 + 1: this lane's head g of each
     const uint32_t head = now.kh * a.group + g;
 #pragma unroll
@@ -183,8 +185,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
         q[c][2 + e] = there ? *reinterpret_cast<const uint32_t*>(s + 16 * c + 8) : 0;
       }
       z[e] = there ? log2_sum(__ldg(a.lse + (uint64_t)(r0 + e) * a.p.n_heads + head)) : INFINITY;
+      const int32_t pos = now.len - (now.rows.y - (r0 + e)), k0 = (int32_t)(warp * 8 + 2 * t);
+      keys[e] = there ? paged_keys(a.m, r0 + e, pos, now.len) : make_int2(0, 0);
+      keys[e].x -= k0, keys[e].y -= k0;
+      gap[e] = (float)(pos - k0);
     }
-    slope = a.m.slopes && g < a.group ? __ldg(a.m.slopes + head) : 0.f;
+    slope = a.m.slopes && g < a.group ? __ldg(a.m.slopes + head) * kLog2e : 0.f;
   };
   while (now.left) {
     if (fresh) load_rows(now.rows.x);
@@ -213,14 +219,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
           }
 #pragma unroll
           for (int e = 0; e < 4; e++) {  // row r0 + e / 2, key + e % 2
-            const int32_t r = r0 + e / 2, k = key + e % 2, pos = now.len - (now.rows.y - r);
-            if (r >= now.rows.y || g >= a.group) continue;
-            const int2 keys = paged_keys(a.m, r, pos, now.len);
-            if (k < keys.x || k >= keys.y) continue;
-            float s = (s0[e] + s1[e]) * a.m.scale;
-            if (cap > 0.f) s = cap * tanh_(s / cap);
-            if (a.m.slopes) s -= slope * fabsf((float)(pos - k));
-            const float p = ex2(fmaf(s, kLog2e, -z[e / 2]));
+            const int32_t k = (int32_t)(now.blk * kBlock) + e % 2;
+            const float s = s0[e] + s1[e];
+            float x = cap > 0.f ? fmaf(cap * kLog2e, tanh_(s * pre), -z[e / 2]) : fmaf(s, sl, -z[e / 2]);
+            if (a.m.slopes) x = fmaf(-slope, fabsf(gap[e / 2] - (float)k), x);
+            const float p = k >= keys[e / 2].x && k < keys[e / 2].y ? ex2(x) : 0.f;
             if (e % 2) sum1 += p;
             else sum0 += p;
           }
