@@ -77,6 +77,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
   constexpr uint32_t NS = G::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t bars[kRowWarps][NS];
+  __shared__ __align__(16) float old_sh[kRowWarps][NS][8];  // the weights of a stage's keys, and their page
+  __shared__ int32_t page_sh[kRowWarps][NS];
   __shared__ uint32_t scan_sh[kRowWarps], found_sh[2];
   pdl_trigger();
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -154,7 +156,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
         const int32_t page = __shfl_sync(0xffffffffu, pages, ahead.blk - base);
         if (lane == 0) {
           const uint32_t st = issued % NS;
-          mbar_arrive_expect_tx(&bars[warp][st], G::kStage);
+          const bool old = page >= 0 && a.decay != 0.f;
+          page_sh[warp][st] = page;
+          mbar_arrive_expect_tx(&bars[warp][st], G::kStage + (old ? 32 : 0));
+          if (old)
+            bulk_g2s_plain(old_sh[warp][st], a.c.weight + paged_weight_at(a.c, page, ahead.kh, ahead.blk * kBlock + warp * 8), 32,
+                           &bars[warp][st]);
           tma_group(ring + st * G::kStage, &kmap, (int)((ahead.blk * kBlock + warp * 8) & ((1u << a.c.shift) - 1)),
                     (int)ahead.kh, page < 0 ? (int)a.c.n_pages : page, &bars[warp][st]);
         }
@@ -197,16 +204,20 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
     fresh = false;
     const int32_t key0 = (int32_t)(now.blk * kBlock + warp * 8), key = key0 + 2 * (int32_t)t;
     if (key0 < now.len) {
-      // The old weights of the lane's two keys come beside the scores.
-      const int32_t old_len = now.len - (now.rows.y - now.rows.x), page = paged_page(a.c, now.b, key0);
-      float2* at = reinterpret_cast<float2*>(a.c.weight + paged_weight_at(a.c, max(page, 0), now.kh, key));
+      // The old weights of the lane's two keys come with the keys, or alone where no row sees them.
+      const int32_t old_len = now.len - (now.rows.y - now.rows.x);
+      const bool seen = active(now);
+      int32_t page = seen ? 0 : paged_page(a.c, now.b, key0);
       float2 w = make_float2(0.f, 0.f);
-      if (g == 0 && page >= 0) w = *at;
+      auto slot = [&] { return reinterpret_cast<float2*>(a.c.weight + paged_weight_at(a.c, page, now.kh, key)); };
+      if (!seen && g == 0 && page >= 0) w = *slot();
       float sum0 = 0.f, sum1 = 0.f;
-      if (active(now)) {
+      if (seen) {
         const uint32_t st = taken % NS, box = ring + st * G::kStage;
         ok = __all_sync(0xffffffffu, ok && wait_mbar(&bars[warp][st], (taken / NS) & 1));
         taken++;
+        w = *reinterpret_cast<const float2*>(&old_sh[warp][st][2 * t]);
+        page = page_sh[warp][st];
         for (int32_t r0 = now.rows.x; r0 < now.rows.y; r0 += 2) {
           if (now.rows.y - now.rows.x > 2) load_rows(r0);  // a sequence of more rows than most
           float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -240,8 +251,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
       if (g == 0 && page >= 0) {
         w.x = a.decay != 0.f && key < old_len ? fmaf(w.x, a.decay, sum0) : sum0;
         w.y = a.decay != 0.f && key + 1 < old_len ? fmaf(w.y, a.decay, sum1) : sum1;
-        if (key + 1 < now.len) *at = w;
-        else if (key < now.len) at->x = w.x;
+        if (key + 1 < now.len) *slot() = w;
+        else if (key < now.len) slot()->x = w.x;
       }
     }
     const uint32_t b = now.b, kh = now.kh;
