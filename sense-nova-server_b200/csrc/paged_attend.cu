@@ -353,10 +353,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
         tm_wait_ld<NC>(r);
         if constexpr (GENERAL) {
           const float gap = (float)(w.t0 + (int32_t)tok - k0);
+          if (cap > 0.f) {  // mostly all scores are far below the cap, and need no exponentials
+            float most = 0.f;
 #pragma unroll
-          for (uint32_t c = 0; c < NC; c++) {
-            const float x = cap > 0.f ? cap * kLog2e * tanh_(s[c] * pre) : s[c] * sl;
-            s[c] = fmaf(-slope, fabsf(gap - (float)c), x);
+            for (uint32_t c = 0; c < NC; c++) most = fmaxf(most, fabsf(s[c]));
+            if (__any_sync(0xffffffffu, most * pre >= kTanhNear)) {
+#pragma unroll
+              for (uint32_t c = 0; c < NC; c++) s[c] = fmaf(-slope, fabsf(gap - (float)c), cap * kLog2e * tanh_(s[c] * pre));
+            } else {
+#pragma unroll
+              for (uint32_t c = 0; c < NC; c++) s[c] = fmaf(-slope, fabsf(gap - (float)c), cap * kLog2e * tanh_near(s[c] * pre));
+            }
+          } else {
+#pragma unroll
+            for (uint32_t c = 0; c < NC; c++) s[c] = fmaf(-slope, fabsf(gap - (float)c), s[c] * sl);
           }
         }
         if (k0 < wlo || k0 + (int32_t)NC > whi) {

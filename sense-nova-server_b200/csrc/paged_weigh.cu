@@ -564,6 +564,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 2)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(in_cta(&s_empty[buf], 0), false);
+      if (GENERAL && cap > 0.f) {  // mostly all scores are far below the cap, and need no exponentials
+        float most = 0.f;
+#pragma unroll
+        for (uint32_t c = 0; c < 32; c++) most = fmaxf(most, fabsf(s[c]));
+        if (__any_sync(0xffffffffu, most * fabsf(pre) >= kTanhNear)) {
+#pragma unroll
+          for (uint32_t c = 0; c < 32; c++) s[c] = cap * kLog2e * tanh_(s[c] * pre);
+        } else {
+#pragma unroll
+          for (uint32_t c = 0; c < 32; c++) s[c] = cap * kLog2e * tanh_near(s[c] * pre);
+        }
+      }
       float2 acc[2] = {{0.f, 0.f}, {0.f, 0.f}};
       const bool full = m.full;
 #pragma unroll
@@ -576,7 +588,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeighThreads, 2)
           const float ts[4] = {t.x, t.y, t.z, t.w}, ws[4] = {w.x, w.y, w.z, w.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float v = cap > 0.f ? cap * kLog2e * tanh_(s[c + e] * pre) : s[c + e] * sl;
+            const float v = cap > 0.f ? s[c + e] : s[c + e] * sl;
             s[c + e] = ex2(fmaf(-ws[e], fabsf(ts[e] - (float)key), v) - zs[e]);
           }
         } else {

@@ -696,3 +696,16 @@ def test_evict_very_long():
     """More candidates than the shared memory of eight CTAs holds keys of."""
     p = Problem([400000], [1], 1, 1, 128, 256, seed=29, weight=True, spare=20)
     check_evict(p, 5000, 4, 64, False)
+
+
+@pytest.mark.parametrize("cap", [20.0, 50.0, 1000.0])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("lens,rows", [([3] * 20, [1] * 20), ([9] * 6, [5] * 6), ([40] * 5, [40] * 5)])
+def test_attend_far_below_the_cap(lens, rows, d, cap):
+    """Scores that the cap hardly changes keep their 32 bits: a score is off by some 2^-22 of itself,
+    not of the cap (which at 50 is 1e-5), and so is the log-sum-exp of few keys."""
+    p = Problem(lens, rows, 8, 2, d, 16, seed=31, peak=0.3)
+    out, lse = run_attend(p, cap=cap)
+    _, z, _, _ = ref.attend(p, p.q, None, out_dtype=None, cap=cap)
+    s = float(p.q.double().norm(dim=-1).max() * p.k.nan_to_num(0).double().norm(dim=-1).max()) / math.sqrt(d)  # a bound on |s|
+    assert ((lse.double() - z).abs() <= 8 * 2.0**-23 * (1 + s + z.abs())).all()
