@@ -67,9 +67,10 @@ __device__ __forceinline__ void next_block(const WeighArgs& a, WeighWalk& w) {
 // The blocks of 64 keys of all (KV head, sequence) pairs form one line that is cut into equal
 // shares, one for each CTA. A warp takes 8 keys of each block through its own ring of TMA
 // boxes: S = Q K^T on m16n8k16 with the heads of two rows as the 16 rows, so a key's sum over
-// heads and rows is one over the lanes of its column. 8 tokens over up to 16384 keys: 36 us
-// (142 MB, 3.9 TB/s, 0.61 of a copy's rate: the chain of a group's steps, not the bytes;
-// 52 with one CTA an SM, 72 with products on the FMA units).
+// heads and rows is one over the lanes of its column; its old weights come with its keys. 8 tokens
+// over up to 16384 keys: 31 us (142 MB, 4.6 TB/s, 0.71 of a copy's rate: the chain of a group's
+// steps, about 2500 cycles, not the bytes; 35 with intervals and scale anew for each group, half as
+// much again with one CTA an SM, twice with products on the FMA units).
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32, WeighRowGeo<D>::kPerSm)
     weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ CUtensorMap kmap) {
