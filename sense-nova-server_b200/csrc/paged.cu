@@ -252,7 +252,7 @@ __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* sh, uint32
 // passes (weights crowd in few exponents: eight counts of each digit, by lane, on banks of
 // their own), then the kept slots in slot order, 4096 at a time. A thread takes four
 // neighbouring slots, which lie in one page. The weights are read once where their keys fit
-// shared memory. 32 lists of up to 16384 weights take 17 us by clusters of 4 (22 by one CTA each),
+// shared memory. 32 lists of up to 16384 weights take 16 us by clusters of 4 (22 by one CTA each),
 // the copy of their 4096 kept slots 43 us (269 MB in all).
 template <bool HELD, bool MANY>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictArgs a) {
