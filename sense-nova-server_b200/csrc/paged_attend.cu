@@ -87,11 +87,11 @@ constexpr float kRefSlack = 8.f;  // log2 that scores may exceed the reference b
 //
 // Bound by the products and the hand-over between them and the softmax: 2048 rows of 16 heads of
 // 256 over 8192 keys take 232 us called back to back (1040 TFLOP/s; 199 in a short burst), the
-// tensor pipe active 66% of the time and the card at its power limit (981 W, 1.79 of 1.965 GHz). 6 x up to 1000 rows of 32 heads of 128 under
-// a window, documents and a distance bias: 134 us; a tile of 64 keys takes 1970 cycles of a CTA, 1000
-// when the softmax warps do nothing, and 15 tiles a pair of CTAs leave a third of its time to the
-// start and the end (queries and tiles are on their way together, gates are loaded ahead of the
-// stores: 146 us without either).
+// tensor pipe active 66% of the time and the card at its power limit (981 W, 1.79 of 1.965
+// GHz). 6 x up to 1000 rows of 32 heads of 128 under a window, documents and a distance bias: 134
+// us; a tile of 64 keys takes 1970 cycles of a CTA, 1000 when the softmax warps do nothing, and 15
+// tiles a pair of CTAs leave a third of its time to the start and the end (queries and tiles are
+// on their way together, gates are loaded ahead of the stores: 146 us without either).
 template <typename T, int D, bool GENERAL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<D>::kPerSm)
     attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
