@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   const uint32_t cs = MANY ? a.cluster : 1, part = blockIdx.x % cs, kh = blockIdx.x / cs, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
   if (tid < 2) own_n[tid] = 0;
   if (tid == 0) s_digit = s_need = 0;
+  __syncthreads();  // set before any warp adds to them: where `take` is 0 no other barrier comes between
   pdl_wait();
   const int32_t len = paged_len(a.c, b), budget = (int32_t)a.p.budget;
   int32_t* kept = a.kept + ((uint64_t)b * a.c.n_kv + kh) * a.p.budget;

@@ -692,6 +692,28 @@ def test_evict_by_clusters(lens, budget, sink, recent, in_place):
     check_evict(p, budget, sink, recent, in_place)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n", [8195, 16384, 40001])
+@pytest.mark.parametrize("sink,recent", [(1000, 0), (0, 1000), (100, 4900)])
+def test_evict_without_a_choice_by_clusters(n, sink, recent, in_place):
+    """A budget of sink and recent slots alone leaves nothing to select: lists of 2, 4 and 8 CTAs."""
+    budget = sink + recent
+    p = Problem([n, 3000], [1, 1], 2, 2, 128, 16, seed=n, weight=True, spare=2 * -(-budget // 16))
+    check_evict(p, budget, sink, recent, in_place)
+
+
+@pytest.mark.parametrize("n", [8195, 16384, 40001])
+def test_evict_without_a_choice_every_time(n):
+    p = Problem([n], [1], 2, 2, 128, 16, seed=n, weight=True, spare=200)
+    cache, batch, lens = p.cache(paged), p.batch(paged), torch.empty_like(p.len_t)
+    into = torch.tensor([p.free[:188]], dtype=torch.int32, device="cuda")
+    want = torch.cat([torch.arange(1000), torch.arange(n - 2000, n)]).to(torch.int32).cuda()
+    kept = torch.full((100, 1, 2, 3000), 99, dtype=torch.int32, device="cuda")
+    for x in kept:
+        cache.evict(batch, 3000, x, into, lens, sink=1000, recent=2000)
+    assert (kept == want).all()
+
+
 def test_evict_very_long():
     """More candidates than the shared memory of eight CTAs holds keys of."""
     p = Problem([400000], [1], 1, 1, 128, 256, seed=29, weight=True, spare=20)
