@@ -311,7 +311,8 @@ typedef struct snl_paged_batch {
 } snl_paged_batch;
 
 /* The rotary table of snl_paged_append: table[pos][f] = (cos, sin) of pos *
- * theta^(-2f / rot_dim), f < rot_dim / 2, angles in 64 bits. table: [n_pos][rot_dim / 2][2]. */
+ * theta^(-2f / rot_dim), f < rot_dim / 2, angles in 64 bits. table: [n_pos][rot_dim / 2][2],
+ * aligned to 8 bytes. */
 int snl_rope_table(double theta, uint32_t rot_dim, uint32_t n_pos, float* table, void* stream);
 
 /* Which axis of a row's position (time, height, width) turns pair f. */

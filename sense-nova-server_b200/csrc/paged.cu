@@ -574,6 +574,7 @@ extern "C" int snl_rope_table(double theta, uint32_t rot_dim, uint32_t n_pos, fl
   if (!table) return fail(SNL_E_INVALID, "snl_rope_table: null argument");
   if (!(theta > 0) || rot_dim == 0 || rot_dim % 2 || rot_dim > 256)
     return fail(SNL_E_INVALID, "snl_rope_table: theta must be positive, rot_dim even and at most 256");
+  if (reinterpret_cast<uintptr_t>(table) & 7) return fail(SNL_E_INVALID, "snl_rope_table: table must be aligned to 8 bytes");
   const uint64_t n = (uint64_t)n_pos * (rot_dim / 2);
   if (n == 0) return SNL_OK;
   if (n > (1ull << 38)) return fail(SNL_E_UNSUPPORTED, "snl_rope_table: too many positions");

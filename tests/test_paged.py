@@ -145,3 +145,10 @@ def test_numbers_that_no_field_holds(lib):
     new = torch.zeros(3, 2, 256)
     for kw in (dict(axes=-1), dict(sections=(1 << 32, 0, 0)), dict(sections=(0, -1, 0)), dict(eps=1e39)):
         refused("SNL_E_INVALID", "append's numbers|eps must be finite", cache.append, batch, None, new, new, None, **kw)
+
+
+def test_rope_table_alignment(lib):
+    """Its pairs are written eight bytes at a time."""
+    table = torch.zeros(4 * 32 * 2 + 1)[1:].view(4, 32, 2)
+    assert table.data_ptr() % 8 == 4
+    refused("SNL_E_INVALID", "aligned to 8 bytes", paged.rope_table, table, 1e4)
