@@ -479,6 +479,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
                                   : (uint64_t)(w.row0 + tok) * a.p.out_row + (uint64_t)head * a.p.out_head;
     const uint64_t gate_at = (uint64_t)(w.row0 + tok) * a.p.gate_row + (uint64_t)head * a.p.gate_head;
     const uint32_t some_rows = __ballot_sync(0xffffffffu, valid && !(parts && nt == 0));
+    // A row without weights is 0 whatever its gate holds, which is not looked at.
+    const uint32_t gated_rows = __ballot_sync(0xffffffffu, valid && l != 0.f);
 #pragma unroll 1
     for (uint32_t c = wg * (D / 2); some_rows && c < (wg + 1) * (D / 2); c += 32) {
       uint32_t r[32];
@@ -524,7 +526,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
               const uint32_t row = (it + i) * 4 + lane / 8;
               const uint64_t from = __shfl_sync(0xffffffffu, gate_at, row) + c + lane % 8 * 4;
               g4[i] = make_uint4(0, 0, 0, 0);
-              if (!(some_rows >> row & 1)) continue;
+              if (!(gated_rows >> row & 1)) continue;
               if (a.p.gate_type == SNL_T_F32) {
                 g4[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.gate) + from));
               } else {
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant
   float g[E];
   if (a.gate) load_as_float<E>(a.gate, r * a.p.gate_row + h * a.p.gate_head + lane * E, a.p.gate_type, g);
 #pragma unroll
-  for (int i = 0; i < E; i++) o[i] *= a.gate ? inv * sigmoidf_(g[i]) : inv;
+  for (int i = 0; i < E; i++) o[i] = l == 0.f ? 0.f : o[i] * (a.gate ? inv * sigmoidf_(g[i]) : inv);
   store_from_float<E>(a.out, r * a.p.out_row + h * a.p.out_head + lane * E, a.p.out_type, o);
   if (a.lse && lane == 0) a.lse[item] = l == 0.f ? -INFINITY : (zero + log2f(l)) * (1.f / kLog2e);
 }

@@ -731,3 +731,33 @@ def test_attend_far_below_the_cap(lens, rows, d, cap):
     _, z, _, _ = ref.attend(p, p.q, None, out_dtype=None, cap=cap)
     s = float(p.q.double().norm(dim=-1).max() * p.k.nan_to_num(0).double().norm(dim=-1).max()) / math.sqrt(d)  # a bound on |s|
     assert ((lse.double() - z).abs() <= 8 * 2.0**-23 * (1 + s + z.abs())).all()
+
+
+# Kernels of attend: tiles in one part and in several, a row's cluster, equal shares.
+EACH_KERNEL = [([300, 150], [37, 50], {}), ([9000], [70], {}), ([300, 150, 77], [1, 1, 1], {}), ([300, 150, 2000], [1, 1, 1], WIDE)]
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("lens,rows,bounds", EACH_KERNEL)
+def test_attend_gate_of_rows_without_keys(lens, rows, bounds, d, bad):
+    """A padding row is 0 whatever its gate holds."""
+    p = Problem(lens, rows, 8, 2, d, seed=d, **bounds)
+    off = torch.arange(p.n, device="cuda") % 3 == 1
+    first = torch.where(off, 2**31 - 1, 0).to(torch.int32)
+    gate = p.normal(p.n, 8, d)
+    want, z = run_attend(p, gate=gate, out_dtype=F32, first=first)
+    gate[off] = bad
+    out, lse = run_attend(p, gate=gate, out_dtype=F32, first=first)
+    assert (out[off] == 0).all() and torch.isneginf(lse[off]).all()
+    assert torch.equal(out, want) and torch.equal(lse, z)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("lens,rows,bounds", EACH_KERNEL)
+def test_attend_gate_of_scores_of_minus_infinity(lens, rows, bounds, d):
+    p = Problem(lens, rows, 8, 2, d, seed=d, **bounds)
+    p.k[..., 0] = math.inf
+    p.q[..., 0] = -1
+    out, lse = run_attend(p, gate=torch.full((p.n, 8, d), math.nan, device="cuda"))
+    assert (out == 0).all() and torch.isneginf(lse).all()
