@@ -662,9 +662,9 @@ int go_weigh(const snl_paged_cache& c, const snl_paged_batch& b, const WeighArgs
                    (size_t)WeighRowGeo<D>::kSmem, s, a, km);
     return SNL_OK;
   }
-  CUtensorMap km, qm;
+  CUtensorMap km, qm{};  // no query is loaded for a batch without rows, and no map describes an empty tensor
   SNL_TRY(page_map(&km, c, c.k, 8, D / 64));
-  SNL_TRY(query_map(&qm, c, b, a.p, a.q, a.group, a.toks));
+  if (b.n_rows) SNL_TRY(query_map(&qm, c, b, a.p, a.q, a.group, a.toks));
   const uint64_t grid = 2ull * c.n_kv * b.n_seqs * ((a.c.max_len + 255) / 256);
   if (grid > 0x7fffffffull) return fail(SNL_E_UNSUPPORTED, "snl_paged_weigh: too many keys");
   static bool attr[2][64] = {};

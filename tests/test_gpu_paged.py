@@ -460,6 +460,14 @@ def test_weigh_long():
     check_weigh(Problem([3000, 2100], [700, 1], 8, 2, 256, 64, seed=22, weight=True), 0.9)
 
 
+@pytest.mark.parametrize("heads", [8, 9, 16, 40, 64])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("decay", [0.0, 0.5])
+def test_weigh_without_rows(heads, d, decay):
+    """The weights decay, whatever the number of heads to a KV head."""
+    check_weigh(Problem([150, 300, 0, 1], [0, 0, 0, 0], heads, 1, d, seed=heads, weight=True), decay)
+
+
 def test_weigh_sums_to_the_rows():
     """Every row hands out a weight of one per head."""
     p = Problem([700], [90], 8, 2, seed=14, weight=True)
