@@ -363,7 +363,8 @@ typedef struct snl_paged_attn_p {
  * h / (n_heads / n_kv). q has the cache's type, gate and out any. lse (or NULL):
  * [n_rows][n_heads] log-sum-exp of the scores. A row that sees no key (or only scores of
  * -inf) gives 0 and -inf. What a row does not see never reaches it, NaN and infinities
- * included. Single tokens, chunks and mixtures of both; long caches are split over the GPU
+ * included; pages before the first slot that a row of their sequence sees may be gone from
+ * the table. Single tokens, chunks and mixtures of both; long caches are split over the GPU
  * and joined in `work`, work_bytes of scratch (snl_paged_attend_workspace() of them, with
  * the same structs, suffice) that concurrent calls may not share. */
 int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch* b, const snl_paged_attn_p* p, const void* q,

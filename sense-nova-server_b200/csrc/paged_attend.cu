@@ -236,9 +236,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
   float l = 0.f, ref = -INFINITY;
   const uint32_t vrun = a.vrun;  // keys of a V box: 8 or 16
   if (warp == 8 || warp == 10) {
-    // Lane g loads the g-th run of keys of the tile (K: of this CTA's half). Keys past the
-    // length and pages outside the cache come from a page coordinate past the end, which reads
-    // zeros.
+    // Lane g loads the g-th run of keys of the tile (K: of this CTA's half). Runs of which no row
+    // sees a key, whose pages may be gone, and pages outside the cache come from a page coordinate
+    // past the end, which reads zeros.
     const bool is_k = warp == 8;
     const uint32_t run = is_k ? 8 : vrun, lanes = is_k ? KT / 16 : KT / vrun, key0 = (is_k ? rank * (KT / 2) : 0) + lane * run;
     const uint32_t NS = is_k ? NK : NV;
@@ -246,7 +246,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttendThreads, Geo<
     auto page_of = [&](uint32_t i) -> int32_t {
       const uint32_t key = (jl - i) * KT + key0;
       int32_t p = -1;
-      if (i < nt && lane < lanes && (int32_t)key < w.len) p = paged_page(a.c, w.b, key);
+      if (i < nt && lane < lanes && (int32_t)key < end && (int32_t)(key + run) > beg) p = paged_page(a.c, w.b, key);
       return p < 0 ? (int32_t)a.c.n_pages : p;
     };
     int32_t now = page_of(0), next = page_of(1);

@@ -262,6 +262,20 @@ def test_bad_indices_are_reported(lib):
     assert lib.snl_device_error(1) == 4 and torch.equal(got[20:], want[20:])
 
 
+@pytest.mark.parametrize("page", [8, 16, 128])
+@pytest.mark.parametrize("d,lens,rows", [(256, [1000, 700], [70, 3]), (128, [1000, 700], [70, 3]), (256, [9000], [40]),
+                                         (128, [1000, 700], [1, 1])])
+def test_attend_pages_that_no_row_sees(d, lens, rows, page):
+    """Pages wholly before every row's window may be gone from the table: nothing changes, nothing is reported."""
+    p = Problem(lens, rows, 8, 2, d, page, seed=page)
+    m = masks_of(p, window=90)
+    want, z = check_attend(p, **m)
+    for i, n in enumerate(lens):
+        p.table[i, :(n - rows[i] - 89) // page] = -1
+    out, lse = run_attend(p, **m)
+    assert torch.equal(out, want) and torch.equal(lse, z)
+
+
 @pytest.mark.parametrize("d,rows", [(128, 1), (256, 1), (128, 3), (256, 3)])
 def test_attend_many_sequences(d, rows):
     """More sequences than one look at 32 boundaries finds, lengths of every kind."""
