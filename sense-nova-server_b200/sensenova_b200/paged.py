@@ -25,6 +25,9 @@ _is_int: dict[Any, bool] = {}
 # structure of as many fields takes 1.4 us to make, most of what a small call costs here.
 _APPEND = struct.Struct("@9If8Q").pack
 _ATTN = struct.Struct("@3Q2I2f2I6Q").pack
+# snl_paged_batch and snl_paged_evict_p: a ctypes field would take a number's low 32 bits.
+_BATCH = struct.Struct("@3Q4I").pack
+_EVICT = struct.Struct("@4I").pack
 
 
 def _type(t) -> int:
@@ -75,8 +78,11 @@ class PagedBatch:
         seqs, width = table.shape
         self.tensors = (table, start, lens)
         self.n_seqs, self.n_rows, self.max_len = seqs, n_rows, max_len
-        self.c = PagedBatchC(_ints(table, "table", seqs, width), _ints(start, "start", seqs + 1),
-                             _ints(lens, "lens", seqs), seqs, n_rows, width, max_len)
+        try:
+            self.c = PagedBatchC.from_buffer_copy(_BATCH(_ints(table, "table", seqs, width), _ints(start, "start", seqs + 1),
+                                                         _ints(lens, "lens", seqs), seqs, n_rows, width, max_len))
+        except struct.error as e:
+            _fail(f"the batch's numbers: {e}")
         self.ref = C.byref(self.c)
 
 
@@ -201,12 +207,15 @@ class PagedCache:
         into [seqs, pages], or in place. kept [seqs, kv heads, budget] and new_lens [seqs]
         receive the kept slots and the lengths; in place new_lens defaults to the batch's."""
         seqs = batch.n_seqs
-        p = PagedEvictP(budget, sink, recent, 0)
-        ip = None
+        ip, width = None, 0
         if into is not None:
-            p.into_stride = into.shape[1]
-            ip = _ints(into, "into", seqs, into.shape[1])
+            width = into.shape[1]
+            ip = _ints(into, "into", seqs, width)
             _need(new_lens is not None, "new_lens is needed with new pages")
+        try:
+            p = PagedEvictP.from_buffer_copy(_EVICT(budget, sink, recent, width))
+        except struct.error as e:
+            _fail(f"evict's numbers: {e}")
         lp = batch.c.len if new_lens is None else _ints(new_lens, "new_lens", seqs)
         rc = self.lib.snl_paged_evict(self.ref, batch.ref, p, _ints(kept, "kept", seqs, self.n_kv, budget), ip,
                                       lp, stream)

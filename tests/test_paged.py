@@ -152,3 +152,14 @@ def test_rope_table_alignment(lib):
     table = torch.zeros(4 * 32 * 2 + 1)[1:].view(4, 32, 2)
     assert table.data_ptr() % 8 == 4
     refused("SNL_E_INVALID", "aligned to 8 bytes", paged.rope_table, table, 1e4)
+
+
+def test_numbers_that_no_field_of_batch_or_evict_holds(lib):
+    cache, batch, q = make()
+    kept = torch.zeros(1, 2, 8, dtype=torch.int32)
+    for kw in (dict(sink=(1 << 32) + 1), dict(recent=1 << 32), dict(sink=-1), dict(recent=1.5)):
+        refused("SNL_E_INVALID", "evict's numbers", cache.evict, batch, 8, kept, **kw)
+    for budget in ((1 << 32) + 8, -1, 8.0):
+        refused("SNL_E_INVALID", "evict's numbers", cache.evict, batch, budget, kept)
+    for rows, longest in ((3, (1 << 32) + 9), (3, -1), (3, 9.0), ((1 << 32) + 3, 9), (-1, 9), ("3", 9)):
+        refused("SNL_E_INVALID", "the batch's numbers", paged.PagedBatch, *batch.tensors, rows, longest)
