@@ -513,7 +513,8 @@ uint32_t log2_of(uint32_t v) {
 int paged_check(const char* what, const snl_paged_cache* c, const snl_paged_batch* b, PagedView* v) {
   const std::string w = what;
   if (!c || !b) return fail(SNL_E_INVALID, w + ": null argument");
-  if (!c->k || !c->v || !b->table || !b->start || !b->len) return fail(SNL_E_INVALID, w + ": null array");
+  // Without sequences the batch's arrays have no elements, and maybe no address.
+  if (!c->k || !c->v || (b->n_seqs && (!b->table || !b->start || !b->len))) return fail(SNL_E_INVALID, w + ": null array");
   if (c->type != SNL_T_F16 && c->type != SNL_T_BF16) return fail(SNL_E_UNSUPPORTED, w + ": the cache is f16 or bf16");
   if (c->head_dim != 128 && c->head_dim != 256) return fail(SNL_E_UNSUPPORTED, w + ": head_dim must be 128 or 256");
   if (c->page_size < 8 || (c->page_size & (c->page_size - 1)))
@@ -661,7 +662,7 @@ extern "C" int snl_paged_evict(const snl_paged_cache* c, const snl_paged_batch* 
   if (!paged_aligned(c->weight)) return fail(SNL_E_INVALID, w + ": the weights must be aligned to 16 bytes");
   if (p->budget == 0 || p->budget > (1u << 30) || (uint64_t)p->sink + p->recent > p->budget)
     return fail(SNL_E_INVALID, w + ": budget must be positive and hold sink + recent slots");
-  if (!kept || !new_len) return fail(SNL_E_INVALID, w + ": null argument");
+  if (b->n_seqs && (!kept || !new_len)) return fail(SNL_E_INVALID, w + ": null argument");
   if (into && (uint64_t)p->into_stride * c->page_size < std::min<uint64_t>(p->budget, (uint64_t)a.c.max_len))
     return fail(SNL_E_INVALID, w + ": the new pages do not hold the budget");
   if (b->n_seqs == 0) return SNL_OK;

@@ -163,3 +163,30 @@ def test_numbers_that_no_field_of_batch_or_evict_holds(lib):
         refused("SNL_E_INVALID", "evict's numbers", cache.evict, batch, budget, kept)
     for rows, longest in ((3, (1 << 32) + 9), (3, -1), (3, 9.0), ((1 << 32) + 3, 9), (-1, 9), ("3", 9)):
         refused("SNL_E_INVALID", "the batch's numbers", paged.PagedBatch, *batch.tensors, rows, longest)
+
+
+def test_batch_without_sequences(lib):
+    """Nothing to do is done, though tensors without elements have no address."""
+    cache, _, _ = make()
+    ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32)  # noqa: E731
+    batch = paged.PagedBatch(ints(0, 4), ints(1), ints(0), 0, 9)
+    q, k = torch.zeros(0, 8, 256, dtype=F16), torch.zeros(0, 2, 256, dtype=F16)
+    cache.append(batch, q, k, k, torch.zeros_like(q))
+    attend(cache, batch, q, lse=torch.zeros(0, 8))
+    cache.weigh(batch, q, torch.zeros(0, 8))
+    cache.evict(batch, 8, ints(0, 2, 8))
+    cache.evict(batch, 8, ints(0, 2, 8), ints(0, 1), ints(0))
+
+
+def test_tables_without_an_address(lib):
+    """A batch with sequences needs its arrays."""
+    cache, batch, q = make()
+    for field in ("table", "start", "len"):
+        b = ffi.PagedBatchC.from_buffer_copy(batch.c)
+        setattr(b, field, None)
+        rc = lib.snl_paged_weigh(cache.ref, C.byref(b), C.byref(ffi.PagedAttnP()), None, None, 1.0, None)
+        assert rc == -1 and b"null array" in lib.snl_last_error()
+    kept = torch.zeros(1, 2, 8, dtype=torch.int32)
+    p = ffi.PagedEvictP(8, 0, 0, 0)
+    for args in ((None, None, batch.c.len), (kept.data_ptr(), None, None)):
+        assert lib.snl_paged_evict(cache.ref, batch.ref, p, *args, None) == -1 and b"null argument" in lib.snl_last_error()
