@@ -180,6 +180,8 @@ class PagedCache:
         if gate is not None:
             gp, gate_row, gate_head = self._rows(gate, "gate", batch, heads)
             gate_type = _type(gate)
+        if not work.is_contiguous():  # its elements are counted below, which an expanded view does not hold
+            _fail("work must be contiguous")
         p = self._attn(batch, heads, scale, cap, window, slopes, first, last, gate_type, _type(out), q_row, q_head,
                        gate_row, gate_head, out_row, out_head)
         rc = self.lib.snl_paged_attend(self.ref, batch.ref, p, qp, gp, op,

@@ -190,3 +190,11 @@ def test_tables_without_an_address(lib):
     p = ffi.PagedEvictP(8, 0, 0, 0)
     for args in ((None, None, batch.c.len), (kept.data_ptr(), None, None)):
         assert lib.snl_paged_evict(cache.ref, batch.ref, p, *args, None) == -1 and b"null argument" in lib.snl_last_error()
+
+
+def test_scratch_that_is_not_there(lib):
+    """The bytes of a view count only where they lie together."""
+    cache, batch, q = make()
+    need = cache.attend_workspace(batch, 8)
+    for work in (torch.zeros(1, dtype=torch.uint8).expand(need), torch.zeros(2 * need, dtype=torch.uint8)[::2]):
+        refused("SNL_E_INVALID", "work must be contiguous", cache.attend, batch, q, torch.zeros_like(q), work)
