@@ -612,6 +612,8 @@ extern "C" int snl_paged_append(const snl_paged_cache* c, const snl_paged_batch*
       !paged_strides(p->in_type, p->k_row, p->k_head) || !paged_strides(p->in_type, p->v_row, p->v_head) ||
       !paged_strides(c->type, p->out_row, p->out_head) || (reinterpret_cast<uintptr_t>(rope) & 7))
     return fail(SNL_E_INVALID, w + ": rows must be aligned to 16 bytes");
+  if (paged_overlap(b->n_rows, p->out_row, p->n_heads ? c->head_dim : 0) || paged_overlap(p->n_heads, p->out_head, c->head_dim))
+    return fail(SNL_E_INVALID, w + ": the rows of q_out overlap");
   if (b->n_seqs == 0) return SNL_OK;
   a.p = *p;
   a.q = q;

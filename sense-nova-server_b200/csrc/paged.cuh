@@ -176,5 +176,7 @@ inline bool paged_strides(uint32_t type, uint64_t row, uint64_t head) {
   const uint64_t m = type == SNL_T_F32 ? 4 : 8;
   return row % m == 0 && head % m == 0;
 }
+// Rows or heads of an output that would be written over one another (an expanded view's).
+inline bool paged_overlap(uint64_t n, uint64_t stride, uint32_t head_dim) { return n > 1 && stride < head_dim; }
 
 }  // namespace snl

@@ -687,6 +687,8 @@ extern "C" int snl_paged_attend(const snl_paged_cache* c, const snl_paged_batch*
       !paged_strides(p->out_type, p->out_row, p->out_head) ||
       (gate && !paged_strides(p->gate_type, p->gate_row, p->gate_head)))
     return fail(SNL_E_INVALID, w + ": rows must be aligned to 16 bytes");
+  if (paged_overlap(b->n_rows, p->out_row, c->head_dim) || paged_overlap(p->n_heads, p->out_head, c->head_dim))
+    return fail(SNL_E_INVALID, w + ": the rows of out overlap");
   if (work_bytes < snl_paged_attend_workspace(c, b, p->n_heads)) return fail(SNL_E_INVALID, w + ": work is too small");
   if (!work) return fail(SNL_E_INVALID, w + ": null argument");
   if (b->n_rows == 0 || b->n_seqs == 0) return SNL_OK;

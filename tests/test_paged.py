@@ -198,3 +198,13 @@ def test_scratch_that_is_not_there(lib):
     need = cache.attend_workspace(batch, 8)
     for work in (torch.zeros(1, dtype=torch.uint8).expand(need), torch.zeros(2 * need, dtype=torch.uint8)[::2]):
         refused("SNL_E_INVALID", "work must be contiguous", cache.attend, batch, q, torch.zeros_like(q), work)
+
+
+def test_outputs_over_one_another(lib):
+    """Rows or heads of an output at one place would be written in no order."""
+    cache, batch, q = make()
+    new = torch.zeros(3, 2, 256, dtype=F16)
+    for view in (torch.zeros(1, 8, 256, dtype=F16).expand(3, 8, 256), torch.zeros(3, 1, 256, dtype=F16).expand(3, 8, 256),
+                 torch.zeros(8192, dtype=F16).as_strided((3, 8, 256), (2048, 128, 1))):
+        refused("SNL_E_INVALID", "out overlap", attend, cache, batch, q, out=view)
+        refused("SNL_E_INVALID", "q_out overlap", cache.append, batch, q, new, new, view)
