@@ -714,6 +714,33 @@ def test_evict_by_clusters(lens, budget, sink, recent, in_place):
     check_evict(p, budget, sink, recent, in_place)
 
 
+def test_evict_many_long_lists():
+    """More lists than clusters have room for, each of more candidates than one CTA holds keys of."""
+    kv, budget, lens = 4, 700, [50001 - 211 * i for i in range(40)]
+    p = Problem([50001], [1], kv, kv, 128, 256, seed=41, weight=True, spare=3 * 40)
+    p.weight.copy_((p.weight * 4000).floor())
+    cache = p.cache(paged)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    start = torch.zeros(41, dtype=torch.int32, device="cuda")
+    batch = paged.PagedBatch(p.table.expand(40, -1).contiguous(), start, lens_t, 0, 50001)  # pages that all sequences share
+    into = torch.tensor(p.free[:120], dtype=torch.int32, device="cuda").view(40, 3)
+    kept, new_lens = torch.empty(40, kv, budget, dtype=torch.int32, device="cuda"), torch.empty_like(lens_t)
+    w = p.keys(0, p.weight[..., None])[..., 0].float()  # [slot, kv]
+    k, v = p.keys(0, p.k).to(F16), p.keys(0, p.v).to(F16)
+    cache.evict(batch, budget, kept, into, new_lens, sink=3, recent=50)
+    assert (new_lens == budget).all()
+    at = torch.arange(budget, device="cuda")
+    for i, n in enumerate(lens):
+        order = torch.sort(w[3:n - 50], dim=0, descending=True, stable=True).indices[:budget - 53] + 3
+        must = torch.cat([torch.arange(3), torch.arange(n - 50, n)]).cuda()[:, None].expand(-1, kv)
+        want = torch.cat([must, order]).sort(0).values.T  # [kv, budget]
+        assert torch.equal(kept[i], want.int())
+        page = into[i, at // 256].long()
+        for h in range(kv):
+            for now, was in ((p.k, k), (p.v, v), (p.weight, w)):
+                assert torch.equal(now[page, h, at % 256], was[want[h], h])
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("n", [8195, 16384, 40001])
 @pytest.mark.parametrize("sink,recent", [(1000, 0), (0, 1000), (100, 4900)])
