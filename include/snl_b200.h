@@ -276,8 +276,9 @@ size_t snl_sample_scratch_bytes(void);
  *
  * All arrays are device memory. Calls enqueue on `stream`, allocate nothing, wait for
  * nothing and may be captured in a CUDA graph. Pointers and strides of q, k, v, gate, out
- * and the pages are aligned to 16 bytes; the last dimension is contiguous. The shapes, types
- * and host-side bounds are checked before anything is enqueued. What only the device can
+ * and the pages, and the addresses of weight, pos, the norms and work, are aligned to 16
+ * bytes; the last dimension is contiguous; rows and heads of outputs do not overlap. The shapes,
+ * types and host-side bounds are checked before anything is enqueued. What only the device can
  * see is bounded there: a page number outside the cache, a length over max_len or the
  * table's pages, a start array that leaves [0, n_rows], a position outside the rotary table. Such an
  * entry is not read or written, its results are undefined, and bit 2 (value 4) of
@@ -302,7 +303,9 @@ typedef struct snl_paged_cache {
 
 /* The step's rows: rows start[b] .. start[b + 1] - 1 are the newest tokens of sequence b,
  * which with them holds len[b] slots; row i of them is at slot len[b] - rows + i. table:
- * [n_seqs][table_stride] page numbers. max_len: at least every len[b]. */
+ * [n_seqs][table_stride] page numbers. max_len: at least every len[b]; grids and parts follow
+ * it, so a bound far above the lengths costs time. Kernels are chosen by the rows of a
+ * sequence on the average: a long chunk beside single tokens is faster in a batch of its own. */
 typedef struct snl_paged_batch {
   const int32_t* table;
   const int32_t* start; /* [n_seqs + 1], start[0] = 0, start[n_seqs] = n_rows */

@@ -166,7 +166,7 @@ __device__ __forceinline__ void store_from_float(void* p, uint64_t at, uint32_t 
     *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
 }
 
-// Host side: the checks that every call makes, and the launches of paged_attend.cu.
+// Host side: the checks that every call makes.
 int paged_check(const char* what, const snl_paged_cache* c, const snl_paged_batch* b, PagedView* v);
 int paged_check_attn(const char* what, const snl_paged_cache& c, const snl_paged_batch& b, const snl_paged_attn_p* p,
                      PagedMask* m);

@@ -107,7 +107,8 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) { return __uint_as_fl
 // A row that ends inside its CTA is written at once; pieces of rows cut by a share's end are
 // left to rows_join_kernel. A warp takes 8 keys of each block through its own ring of TMA
 // boxes: S = Q K^T on m16n8k16 (query heads as rows), O^T += V^T P^T on m16n8k8, whose B
-// operand is the score fragment as it stands.
+// operand is the score fragment as it stands: its weights are rounded to the cache's type (2^-11 or
+// 2^-8 of each, as V itself is), sums and output stay in 32 bits.
 //
 // Bound by memory: 16 tokens of 16 heads of 256 over up to 32768 keys 189 us (1.19 GB, 6.3
 // TB/s, 0.97 of a copy's rate; 243 with the tiles of attend_kernel), 64 of 32 heads of 128 over
@@ -537,6 +538,12 @@ int go_rows(const snl_paged_cache& c, const RowArgs& r, uint32_t grid, cudaStrea
 // (single rows 193 against 243), at 13 rows of 8 of up to 2048 keys 24 against 26, and 2 rows of
 // one 17 against 21; at head_dim 128 and 104 rows of 64 sequences of up to 4096 keys 129
 // against 161.
+//
+// Those rows were spread evenly. The host knows how many there are, not where: one sequence with
+// many of them beside single tokens passes too, and its keys are read once for each of its rows. 32
+// tokens over 512 keys of heads of 128 and 34 rows over 4096 take 113 us, in two calls 15 + 23; over
+// 32768 633, in two calls 15 + 60; at head_dim 256 32 tokens over 2048 keys and 9 rows over 8192 85,
+// in two calls 52 + 23. A caller that has both kinds gives them a batch each.
 bool attend_rows_fits(const snl_paged_cache& c, const snl_paged_batch& b, uint32_t group) {
   const uint64_t blocks = (uint64_t)b.n_rows * (b.max_len / kBlock + 2);
   const bool small = blocks * c.n_kv <= 8192, wide = c.head_dim == 256;
